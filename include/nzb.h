@@ -473,6 +473,134 @@ NZB_API int nzb_fill(float* data, float value, int64_t n, void* stream);
 NZB_API int nzb_expand(float* out, const float* in, int64_t per_batch, int64_t batches, void* stream);
 NZB_API int nzb_scale(float* data, float factor, int64_t n, void* stream);
 
+/* Token models --------------------------------------------------------------------------------
+ * Rows of a table, layer norm, log probabilities of tokens and the orthogonalised update: what a model of
+ * tokens needs next to Linear, the softmax head and Adam. NeuZephyr has no counterpart of these four. All of
+ * them compute in fp32 whatever the stored type, round once at the end, use no floating-point atomics (the
+ * same call gives the same bits) and only work on the arguments they are given, so calls on different streams
+ * and captured graphs share nothing. Strides ("ld") are in elements between the starts of two rows; the
+ * elements of a row are contiguous. Vectors of 16 bytes are used where a row's address allows; any address
+ * that is a multiple of the element's size is accepted.
+ */
+enum { NZB_F32 = 0, NZB_F16 = 1, NZB_BF16 = 2 };
+enum { NZB_I32 = 0, NZB_I64 = 1 };
+
+/*
+ * Embedding: y[t] = scale * table[index[t]] for `tokens` indices into a table {vocab, dim}. An index outside
+ * [0, vocab) reads nothing and gives a row of zeros.
+ *   dtype        of y and dy
+ *   table_dtype  of the table: dtype, or NZB_F32
+ * Backward: dtable[v] += scale * sum over t with index[t] == v of dy[t], in fp32 and in the order of t
+ * (pieces of at most 64 tokens, then the pieces), with overwrite != 0: dtable = ... and rows of tokens that
+ * do not occur are set to zero. Without it those rows are neither read nor written. Tokens equal to
+ * padding_index, or outside [0, vocab), contribute nothing (padding_index -1: none). ld_table is then the
+ * stride of dtable, whose type is fp32 always.
+ */
+typedef struct nzb_embedding_desc {
+    int64_t tokens, vocab, dim;
+    int64_t ld_table, ld_y;
+    int64_t padding_index;
+    float scale;
+    int32_t dtype, table_dtype, index_type;
+    int32_t overwrite;
+    int32_t reserved;
+} nzb_embedding_desc;
+
+NZB_API int nzb_embedding_forward(const nzb_embedding_desc* desc, const void* table, const void* index, void* y,
+                                  void* stream);
+NZB_API int nzb_embedding_backward_workspace_bytes(const nzb_embedding_desc* desc, size_t* bytes_out);
+NZB_API int nzb_embedding_backward(const nzb_embedding_desc* desc, const void* dy, const void* index, float* dtable,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Layer norm over the last dimension: mean and variance of each row (the variance from the centred row),
+ * rstd = 1 / sqrt(var + eps), y = (x - mean) * rstd * gamma + beta. gamma and beta (fp32, {dim}) may be null
+ * (1 and 0), mean and rstd (fp32, {rows}) may be null when nothing reads them. y may be x.
+ * Backward, with h = (x - mean) * rstd and g = dy * gamma:
+ *   dx (+)= rstd * (g - mean(g) - h * mean(g * h))     = with overwrite_dx, += without
+ *   dgamma (+)= sum over rows of dy * h, dbeta (+)= sum over rows of dy      = with overwrite_dparams
+ * Null outputs are skipped. dx may be dy. dtype is the type of x, y, dy and dx.
+ */
+typedef struct nzb_layernorm_desc {
+    int64_t rows, dim;
+    int64_t ld_x, ld_y;    /* ld_y: of y, and of dy in the backward pass */
+    int64_t ld_dx;
+    float eps;
+    int32_t dtype;
+    int32_t overwrite_dx, overwrite_dparams;
+} nzb_layernorm_desc;
+
+NZB_API int nzb_layernorm_forward(const nzb_layernorm_desc* desc, const void* x, const float* gamma,
+                                  const float* beta, void* y, float* mean, float* rstd, void* stream);
+NZB_API int nzb_layernorm_backward_workspace_bytes(const nzb_layernorm_desc* desc, size_t* bytes_out);
+NZB_API int nzb_layernorm_backward(const nzb_layernorm_desc* desc, const void* dy, const void* x, const float* mean,
+                                   const float* rstd, const float* gamma, void* dx, float* dgamma, float* dbeta,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of given tokens: with z = scale * logits (scale > 0, the inverse temperature) and
+ * lse = ln sum exp z over each row of `vocab` logits,
+ *   logprob[r] = z[target[r]] - lse, entropy[r] = -sum p ln p with p = exp(z - lse),
+ *   top_logprob / top_index {rows, top_k}: the top_k largest logits' log probabilities and columns, largest
+ *   first, equal ones by the lower column (top_k <= 32 and <= vocab).
+ * Any output may be null. Targets and top_index have the type index_type. A target outside [0, vocab) stands
+ * for a position without one: its logprob is 0. Logits of -inf (or of the type's lowest value) are masked:
+ * probability 0. A row without a z above -1e30 is empty: lse and its log probabilities are -inf, its entropy
+ * is 0. A NaN in a row makes the row's results NaN; it ranks last among the alternatives.
+ * Backward: dlogits = scale * (dlogprob * (1[target] - p) - dentropy * p * (ln p + entropy)), from lse and
+ * entropy of the forward pass; dlogprob or dentropy may be null (0), entropy too when dentropy is. Rows that
+ * are empty get zeros; positions without a target only the entropy's part. dlogits may be logits.
+ */
+typedef struct nzb_token_logprob_desc {
+    int64_t rows, vocab;
+    int64_t ld_logits, ld_dlogits;
+    float scale;
+    int32_t dtype, index_type;
+    int32_t top_k;
+} nzb_token_logprob_desc;
+
+NZB_API int nzb_token_logprob_forward(const nzb_token_logprob_desc* desc, const void* logits, const void* targets,
+                                      float* logprob, float* entropy, float* lse, float* top_logprob, void* top_index,
+                                      void* stream);
+NZB_API int nzb_token_logprob_backward(const nzb_token_logprob_desc* desc, const void* logits, const void* targets,
+                                       const float* lse, const float* entropy, const float* dlogprob,
+                                       const float* dentropy, void* dlogits, void* stream);
+
+/*
+ * Orthogonalised update: brings the singular values of each of `batch` matrices G {rows, cols} near 1 by
+ * `steps` Newton-Schulz products, X = G / (|G|_F + eps), then steps times
+ *   A = X X^T, B = coef[1] A + coef[2] A A, X = coef[0] X + B X      (rows <= cols; else with X^T X and X B).
+ * X is held in fp32; the tensor cores read fp16 copies of X, A and B (scaled by 2^12, fp32 sums), the diagonal
+ * of B is kept in fp32. Relative error of the result against 64 bits: about 1e-3 (2-norm), whatever out_dtype.
+ * Coefficients have to keep the singular values of X below 2.8, as (3.4445, -4.775, 2.0315) do. A matrix of
+ * zeros gives zeros.
+ */
+typedef struct nzb_orthogonalize_desc {
+    int64_t batch, rows, cols;
+    int64_t ld_g, stride_g;      /* between rows and between matrices */
+    int64_t ld_out, stride_out;
+    float coef[3];
+    float eps;
+    int32_t steps;               /* 1 .. 64 */
+    int32_t dtype, out_dtype;
+    int32_t reserved;
+} nzb_orthogonalize_desc;
+
+NZB_API int nzb_orthogonalize_workspace_bytes(const nzb_orthogonalize_desc* desc, size_t* bytes_out);
+NZB_API int nzb_orthogonalize(const nzb_orthogonalize_desc* desc, const void* g, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * One Muon step on a weight matrix (fp32, like nzb_adam): momentum = mu * momentum + grad, u = momentum or,
+ * with nesterov, grad + mu * momentum, w = (1 - lr * weight_decay) * w - lr * scale * orthogonalised(u).
+ * desc gives the matrix (batch, rows, cols, coefficients, steps, eps); its strides and types are not used:
+ * w, momentum and grad are contiguous.
+ */
+NZB_API int nzb_muon_workspace_bytes(const nzb_orthogonalize_desc* desc, size_t* bytes_out);
+NZB_API int nzb_muon(const nzb_orthogonalize_desc* desc, float* w, float* momentum, const float* grad, float lr,
+                     float scale, float mu, float weight_decay, int nesterov, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

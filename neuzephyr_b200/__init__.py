@@ -7,4 +7,6 @@ tests and benchmarks; it uses torch for device memory and streams, never for com
 from . import _capi  # noqa: F401
 from .ops import (gemm, gemm_host, gemm_f16, gemm_workspace_bytes, tensorcore_gemm, gemm_backward, matmul_f32, cast_f32_f16,  # noqa: F401
                   device_status, conv2d_forward, conv2d_backward_data, conv2d_backward_weight,
-                  conv2d_backward_bias, conv2d_backward, linear_forward, linear_backward)
+                  conv2d_backward_bias, conv2d_backward, linear_forward, linear_backward,
+                  embedding, embedding_backward, layernorm_forward, layernorm_backward, token_logprobs,
+                  token_logprobs_backward, TokenLogprobs, orthogonalize, muon_step)

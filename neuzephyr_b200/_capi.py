@@ -8,6 +8,8 @@ LIB_PATH = os.path.join(HERE, "libnzb.so")
 
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_DEVICE_TIMEOUT, ERR_NO_DEVICE = range(7)
 BIAS_NONE, BIAS_ROW, BIAS_COL, BIAS_MATRIX = range(4)
+F32, F16, BF16 = range(3)
+I32, I64 = range(2)
 STATIC_SCRATCH_BYTES = 32 << 20
 
 EXPORTS = [
@@ -21,6 +23,10 @@ EXPORTS = [
     "nzb_add_backward", "nzb_relu", "nzb_relu_backward", "nzb_avgpool", "nzb_avgpool_backward", "nzb_avgpool_backward_ex", "nzb_softmax",
     "nzb_softmax_backward", "nzb_bce", "nzb_bce_backward", "nzb_adam", "nzb_adam_multi", "nzb_softmax_bce_forward",
     "nzb_softmax_bce_backward", "nzb_maxpool", "nzb_maxpool_backward", "nzb_fill", "nzb_expand", "nzb_scale",
+    "nzb_embedding_forward", "nzb_embedding_backward_workspace_bytes", "nzb_embedding_backward",
+    "nzb_layernorm_forward", "nzb_layernorm_backward_workspace_bytes", "nzb_layernorm_backward",
+    "nzb_token_logprob_forward", "nzb_token_logprob_backward",
+    "nzb_orthogonalize_workspace_bytes", "nzb_orthogonalize", "nzb_muon_workspace_bytes", "nzb_muon",
 ]
 
 
@@ -49,6 +55,32 @@ class LinearDesc(ctypes.Structure):
     """struct nzb_linear_desc"""
     _fields_ = [("batch", ctypes.c_int64), ("in_features", ctypes.c_int64), ("out_features", ctypes.c_int64),
                 ("relu", ctypes.c_int32), ("overwrite_dx", ctypes.c_int32)]
+
+
+class EmbeddingDesc(ctypes.Structure):
+    """struct nzb_embedding_desc"""
+    _fields_ = [(n, ctypes.c_int64) for n in ("tokens", "vocab", "dim", "ld_table", "ld_y", "padding_index")] + \
+               [("scale", ctypes.c_float)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "table_dtype", "index_type", "overwrite", "reserved")]
+
+
+class LayernormDesc(ctypes.Structure):
+    """struct nzb_layernorm_desc"""
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "dim", "ld_x", "ld_y", "ld_dx")] + [("eps", ctypes.c_float)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "overwrite_dx", "overwrite_dparams")]
+
+
+class TokenLogprobDesc(ctypes.Structure):
+    """struct nzb_token_logprob_desc"""
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "vocab", "ld_logits", "ld_dlogits")] + \
+               [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("dtype", "index_type", "top_k")]
+
+
+class OrthogonalizeDesc(ctypes.Structure):
+    """struct nzb_orthogonalize_desc"""
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "rows", "cols", "ld_g", "stride_g", "ld_out", "stride_out")] + \
+               [("coef", ctypes.c_float * 3), ("eps", ctypes.c_float)] + \
+               [(n, ctypes.c_int32) for n in ("steps", "dtype", "out_dtype", "reserved")]
 
 
 class AdamTensor(ctypes.Structure):
@@ -131,6 +163,19 @@ def lib():
         L.nzb_fill.argtypes = [vp, f32, i64, vp]
         L.nzb_expand.argtypes = [vp, vp, i64, i64, vp]
         L.nzb_scale.argtypes = [vp, f32, i64, vp]
+        # descriptors of these go by address (ctypes.addressof / byref both convert)
+        L.nzb_embedding_forward.argtypes = [vp] * 5
+        L.nzb_embedding_backward_workspace_bytes.argtypes = [vp, ctypes.POINTER(sz)]
+        L.nzb_embedding_backward.argtypes = [vp, vp, vp, vp, vp, sz, vp]
+        L.nzb_layernorm_forward.argtypes = [vp] * 8
+        L.nzb_layernorm_backward_workspace_bytes.argtypes = [vp, ctypes.POINTER(sz)]
+        L.nzb_layernorm_backward.argtypes = [vp] * 10 + [sz, vp]
+        L.nzb_token_logprob_forward.argtypes = [vp] * 9
+        L.nzb_token_logprob_backward.argtypes = [vp] * 9
+        L.nzb_orthogonalize_workspace_bytes.argtypes = [vp, ctypes.POINTER(sz)]
+        L.nzb_orthogonalize.argtypes = [vp, vp, vp, vp, sz, vp]
+        L.nzb_muon_workspace_bytes.argtypes = [vp, ctypes.POINTER(sz)]
+        L.nzb_muon.argtypes = [vp, vp, vp, vp, f32, f32, f32, f32, ci, vp, sz, vp]
         _lib = L
     return _lib
 

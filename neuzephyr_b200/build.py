@@ -12,8 +12,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnzb.so")
-SOURCES = ["nzb_api.cu", "nzb_cast.cu", "nzb_gemm.cu", "nzb_static.cu", "nzb_selftest.cu", "nzb_matmul32.cu", "nzb_host_gemm.cu", "nzb_ops.cu", "nzb_train_ops.cu", "nzb_conv.cu", "nzb_conv_nhwc.cu", "nzb_linear.cu"]
-HEADERS = ["nzb_internal.h", "nzb_ptx.cuh", os.path.join("..", "..", "include", "nzb.h")]
+SOURCES = ["nzb_api.cu", "nzb_cast.cu", "nzb_gemm.cu", "nzb_static.cu", "nzb_selftest.cu", "nzb_matmul32.cu", "nzb_host_gemm.cu", "nzb_ops.cu", "nzb_train_ops.cu", "nzb_conv.cu", "nzb_conv_nhwc.cu", "nzb_linear.cu",
+           "nzb_embedding.cu", "nzb_layernorm.cu", "nzb_logprob.cu", "nzb_orthogonalize.cu"]
+HEADERS = ["nzb_internal.h", "nzb_ptx.cuh", "nzb_gemm_tile.cuh", "nzb_elem.cuh", os.path.join("..", "..", "include", "nzb.h")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared"] + os.environ.get("NZB_EXTRA_NVCC_FLAGS", "").split()

@@ -1,0 +1,124 @@
+// Element types of the token-model operators: 16-byte vectors of fp32 / fp16 / bf16 as floats, rows whose start
+// is no multiple of 16 bytes, warp and block sums.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace nzb {
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int VEC = 4;
+    static __device__ __forceinline__ float to(float v) { return v; }
+    static __device__ __forceinline__ float from(float v) { return v; }
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
+        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+template <>
+struct Elem<__half> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// A row of n elements seen as 16-byte blocks of memory: block v holds the elements v * VEC - lead ..
+// v * VEC - lead + VEC - 1, where `lead` is how many elements before the row share its first block. Blocks
+// that lie whole within the row are moved as one vector, the first and the last one element by element, so
+// nothing outside the row is touched.
+template <typename T>
+__device__ __forceinline__ int row_lead(const T* row) {
+    return static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_block(const T* row, int64_t first, int64_t n) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (first >= 0 && first + VEC <= n) return *reinterpret_cast<const uint4*>(row + first);
+    union { uint4 u; T e[VEC]; } b;
+    b.u = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < VEC; i++)
+        if (first + i >= 0 && first + i < n) b.e[i] = row[first + i];
+    return b.u;
+}
+template <typename T>
+__device__ __forceinline__ void store_block(T* row, int64_t first, int64_t n, const uint4& v) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (first >= 0 && first + VEC <= n) {
+        *reinterpret_cast<uint4*>(row + first) = v;
+        return;
+    }
+    union { uint4 u; T e[VEC]; } b;
+    b.u = v;
+#pragma unroll
+    for (int i = 0; i < VEC; i++)
+        if (first + i >= 0 && first + i < n) row[first + i] = b.e[i];
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Calls f with a null pointer of the element type that `dtype` names.
+#define NZB_DISPATCH_DTYPE(dtype, T, ...)                                             \
+    do {                                                                              \
+        if ((dtype) == NZB_F32) { using T = float; __VA_ARGS__; }                     \
+        else if ((dtype) == NZB_F16) { using T = __half; __VA_ARGS__; }               \
+        else { using T = __nv_bfloat16; __VA_ARGS__; }                                \
+    } while (0)
+
+inline bool known_dtype(int32_t t) { return t == 0 || t == 1 || t == 2; }
+inline int64_t dtype_size(int32_t t) { return t == 0 ? 4 : 2; }
+inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+}  // namespace nzb

@@ -1,0 +1,708 @@
+// Orthogonalised update of a weight matrix by Newton-Schulz products, and the Muon step that applies it. Beside
+// the Adam and SGD steps.
+//
+//   X = G / (|G|_F + eps); steps times: A = X X^T, B = c1 A + c2 A A, X = c0 X + B X      (rows <= cols)
+// and A = X^T X, X = c0 X + X B for a tall matrix: either operand of a product may be K-major or MN-major, so no
+// pass transposes anything. S is the short side, L the long one; a step costs 2 S^2 L + 2 S^3 + 2 S^2 L operations,
+// of which the symmetric A and B need one half each.
+//
+// Precision. The recurrence multiplies small singular values by c0 (3.4) a step, and with them whatever noise the
+// roundings put there, so X itself is held in fp32: X = (c0 + B_ii) X32 + (B - diag B) X16. Only the products'
+// operands are fp16 (rounding 2^-12 relative), stored times 2^12 so that entries down to 2^-26 keep all bits, and
+// B's diagonal, which carries most of B once X is near orthogonal, multiplies the fp32 X. Simulated against 64 bits
+// on full-rank, decaying and nearly low-rank matrices: 3e-4 .. 1e-3 for sides of 128 and more; with X rounded
+// to bf16 in every step 1e-2 .. 3e-1.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "nzb_elem.cuh"
+#include "nzb_gemm_tile.cuh"
+#include "nzb_internal.h"
+#include "nzb_ptx.cuh"
+
+namespace nzb {
+
+constexpr float kNsScale = 4096.f;            // 2^12: what the fp16 copies of X, A and B are multiplied by
+constexpr float kNsUnscale = 1.f / 4096.f;
+
+enum { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2 };
+enum { NS_OUT_STATE = 0, NS_OUT_F32 = 1, NS_OUT_F16 = 2, NS_OUT_BF16 = 3, NS_OUT_WEIGHT = 4 };
+
+struct NsParams {
+    int32_t M, N;              // output extents
+    int32_t k_blocks, last_ksteps;
+    int32_t tiles_m, tiles_n, group_m;
+    int32_t a_mn, b_mn;
+    int32_t by_column;         // NS_APPLY of a tall matrix: the diagonal belongs to the columns
+    int32_t out_kind, out_vec; // NS_APPLY
+    int64_t tiles, tiles_per_matrix;
+    float c0, c1, c2;
+    __half* out16;             // A, B or the next X, times 2^12
+    int64_t ld16, stride16;
+    const __half* gram;        // NS_POLY: A times 2^12, same layout as out16
+    float* diag;               // c0 + B_ii, `short_side` per matrix
+    int64_t short_side;
+    float* X32;
+    int64_t ldx, stridex;
+    void* out;                 // NS_APPLY, last step
+    int64_t ld_out, stride_out;
+    float w_keep, w_step;      // NS_OUT_WEIGHT: w = w_keep w - w_step x
+    int* status;
+};
+
+template <bool PAIR_>
+struct NsCfg {
+    static constexpr bool PAIR = PAIR_;
+    static constexpr int BM = 128;                    // rows per CTA
+    static constexpr int TILE = PAIR ? 256 : 128;     // the tile of a CTA, or of a pair, is square
+    static constexpr int STAGES = 6;
+    static constexpr int OPERAND_BYTES = 128 * 64 * 2;  // per CTA and operand: 128 rows x 64 k
+    static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+    static constexpr int EPI_STRIDE = 36;
+    static constexpr int EPI_BYTES = 4 * 32 * EPI_STRIDE * 4;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
+    static constexpr int TMEM_COLS = 2 * TILE;
+    static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB shared memory of an sm_100 CTA");
+};
+
+// Symmetric outputs: tile numbers run over the lower triangle, row of tiles by row of tiles.
+template <int MODE>
+__device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32_t& mt, int32_t& nt, int32_t& b) {
+    b = static_cast<int32_t>(tile / p.tiles_per_matrix);
+    const int32_t rem = static_cast<int32_t>(tile - b * p.tiles_per_matrix);
+    if (MODE == NS_APPLY) {
+        const int32_t group = p.group_m * p.tiles_n, g = rem / group, first = g * p.group_m;
+        const int32_t gm = min(p.tiles_m - first, p.group_m), within = rem - g * group;
+        mt = first + within % gm;
+        nt = within / gm;
+    } else {
+        int32_t m = static_cast<int32_t>((sqrtf(8.f * rem + 1.f) - 1.f) * 0.5f);
+        while (m * (m + 1) / 2 > rem) m--;
+        while ((m + 1) * (m + 2) / 2 <= rem) m++;
+        mt = m;
+        nt = rem - m * (m + 1) / 2;
+    }
+}
+
+// Drains a quarter (32 rows) of a finished A or B tile: every lane holds one row, 32 columns at a time. Writes
+// the fp16 entries and, off the diagonal tiles, their mirror image.
+template <class Cfg, int MODE>
+__device__ __forceinline__ void ns_drain_symmetric(const NsParams& p, uint32_t tmem, int lane, int32_t b, int32_t row0,
+                                                   int32_t col_tile, bool mirror) {
+    using namespace ptx;
+    __half* out = p.out16 + b * p.stride16;
+    const int32_t row = row0 + lane;
+    const bool row_ok = row < p.M;
+#pragma unroll 1
+    for (int c0 = 0; c0 < Cfg::TILE; c0 += 32) {
+        const int32_t col0 = col_tile + c0;
+        if (col0 >= p.N) break;  // warp-uniform; the padded leading dimension covers a started group of 32
+        uint32_t v[32];
+        tmem_ld_32x32(tmem + c0, v);
+        tmem_ld_wait();
+        __half2 h[16];
+        if (MODE == NS_GRAM) {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                h[j] = __floats2half2_rn(__uint_as_float(v[2 * j]) * kNsUnscale, __uint_as_float(v[2 * j + 1]) * kNsUnscale);
+        } else {
+            uint4 g[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                g[j] = row_ok ? *reinterpret_cast<const uint4*>(p.gram + b * p.stride16 + static_cast<int64_t>(row) * p.ld16 + col0 + 8 * j)
+                              : make_uint4(0, 0, 0, 0);
+            const __half2* gh = reinterpret_cast<const __half2*>(g);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float2 a = __half22float2(gh[j]);
+                // 2^12 B
+                const float x = p.c1 * a.x + p.c2 * (__uint_as_float(v[2 * j]) * kNsUnscale);
+                const float y = p.c1 * a.y + p.c2 * (__uint_as_float(v[2 * j + 1]) * kNsUnscale);
+                const int32_t c = col0 + 2 * j;
+                if (row_ok && (row == c || row == c + 1))
+                    p.diag[b * p.short_side + row] = p.c0 + (row == c ? x : y) * kNsUnscale;
+                h[j] = __floats2half2_rn(row == c ? 0.f : x, row == c + 1 ? 0.f : y);
+            }
+        }
+        if (row_ok) {
+            uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * p.ld16 + col0);
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(h);
+#pragma unroll
+            for (int j = 0; j < 4; j++) to[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
+        if (mirror) {
+            // entry (row, col) to (col, row): the lanes' rows are neighbours there. Two lanes trade halves so that
+            // each writes a pair of rows: the even lane of column 2j, the odd one of column 2j + 1.
+            const int32_t pair_row = row0 + (lane & ~1);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const __half give = lane & 1 ? __low2half(h[j]) : __high2half(h[j]);
+                const __half got = __ushort_as_half(__shfl_xor_sync(0xffffffffu, __half_as_ushort(give), 1));
+                const __half2 two = lane & 1 ? __halves2half2(got, __high2half(h[j])) : __halves2half2(__low2half(h[j]), got);
+                const int32_t c = col0 + 2 * j + (lane & 1);
+                if (c < p.N && pair_row < p.M) *reinterpret_cast<__half2*>(out + static_cast<int64_t>(c) * p.ld16 + pair_row) = two;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void ns_put_half4(__half* at, const float4& x) {
+    const __half2 lo = __floats2half2_rn(x.x, x.y), hi = __floats2half2_rn(x.z, x.w);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t*>(&lo);
+    u.y = *reinterpret_cast<const uint32_t*>(&hi);
+    *reinterpret_cast<uint2*>(at) = u;
+}
+template <typename T>
+__device__ __forceinline__ void ns_put4(T* at, const float4& x, int n, bool vec) {
+    const float f[4] = {x.x, x.y, x.z, x.w};
+    if (vec && n >= 4) {
+        union { T e[4]; uint2 two; uint4 four; } u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) u.e[i] = Elem<T>::from(f[i]);
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(at) = u.four;
+        else *reinterpret_cast<uint2*>(at) = u.two;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < n) at[i] = Elem<T>::from(f[i]);
+}
+
+// Drains a quarter of a finished B X tile through shared memory, so that eight lanes share 128 bytes of a row of
+// X32, and completes the step: x = diag * x + product, or the result's element.
+template <class Cfg>
+__device__ __forceinline__ void ns_drain_apply(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b,
+                                               int32_t row0, int32_t col_tile) {
+    using namespace ptx;
+    const float* diag = p.diag + b * p.short_side;
+#pragma unroll 1
+    for (int c0 = 0; c0 < Cfg::TILE; c0 += 32) {
+        const int32_t col0 = col_tile + c0;
+        if (col0 >= p.N) break;  // warp-uniform
+        uint32_t v[32];
+        tmem_ld_32x32(tmem + c0, v);
+        tmem_ld_wait();
+        float4* dst = reinterpret_cast<float4*>(stage + lane * Cfg::EPI_STRIDE);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                                 __uint_as_float(v[4 * j + 3]));
+        __syncwarp();
+        const int cl = (lane & 7) * 4;
+        const int32_t gc = col0 + cl;
+        float4 dc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.by_column) {
+            dc.x = gc < p.N ? diag[gc] : 0.f;
+            dc.y = gc + 1 < p.N ? diag[gc + 1] : 0.f;
+            dc.z = gc + 2 < p.N ? diag[gc + 2] : 0.f;
+            dc.w = gc + 3 < p.N ? diag[gc + 3] : 0.f;
+        }
+#pragma unroll
+        for (int rr = 0; rr < 32; rr += 4) {
+            const int r = rr + (lane >> 3);
+            const int32_t gr = row0 + r;
+            if (gr < p.M && gc < p.N) {
+                float4 x = *reinterpret_cast<const float4*>(stage + r * Cfg::EPI_STRIDE + cl);
+                float* xp = p.X32 + b * p.stridex + static_cast<int64_t>(gr) * p.ldx + gc;
+                const float4 o = *reinterpret_cast<const float4*>(xp);
+                if (!p.by_column) dc.x = dc.y = dc.z = dc.w = diag[gr];
+                constexpr float k = kNsUnscale * kNsUnscale;
+                x.x = fmaf(dc.x, o.x, x.x * k);
+                x.y = fmaf(dc.y, o.y, x.y * k);
+                x.z = fmaf(dc.z, o.z, x.z * k);
+                x.w = fmaf(dc.w, o.w, x.w * k);
+                if (p.out_kind == NS_OUT_STATE) {
+                    *reinterpret_cast<float4*>(xp) = x;  // the padded row holds whole groups of four
+                    x.x *= kNsScale; x.y *= kNsScale; x.z *= kNsScale; x.w *= kNsScale;
+                    ns_put_half4(p.out16 + b * p.stride16 + static_cast<int64_t>(gr) * p.ld16 + gc, x);
+                } else {
+                    const int64_t at = b * p.stride_out + static_cast<int64_t>(gr) * p.ld_out + gc;
+                    const int n = p.N - gc;
+                    if (p.out_kind == NS_OUT_F32) {
+                        ns_put4(static_cast<float*>(p.out) + at, x, n, p.out_vec);
+                    } else if (p.out_kind == NS_OUT_F16) {
+                        ns_put4(static_cast<__half*>(p.out) + at, x, n, p.out_vec);
+                    } else if (p.out_kind == NS_OUT_BF16) {
+                        ns_put4(static_cast<__nv_bfloat16*>(p.out) + at, x, n, p.out_vec);
+                    } else {
+                        float* w = static_cast<float*>(p.out) + at;
+                        const float f[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (i < n) w[i] = fmaf(-p.w_step, f[i], p.w_keep * w[i]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// One product of all matrices. CTA layout (192 threads, persistent over the tiles): warp 0 TMA producer, warp 1
+// tensor-memory allocator and MMA issuer, warps 2-5 epilogue; two accumulators, so that a tile's epilogue runs
+// under the next tile's products. PAIR: two CTAs share a 256 x 256 tile (each loads its 128 rows of both operands).
+// Every wait is bounded; on expiry the CTA raises its abort flag, waits for its copies in flight, frees its tensor
+// memory and returns with NZB_ERR_DEVICE_TIMEOUT in the status word.
+template <class Cfg, int MODE>
+__global__ void __launch_bounds__(192, 1)
+ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsParams p) {
+    using namespace ptx;
+    constexpr bool PAIR = Cfg::PAIR;
+    constexpr int STAGES = Cfg::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* epi = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::EPI_BYTES);
+    uint64_t* full = bars;
+    uint64_t* empty = bars + STAGES;
+    uint64_t* tfull = bars + 2 * STAGES;
+    uint64_t* tempty = bars + 2 * STAGES + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+    const int64_t first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], PAIR ? 8 : 4);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        if constexpr (PAIR) {
+            tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    if constexpr (PAIR) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int64_t tile = first_tile; tile < p.tiles && ok; tile += step) {
+            int32_t mt, nt, b;
+            ns_decode<MODE>(p, tile, mt, nt, b);
+            const int32_t row_a = mt * Cfg::TILE + (int32_t)rank * 128, row_b = nt * Cfg::TILE + (int32_t)rank * 128;
+            for (int32_t kb = 0; kb < p.k_blocks; kb++, it++) {
+                const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+                if (!mbar_wait_warp(&empty[s], ph ^ 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                if (elect_one()) {
+                    uint8_t* sa = smem + s * Cfg::STAGE_BYTES;
+                    if constexpr (PAIR) {
+                        const uint32_t leader_full = map_to_cta(smem_u32(&full[s]), 0);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
+                        load_operand_pair<128>(sa, &tmA, p.a_mn, kb * 64, row_a, b, leader_full);
+                        load_operand_pair<128>(sa + Cfg::OPERAND_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, leader_full);
+                    } else {
+                        mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
+                        load_operand<128>(sa, &tmA, p.a_mn, kb * 64, row_a, b, &full[s]);
+                        load_operand<128>(sa + Cfg::OPERAND_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, &full[s]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok && rank == 0 && lane == 0) {
+            // wait (bounded) for the copies still in flight so none lands after exit
+            const uint32_t first = it > (uint32_t)STAGES ? it - STAGES : 0;
+            const long long t0 = clock64();
+            for (uint32_t j = first; j < it; j++) {
+                while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1)) {
+                    if (clock64() - t0 > kWaitCycleLimit) break;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t idesc = make_idesc_f16_f32(Cfg::TILE, Cfg::TILE) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
+            const uint64_t hi_a = desc_high_bits(p.a_mn), hi_b = desc_high_bits(p.b_mn);
+            const uint32_t ka = desc_kstep(p.a_mn), kb_step = desc_kstep(p.b_mn);
+            uint32_t it = 0, tcount = 0;
+            bool ok = true;
+            for (int64_t tile = first_tile; tile < p.tiles && ok; tile += step, tcount++) {
+                const uint32_t acc = tcount & 1, aph = (tcount >> 1) & 1;
+                if (!mbar_wait_warp(&tempty[acc], aph ^ 1, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * Cfg::TILE;
+                for (int32_t kb = 0; kb < p.k_blocks; kb++, it++) {
+                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+                    if (!mbar_wait_warp(&full[s], ph, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + s * Cfg::STAGE_BYTES);
+                    const uint64_t da = hi_a | ((sa & 0x3ffff) >> 4);
+                    const uint64_t db = hi_b | (((sa + Cfg::OPERAND_BYTES) & 0x3ffff) >> 4);
+                    const int32_t ksteps = kb == p.k_blocks - 1 ? p.last_ksteps : 4;
+                    if (elect_one()) {
+                        if constexpr (PAIR) {
+                            mma_f16_ss_pair(d_tmem, da, db, idesc, kb > 0 ? 1u : 0u);
+                            if (ksteps > 1) mma_f16_ss_pair(d_tmem, da + ka, db + kb_step, idesc, 1u);
+                            if (ksteps > 2) mma_f16_ss_pair(d_tmem, da + 2 * ka, db + 2 * kb_step, idesc, 1u);
+                            if (ksteps > 3) mma_f16_ss_pair(d_tmem, da + 3 * ka, db + 3 * kb_step, idesc, 1u);
+                            mma_commit_pair(&empty[s]);
+                        } else {
+                            mma_f16_ss(d_tmem, da, db, idesc, kb > 0 ? 1u : 0u);
+                            if (ksteps > 1) mma_f16_ss(d_tmem, da + ka, db + kb_step, idesc, 1u);
+                            if (ksteps > 2) mma_f16_ss(d_tmem, da + 2 * ka, db + 2 * kb_step, idesc, 1u);
+                            if (ksteps > 3) mma_f16_ss(d_tmem, da + 3 * ka, db + 3 * kb_step, idesc, 1u);
+                            mma_commit(&empty[s]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one()) {
+                    if constexpr (PAIR) mma_commit_pair(&tfull[acc]);
+                    else mma_commit(&tfull[acc]);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        float* stage = epi + (warp - 2) * 32 * Cfg::EPI_STRIDE;
+        uint32_t tcount = 0;
+        for (int64_t tile = first_tile; tile < p.tiles; tile += step, tcount++) {
+            int32_t mt, nt, b;
+            ns_decode<MODE>(p, tile, mt, nt, b);
+            const uint32_t acc = tcount & 1, aph = (tcount >> 1) & 1;
+            if (!mbar_wait_bounded(&tfull[acc], aph, abort_flag)) break;
+            __syncwarp();
+            tc_fence_after();
+            const int32_t row0 = mt * Cfg::TILE + (int32_t)rank * 128 + q * 32;
+            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::TILE;
+            if constexpr (MODE == NS_APPLY) ns_drain_apply<Cfg>(p, tmem, stage, lane, b, row0, nt * Cfg::TILE);
+            else ns_drain_symmetric<Cfg, MODE>(p, tmem, lane, b, row0, nt * Cfg::TILE, mt != nt);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty[acc]), 0));
+                else mbar_arrive(&tempty[acc]);
+            }
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    if constexpr (PAIR) cluster_sync_all();
+    else __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) {
+        *p.status = NZB_ERR_DEVICE_TIMEOUT;
+        __threadfence_system();
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        if constexpr (PAIR) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+        else tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    }
+}
+
+// ---- Frobenius norm and first state ---------------------------------------------------------------------------
+constexpr int kNormParts = 256;  // partial sums per matrix
+
+// Sums of squares in 64 bits (fp32 squares leave the range from 1.8e19 on). For the Muon step the pass also updates
+// the momentum and leaves the matrix to orthogonalise in X32.
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(256)
+ns_norm_kernel(const T* __restrict__ g, float* __restrict__ momentum, float* __restrict__ X32, double* __restrict__ partial,
+               int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float mu, int nesterov) {
+    __shared__ double buf[8];
+    const int64_t b = blockIdx.y, n = rows * cols;
+    const T* from = g + b * stride_g;
+    double sum = 0.0;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / cols, c = i - r * cols;
+        float v = Elem<T>::to(from[r * ld_g + c]);
+        if (MUON) {
+            float* m = momentum + b * n + i;
+            const float moved = fmaf(mu, *m, v);
+            *m = moved;
+            v = nesterov ? fmaf(mu, moved, v) : moved;
+            X32[(b * rows + r) * ldx + c] = v;
+        }
+        sum += static_cast<double>(v) * v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; w++) sum += buf[w];
+        partial[b * kNormParts + blockIdx.x] = sum;
+    }
+}
+
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(256)
+ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __restrict__ X16, const double* __restrict__ partial,
+                int parts, int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float eps) {
+    __shared__ double buf[8];
+    const int64_t b = blockIdx.y, n = rows * cols;
+    double sum = threadIdx.x < parts ? partial[b * kNormParts + threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < 8; w++) sum += buf[w];
+    const float div = static_cast<float>(sqrt(sum) + eps);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / cols, c = i - r * cols, at = (b * rows + r) * ldx + c;
+        const float x = (MUON ? X32[at] : Elem<T>::to(g[b * stride_g + r * ld_g + c])) / div;
+        X32[at] = x;
+        X16[at] = __float2half_rn(x * kNsScale);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------
+struct NsPlan {
+    bool tall;
+    int64_t S, L, ldx, lda;
+    size_t x32, x16, gram, diag, norm;
+    size_t total() const { return x32 + 2 * x16 + 2 * gram + diag + norm; }
+};
+
+static int plan_ns(const nzb_orthogonalize_desc* d, NsPlan* pl) {
+    if (!d) return fail(NZB_ERR_BAD_ARG, "descriptor is null");
+    if (d->batch < 0 || d->rows < 0 || d->cols < 0) return fail(NZB_ERR_BAD_ARG, "negative extent");
+    if (d->batch > 65535 || d->rows > (1 << 24) || d->cols > (1 << 24)) return fail(NZB_ERR_UNSUPPORTED, "batch at most 65535, sides at most 2^24");
+    if (d->steps < 1 || d->steps > 64) return fail(NZB_ERR_BAD_ARG, "steps must be in [1, 64]");
+    if (!(d->eps >= 0.f)) return fail(NZB_ERR_BAD_ARG, "eps is negative or NaN");
+    pl->tall = d->rows > d->cols;
+    pl->S = pl->tall ? d->cols : d->rows;
+    pl->L = pl->tall ? d->rows : d->cols;
+    if (pl->S > (1 << 20)) return fail(NZB_ERR_UNSUPPORTED, "the short side is at most 2^20");
+    pl->ldx = round_up(d->cols > 0 ? d->cols : 1, kOperandKAlign);
+    pl->lda = round_up(pl->S > 0 ? pl->S : 1, kOperandKAlign);
+    pl->x32 = (size_t)round_up(d->batch * d->rows * pl->ldx * 4, 256);
+    pl->x16 = (size_t)round_up(d->batch * d->rows * pl->ldx * 2, 256);
+    pl->gram = (size_t)round_up(d->batch * pl->S * pl->lda * 2, 256);
+    pl->diag = (size_t)round_up(d->batch * pl->S * 4, 256);
+    pl->norm = (size_t)(d->batch * kNormParts * 8);
+    return NZB_OK;
+}
+
+template <class Cfg, int MODE>
+static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, NsParams& p, int64_t batch, const DeviceState& ds,
+                          cudaStream_t s) {
+    static std::atomic<uint64_t> smem_set{0};
+    const auto kernel = ns_product_kernel<Cfg, MODE>;
+    int rc = ensure_dynamic_smem(smem_set, reinterpret_cast<const void*>(kernel), Cfg::SMEM_BYTES);
+    if (rc != NZB_OK) return rc;
+    p.tiles_m = (p.M + Cfg::TILE - 1) / Cfg::TILE;
+    p.tiles_n = (p.N + Cfg::TILE - 1) / Cfg::TILE;
+    p.group_m = 8;
+    p.tiles_per_matrix = MODE == NS_APPLY ? (int64_t)p.tiles_m * p.tiles_n : (int64_t)p.tiles_m * (p.tiles_m + 1) / 2;
+    p.tiles = p.tiles_per_matrix * batch;
+    int64_t workers = Cfg::PAIR ? ds.sm_count / 2 : ds.sm_count;
+    if (p.tiles < workers) workers = p.tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(Cfg::PAIR ? 2 * workers : workers));
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = Cfg::PAIR ? 2 : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, p));
+    return NZB_OK;
+}
+
+// A product's operand of the whole batch: `rows` x `cols` halves, the contraction along the row or down the rows.
+static int operand(CUtensorMap* map, const __half* base, bool mn, int64_t rows, int64_t cols, int64_t ld, int64_t batch) {
+    return mn ? make_operand_map_mn(map, base, rows, cols, ld, batch) : make_operand_map(map, base, cols, ld, rows, batch, 128);
+}
+
+struct NsTarget {
+    int kind;
+    void* out;
+    int64_t ld, stride;
+    float w_keep, w_step;
+};
+
+static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws, const NsTarget& target, const DeviceState& ds,
+                  cudaStream_t s) {
+    float* X32 = reinterpret_cast<float*>(ws);
+    __half* X16[2] = {reinterpret_cast<__half*>(ws + pl.x32), reinterpret_cast<__half*>(ws + pl.x32 + pl.x16)};
+    __half* A16 = reinterpret_cast<__half*>(ws + pl.x32 + 2 * pl.x16);
+    __half* B16 = reinterpret_cast<__half*>(ws + pl.x32 + 2 * pl.x16 + pl.gram);
+    float* diag = reinterpret_cast<float*>(ws + pl.x32 + 2 * pl.x16 + 2 * pl.gram);
+    CUtensorMap x_k[2], x_mn[2], gram_k, poly_k;
+    int rc;
+    for (int i = 0; i < 2; i++) {
+        if ((rc = operand(&x_k[i], X16[i], false, d->rows, d->cols, pl.ldx, d->batch)) != NZB_OK) return rc;
+        if ((rc = operand(&x_mn[i], X16[i], true, d->rows, d->cols, pl.ldx, d->batch)) != NZB_OK) return rc;
+    }
+    if ((rc = operand(&gram_k, A16, false, pl.S, pl.S, pl.lda, d->batch)) != NZB_OK) return rc;
+    if ((rc = operand(&poly_k, B16, false, pl.S, pl.S, pl.lda, d->batch)) != NZB_OK) return rc;
+    const auto contraction = [](NsParams& p, int64_t k) {
+        p.k_blocks = (int32_t)((k + 63) / 64);
+        p.last_ksteps = (int32_t)((k - (int64_t)(p.k_blocks - 1) * 64 + 15) / 16);
+    };
+    for (int step = 0; step < d->steps; step++) {
+        const int cur = step & 1;
+        NsParams p{};
+        p.c0 = d->coef[0]; p.c1 = d->coef[1]; p.c2 = d->coef[2];
+        p.diag = diag;
+        p.short_side = pl.S;
+        p.status = ds.status_dev;
+        // A = X X^T, or X^T X of a tall matrix
+        p.M = p.N = (int32_t)pl.S;
+        contraction(p, pl.L);
+        p.a_mn = p.b_mn = pl.tall;
+        p.out16 = A16;
+        p.ld16 = pl.lda;
+        p.stride16 = pl.S * pl.lda;
+        const CUtensorMap& x = pl.tall ? x_mn[cur] : x_k[cur];
+        rc = launch_product<NsCfg<false>, NS_GRAM>(x, x, p, d->batch, ds, s);
+        if (rc != NZB_OK) return rc;
+        // B = c1 A + c2 A A; A is symmetric, so both operands are read along its rows
+        contraction(p, pl.S);
+        p.a_mn = p.b_mn = 0;
+        p.out16 = B16;
+        p.gram = A16;
+        rc = launch_product<NsCfg<false>, NS_POLY>(gram_k, gram_k, p, d->batch, ds, s);
+        if (rc != NZB_OK) return rc;
+        // X = c0 X + B X, or c0 X + X B
+        p.M = (int32_t)d->rows;
+        p.N = (int32_t)d->cols;
+        p.by_column = pl.tall;
+        p.b_mn = !pl.tall;
+        p.out16 = X16[cur ^ 1];
+        p.ld16 = p.ldx = pl.ldx;
+        p.stride16 = p.stridex = d->rows * pl.ldx;
+        p.X32 = X32;
+        if (step == d->steps - 1) {
+            const int64_t size = target.kind == NS_OUT_F16 || target.kind == NS_OUT_BF16 ? 2 : 4;
+            p.out_kind = target.kind;
+            p.out = target.out;
+            p.ld_out = target.ld;
+            p.stride_out = target.stride;
+            p.out_vec = aligned_to(target.out, 4 * size) && target.ld % 4 == 0 && target.stride % 4 == 0;
+            p.w_keep = target.w_keep;
+            p.w_step = target.w_step;
+        }
+        rc = launch_product<NsCfg<false>, NS_APPLY>(pl.tall ? x_k[cur] : poly_k, pl.tall ? poly_k : x_mn[cur], p, d->batch, ds, s);
+        if (rc != NZB_OK) return rc;
+    }
+    return NZB_OK;
+}
+
+static int check_ws(const NsPlan& pl, const void* ws, size_t bytes) {
+    if (!ws || bytes < pl.total()) return fail(NZB_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", pl.total(), ws ? bytes : (size_t)0);
+    if (!aligned_to(ws, 256)) return fail(NZB_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    return NZB_OK;
+}
+
+// CTAs of the two elementwise passes: at least eight elements per thread.
+static unsigned elementwise_ctas(int64_t n, int64_t most) {
+    int64_t ctas = (n + 2047) / 2048;
+    return (unsigned)(ctas < 1 ? 1 : ctas > most ? most : ctas);
+}
+
+}  // namespace nzb
+
+using namespace nzb;
+
+extern "C" {
+
+int nzb_orthogonalize_workspace_bytes(const nzb_orthogonalize_desc* d, size_t* bytes_out) {
+    if (!bytes_out) return fail(NZB_ERR_BAD_ARG, "bytes_out is null");
+    NsPlan pl;
+    int rc = plan_ns(d, &pl);
+    if (rc != NZB_OK) return rc;
+    *bytes_out = pl.total();
+    return NZB_OK;
+}
+
+int nzb_orthogonalize(const nzb_orthogonalize_desc* d, const void* g, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+    NsPlan pl;
+    int rc = plan_ns(d, &pl);
+    if (rc != NZB_OK) return rc;
+    if (!known_dtype(d->dtype) || !known_dtype(d->out_dtype)) return fail(NZB_ERR_BAD_ARG, "unknown element type");
+    if (d->ld_g < d->cols || d->ld_out < d->cols) return fail(NZB_ERR_BAD_ARG, "leading dimension smaller than the row length");
+    if (d->batch == 0 || d->rows == 0 || d->cols == 0) return NZB_OK;
+    if (!g || !out) return fail(NZB_ERR_BAD_ARG, "g and out must be non-null");
+    if (!aligned_to(g, dtype_size(d->dtype)) || !aligned_to(out, dtype_size(d->out_dtype)))
+        return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
+    rc = check_ws(pl, workspace, workspace_bytes);
+    if (rc != NZB_OK) return rc;
+    DeviceState* ds;
+    rc = get_device_state(&ds);
+    if (rc != NZB_OK) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    float* X32 = reinterpret_cast<float*>(ws);
+    __half* X16 = reinterpret_cast<__half*>(ws + pl.x32);
+    double* partial = reinterpret_cast<double*>(ws + pl.total() - pl.norm);
+    const int64_t n = d->rows * d->cols;
+    const unsigned parts = elementwise_ctas(n, kNormParts);
+    NZB_DISPATCH_DTYPE(d->dtype, T, {
+        const T* from = static_cast<const T*>(g);
+        ns_norm_kernel<T, false><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(from, nullptr, nullptr, partial, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, 0.f, 0);
+        ns_start_kernel<T, false><<<dim3(elementwise_ctas(n, 2048), (unsigned)d->batch), 256, 0, s>>>(from, X32, X16, partial, (int)parts, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, d->eps);
+    });
+    NZB_CUDA_TRY(cudaGetLastError());
+    const int kind = d->out_dtype == NZB_F32 ? NS_OUT_F32 : d->out_dtype == NZB_F16 ? NS_OUT_F16 : NS_OUT_BF16;
+    return run_ns(d, pl, ws, NsTarget{kind, out, d->ld_out, d->stride_out, 0.f, 0.f}, *ds, s);
+}
+
+int nzb_muon_workspace_bytes(const nzb_orthogonalize_desc* d, size_t* bytes_out) {
+    return nzb_orthogonalize_workspace_bytes(d, bytes_out);
+}
+
+int nzb_muon(const nzb_orthogonalize_desc* d, float* w, float* momentum, const float* grad, float lr, float scale, float mu,
+             float weight_decay, int nesterov, void* workspace, size_t workspace_bytes, void* stream) {
+    NsPlan pl;
+    int rc = plan_ns(d, &pl);
+    if (rc != NZB_OK) return rc;
+    if (d->batch == 0 || d->rows == 0 || d->cols == 0) return NZB_OK;
+    if (!w || !momentum || !grad) return fail(NZB_ERR_BAD_ARG, "w, momentum and grad must be non-null");
+    if (!aligned_to(w, 4) || !aligned_to(momentum, 4) || !aligned_to(grad, 4))
+        return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
+    rc = check_ws(pl, workspace, workspace_bytes);
+    if (rc != NZB_OK) return rc;
+    DeviceState* ds;
+    rc = get_device_state(&ds);
+    if (rc != NZB_OK) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    float* X32 = reinterpret_cast<float*>(ws);
+    __half* X16 = reinterpret_cast<__half*>(ws + pl.x32);
+    double* partial = reinterpret_cast<double*>(ws + pl.total() - pl.norm);
+    const int64_t n = d->rows * d->cols;
+    const unsigned parts = elementwise_ctas(n, kNormParts);
+    ns_norm_kernel<float, true><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(grad, momentum, X32, partial, d->rows, d->cols, d->cols, n, pl.ldx, mu, nesterov);
+    ns_start_kernel<float, true><<<dim3(elementwise_ctas(n, 2048), (unsigned)d->batch), 256, 0, s>>>(nullptr, X32, X16, partial, (int)parts, d->rows, d->cols, 0, 0, pl.ldx, d->eps);
+    NZB_CUDA_TRY(cudaGetLastError());
+    return run_ns(d, pl, ws, NsTarget{NS_OUT_WEIGHT, w, d->cols, n, 1.f - lr * weight_decay, lr * scale}, *ds, s);
+}
+
+}  // extern "C"
