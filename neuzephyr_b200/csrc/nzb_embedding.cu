@@ -3,12 +3,14 @@
 //
 // Backward: dW[v] = scale * sum_{t: id_t = v} dy[t]. Atomics would add in an order that changes from run to run,
 // so the tokens are sorted first (stable, by token number) and every row is summed in the order of t:
-//   1. one CTA per tile of 16384 tokens sorts the tile in shared memory (radix, up to 9 bits a pass; the items
-//      wait in registers between passes, so one copy of the keys is enough) and cuts the runs of equal tokens
-//      into pieces of at most 64;
-//   2. one warp per piece and 32 vectors of columns sums the piece's rows; a run of one piece goes straight to
-//      the table, the pieces of a longer one to the workspace;
-//   3. the pieces of the longer runs are added in order.
+//   1. the tokens that occur are marked in a bit map;
+//   2. one CTA per tile of 16384 tokens sorts the tile in shared memory (radix, up to 9 bits a pass; the items
+//      wait in registers between passes, so one copy of the keys is enough), while the other SMs clear the
+//      rows of the tokens that do not occur: most of the bytes, and nothing they need from the sort;
+//   3. the sorted tokens are cut into chunks of 32, whatever runs of equal tokens they hold: one warp per chunk and
+//      32 vectors of columns. A run inside a chunk goes straight to the table, what crosses a chunk's border
+//      to the workspace, so a token that makes up a tenth of the text costs no more than any other;
+//   4. the parts of the runs that cross are added in order.
 // Tiles after the first add to the rows the earlier ones wrote, in launch order: the same bits every time.
 #include "nzb_internal.h"
 #include "nzb_elem.cuh"
@@ -19,18 +21,14 @@ constexpr int kSortTile = 16384;
 constexpr int kSortThreads = 1024;
 constexpr int kSortItems = kSortTile / kSortThreads;
 constexpr int kSortMaxBins = 512;
-constexpr int kPiece = 64;                                  // tokens summed by one warp
-constexpr int kMaxSlots = 2 * (kSortTile / kPiece);         // pieces of runs longer than kPiece, per tile
+constexpr int kChunk = 32;                                  // sorted tokens per warp of the sums
+constexpr int kEmbeddingFly = 4;                            // blocks in flight per thread, forward
 
 // What the sort leaves for the sums, per tile.
 struct SortTile {
-    int32_t pieces, runs;                 // runs: those of more than one piece
-    int32_t order[kSortTile];             // token positions within the tile, sorted
-    int32_t piece_start[kSortTile + 1];
-    int32_t piece_key[kSortTile];
-    int32_t piece_slot[kSortTile];        // partial sum's row, or -1: the piece is a whole run
-    int32_t run_key[kSortTile / kPiece + 1];
-    int32_t run_slot[kSortTile / kPiece + 2];  // first partial row; the next run's start is its end
+    int32_t count, pad[3];       // tokens that take part
+    uint32_t key[kSortTile];     // their numbers, sorted
+    int32_t order[kSortTile];    // their positions within the tile
 };
 
 struct SortSmem {
@@ -39,8 +37,6 @@ struct SortSmem {
     uint32_t bin_base[kSortMaxBins];
     uint16_t pos[kSortTile];
     int32_t scan[32];
-    int32_t scan2[32];
-    int32_t scan3[32];
 };
 
 __device__ __forceinline__ int32_t warp_inclusive_sum(int32_t v, int lane) {
@@ -51,22 +47,46 @@ __device__ __forceinline__ int32_t warp_inclusive_sum(int32_t v, int lane) {
     }
     return v;
 }
-__device__ __forceinline__ int32_t warp_inclusive_max(int32_t v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v = max(v, u);
+template <typename Index>
+__device__ __forceinline__ uint32_t sort_key(Index index, int64_t vocab, int64_t padding) {
+    const int64_t v = static_cast<int64_t>(index);
+    return v >= 0 && v < vocab && v != padding ? static_cast<uint32_t>(v) : static_cast<uint32_t>(vocab);
+}
+
+template <typename Index>
+__global__ void __launch_bounds__(256)
+embedding_mark_kernel(const Index* __restrict__ index, int64_t tokens, int64_t vocab, int64_t padding, uint32_t* __restrict__ present) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (t >= tokens) return;
+    const uint32_t v = sort_key(index[t], vocab, padding);
+    if (v != vocab) atomicOr(present + (v >> 5), 1u << (v & 31));
+}
+
+// Clears the rows whose bit is not set: a warp per row.
+__device__ __forceinline__ void clear_rows(const uint32_t* present, float* dtable, int64_t vocab, int64_t dim, int64_t ld_table,
+                                           int64_t warp, int64_t warps, int lane) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int64_t v = warp; v < vocab; v += warps) {
+        if (present[v >> 5] >> (v & 31) & 1) continue;
+        float* row = dtable + v * ld_table;
+        const int lead = row_lead(row);
+        for (int64_t c = lane * 4 - lead; c < dim; c += 128) store_block(row, c, dim, zero);
     }
-    return v;
 }
 
 template <typename Index>
 __global__ void __launch_bounds__(kSortThreads, 1)
 embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t vocab, int64_t padding, int digit_bits,
-                      int passes, SortTile* __restrict__ out_tiles, uint32_t* __restrict__ present) {
+                      int passes, int tiles, SortTile* __restrict__ out_tiles, const uint32_t* __restrict__ present,
+                      float* __restrict__ dtable, int64_t dim, int64_t ld_table) {
     extern __shared__ uint4 smem_sort[];
     SortSmem& s = *reinterpret_cast<SortSmem*>(smem_sort);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (blockIdx.x >= tiles) {
+        clear_rows(present, dtable, vocab, dim, ld_table, static_cast<int64_t>(blockIdx.x - tiles) * 32 + warp,
+                   static_cast<int64_t>(gridDim.x - tiles) * 32, lane);
+        return;
+    }
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kSortTile;
     const int count = static_cast<int>(min(static_cast<int64_t>(kSortTile), tokens - t0));
     SortTile& out = out_tiles[blockIdx.x];
@@ -77,15 +97,7 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
 #pragma unroll
     for (int i = 0; i < kSortItems; i++) {
         const int at = warp * (kSortTile / 32) + i * 32 + lane;
-        uint32_t key = none;
-        if (at < count) {
-            const int64_t v = static_cast<int64_t>(index[t0 + at]);
-            if (v >= 0 && v < vocab && v != padding) {
-                key = static_cast<uint32_t>(v);
-                if (blockIdx.x == 0) atomicOr(present + (key >> 5), 1u << (key & 31));
-            }
-        }
-        k[i] = key;
+        k[i] = at < count ? sort_key(index[t0 + at], vocab, padding) : none;
         p[i] = static_cast<uint16_t>(at);
     }
 
@@ -99,7 +111,13 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
 #pragma unroll
         for (int i = 0; i < kSortItems; i++) {
             const uint32_t d = (k[i] >> shift) & mask;
-            const uint32_t peers = __match_any_sync(0xffffffffu, d);
+            // lanes with the same digit: a ballot per bit (a match instruction takes a turn per different value,
+            // which made the pass over the low bits 15 us instead of 4)
+            uint32_t peers = 0xffffffffu;
+            for (int bit = 0; bit < digit_bits; bit++) {
+                const uint32_t set = __ballot_sync(0xffffffffu, d >> bit & 1);
+                peers &= d >> bit & 1 ? set : ~set;
+            }
             const int leader = __ffs(peers) - 1;
             uint32_t before = 0;
             if (lane == leader) {
@@ -146,82 +164,10 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
             __syncthreads();
         }
     }
-    for (int i = tid; i < count; i += kSortThreads) out.order[i] = s.pos[i];
-
-    // runs of equal tokens and their pieces: every thread looks at kSortItems neighbours
-    const int i0 = tid * kSortItems;
-    int32_t last_head = -1;
-#pragma unroll
-    for (int i = 0; i < kSortItems; i++) {
-        const int at = i0 + i;
-        if (at == 0 || s.key[at] != s.key[at - 1]) last_head = at;
-    }
-    const int32_t head_incl = warp_inclusive_max(last_head, lane);
-    if (lane == 31) s.scan[warp] = head_incl;
-    __syncthreads();
-    if (warp == 0) s.scan[lane] = warp_inclusive_max(s.scan[lane], lane);
-    __syncthreads();
-    int32_t head = __shfl_up_sync(0xffffffffu, head_incl, 1);
-    if (lane == 0) head = -1;
-    if (warp > 0) head = max(head, s.scan[warp - 1]);
-    const int32_t head0 = head;
-    int32_t n_piece = 0, n_slot = 0, n_run = 0;
-#pragma unroll
-    for (int i = 0; i < kSortItems; i++) {
-        const int at = i0 + i;
-        if (at == 0 || s.key[at] != s.key[at - 1]) head = at;
-        if (s.key[at] != none && (at - head) % kPiece == 0) {
-            n_piece++;
-            if (head + kPiece < kSortTile && s.key[head + kPiece] == s.key[at]) {
-                n_slot++;
-                if (at == head) n_run++;
-            }
-        }
-    }
-    const int32_t ip = warp_inclusive_sum(n_piece, lane), is = warp_inclusive_sum(n_slot, lane), ir = warp_inclusive_sum(n_run, lane);
-    __syncthreads();
-    if (lane == 31) {
-        s.scan[warp] = ip;
-        s.scan2[warp] = is;
-        s.scan3[warp] = ir;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        s.scan[lane] = warp_inclusive_sum(s.scan[lane], lane);
-        s.scan2[lane] = warp_inclusive_sum(s.scan2[lane], lane);
-        s.scan3[lane] = warp_inclusive_sum(s.scan3[lane], lane);
-    }
-    __syncthreads();
-    int32_t piece = ip - n_piece + (warp > 0 ? s.scan[warp - 1] : 0);
-    int32_t slot = is - n_slot + (warp > 0 ? s.scan2[warp - 1] : 0);
-    int32_t run = ir - n_run + (warp > 0 ? s.scan3[warp - 1] : 0);
-    head = head0;
-#pragma unroll
-    for (int i = 0; i < kSortItems; i++) {
-        const int at = i0 + i;
-        if (at == 0 || s.key[at] != s.key[at - 1]) {
-            if (s.key[at] == none) out.piece_start[piece] = at;  // end of the last piece: one thread gets here
-            head = at;
-        }
-        if (s.key[at] != none && (at - head) % kPiece == 0) {
-            const bool longer = head + kPiece < kSortTile && s.key[head + kPiece] == s.key[at];
-            out.piece_start[piece] = at;
-            out.piece_key[piece] = static_cast<int32_t>(s.key[at]);
-            out.piece_slot[piece] = longer ? slot : -1;
-            if (longer && at == head) {
-                out.run_key[run] = static_cast<int32_t>(s.key[at]);
-                out.run_slot[run] = slot;
-                run++;
-            }
-            if (longer) slot++;
-            piece++;
-        }
-    }
-    if (tid == kSortThreads - 1) {
-        out.pieces = piece;
-        out.runs = run;
-        out.run_slot[run] = slot;
-        if (s.key[kSortTile - 1] != none) out.piece_start[piece] = kSortTile;
+    for (int i = tid; i < kSortTile; i += kSortThreads) {
+        out.key[i] = s.key[i];
+        out.order[i] = s.pos[i];
+        if (s.key[i] == none ? i == 0 || s.key[i - 1] != none : i == kSortTile - 1) out.count = s.key[i] == none ? i : kSortTile;
     }
 }
 
@@ -248,111 +194,176 @@ __device__ __forceinline__ void put_columns(float* row, int64_t c, int64_t dim, 
 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
-embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile, const uint32_t* __restrict__ present,
-                     float* __restrict__ dtable, float* __restrict__ partial, int64_t vocab, int64_t dim, int64_t ld_table,
-                     int64_t ld_y, float scale, int add, int zero_rest, int vec_out) {
-    constexpr int VEC = Elem<T>::VEC;
+embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile, float* __restrict__ dtable,
+                     float* __restrict__ partial, int64_t dim, int64_t ld_table, int64_t ld_y, float scale, int add, int vec_out) {
+    constexpr int VEC = Elem<T>::VEC, FLY = 8;  // FLY: rows of dy in flight
     const int lane = threadIdx.x & 31;
-    const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int64_t warps = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
+    const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     const int64_t blocks = (dim + 32 * VEC - 1) / (32 * VEC);  // column blocks of a row
-    const int64_t items = tile->pieces * blocks;
-    for (int64_t item = warp; item < items; item += warps) {
-        const int64_t piece = item / blocks, c0 = (item - piece * blocks) * 32 * VEC;
-        const int i0 = tile->piece_start[piece], i1 = tile->piece_start[piece + 1];
-        const int slot = tile->piece_slot[piece];
-        float acc[VEC];
+    const int64_t chunk = item / blocks, c0 = (item - chunk * blocks) * 32 * VEC;
+    const int count = tile->count, i0 = static_cast<int>(chunk) * kChunk;
+    if (i0 >= count) return;
+    const int i1 = min(i0 + kChunk, count);
+    const uint32_t none = 0xffffffffu;
+    const uint32_t my_key = i0 + lane < i1 ? tile->key[i0 + lane] : none;
+    const int32_t my_row = i0 + lane < i1 ? tile->order[i0 + lane] : 0;
+    const uint32_t key_before = i0 > 0 ? tile->key[i0 - 1] : none, key_after = i1 < count ? tile->key[i1] : none;
+    const int64_t c = ALIGNED ? c0 + lane * VEC : c0 + lane;
+    float acc[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) acc[i] = 0.f;
-        const int64_t c = ALIGNED ? c0 + lane * VEC : c0 + lane;
-        for (int i = i0; i < i1; i++) {
-            const T* row = dy + static_cast<int64_t>(tile->order[i]) * ld_y;
-            if (ALIGNED) {
-                float f[VEC];
-                if (c < dim) {
-                    Elem<T>::unpack(load_block(row, c, dim), f);
+    for (int j = 0; j < VEC; j++) acc[j] = 0.f;
+    for (int g = 0; g < i1 - i0; g += FLY) {
+        uint4 u[FLY];
+        T e[FLY][ALIGNED ? 1 : VEC];
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) acc[j] += f[j];
+        for (int f = 0; f < FLY; f++) {
+            const T* row = dy + static_cast<int64_t>(__shfl_sync(0xffffffffu, my_row, g + f)) * ld_y;
+            u[f] = make_uint4(0, 0, 0, 0);
+            if (g + f < i1 - i0) {
+                if (ALIGNED) {
+                    if (c < dim) u[f] = load_block(row, c, dim);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) e[f][ALIGNED ? 0 : j] = c + j * 32 < dim ? row[c + j * 32] : Elem<T>::from(0.f);
                 }
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < FLY; f++) {
+            const int i = g + f;
+            if (i >= i1 - i0) break;
+            float v[VEC];
+            if (ALIGNED) {
+                Elem<T>::unpack(u[f], v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) v[j] = Elem<T>::to(e[f][ALIGNED ? 0 : j]);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; j++) acc[j] += v[j];
+            const uint32_t key = __shfl_sync(0xffffffffu, my_key, i);
+            const bool last = i + 1 == i1 - i0;
+            const uint32_t next = last ? key_after : __shfl_sync(0xffffffffu, my_key, i + 1);
+            if (next == key && !last) continue;
+            // the run ends here, or goes on in the next chunk
+            const uint32_t first_key = __shfl_sync(0xffffffffu, my_key, 0);
+            const bool from_before = key == first_key && key == key_before;
+            const bool whole = !from_before && next != key;
+            float* to = whole ? dtable + static_cast<int64_t>(key) * ld_table : partial + (2 * chunk + (from_before ? 0 : 1)) * dim;
+            if (whole) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) acc[j] *= scale;
+            }
+            if (ALIGNED) {
+                if (c < dim) put_columns<VEC>(to, c, dim, acc, whole && add, whole ? vec_out : dim % 4 == 0);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; j++)
-                    if (c + j * 32 < dim) acc[j] += Elem<T>::to(row[c + j * 32]);
+                    if (c + j * 32 < dim) to[c + j * 32] = whole && add ? to[c + j * 32] + acc[j] : acc[j];
             }
-        }
-        const bool whole = slot < 0;
-        float* to = whole ? dtable + static_cast<int64_t>(tile->piece_key[piece]) * ld_table : partial + static_cast<int64_t>(slot) * dim;
-        if (whole) {
 #pragma unroll
-            for (int j = 0; j < VEC; j++) acc[j] *= scale;
+            for (int j = 0; j < VEC; j++) acc[j] = 0.f;
         }
-        if (ALIGNED) {
-            if (c < dim) put_columns<VEC>(to, c, dim, acc, whole && add, whole ? vec_out : dim % 4 == 0);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if (c + j * 32 < dim) to[c + j * 32] = whole && add ? to[c + j * 32] + acc[j] : acc[j];
-        }
-    }
-    if (!zero_rest) return;
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t v = warp; v < vocab; v += warps) {
-        if (present[v >> 5] >> (v & 31) & 1) continue;
-        float* row = dtable + v * ld_table;
-        for (int64_t c = lane * 4; c < dim; c += 128) put_columns<4>(row, c, dim, zero, false, vec_out);
     }
 }
 
+// Runs over more than one chunk: the warp of the chunk such a run starts in adds its parts, 32 columns x 4.
 __global__ void __launch_bounds__(256)
 embedding_join_kernel(const SortTile* __restrict__ tile, const float* __restrict__ partial, float* __restrict__ dtable,
                       int64_t dim, int64_t ld_table, float scale, int add) {
-    const int runs = tile->runs;
-    const int64_t blocks = (dim + 255) / 256;
-    for (int64_t item = blockIdx.x; item < runs * blocks; item += gridDim.x) {
-        const int64_t run = item / blocks;
-        const int64_t c = (item - run * blocks) * 256 + threadIdx.x;
-        if (c >= dim) continue;
-        const int s0 = tile->run_slot[run], s1 = tile->run_slot[run + 1];
-        float acc = 0.f;
-        for (int s = s0; s < s1; s++) acc += partial[static_cast<int64_t>(s) * dim + c];
-        float* to = dtable + static_cast<int64_t>(tile->run_key[run]) * ld_table + c;
-        *to = add ? *to + scale * acc : scale * acc;
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    const int64_t blocks = (dim + 127) / 128;
+    const int64_t chunk = item / blocks;
+    const int count = tile->count, i0 = static_cast<int>(chunk) * kChunk, i1 = i0 + kChunk;
+    if (i1 >= count) return;
+    const uint32_t key = tile->key[i1 - 1];
+    if (tile->key[i1] != key || (i0 > 0 && tile->key[i0 - 1] == key)) return;
+    // parts in the chunks behind: one, and one more for every border the run crosses
+    int parts = 1;
+    for (int i = i1 + kChunk;; i += 32 * kChunk) {
+        const int at = i + lane * kChunk;
+        const uint32_t ends = __ballot_sync(0xffffffffu, at >= count || tile->key[at] != key);
+        parts += ends ? __ffs(ends) - 1 : 32;
+        if (ends) break;
     }
+    const int64_t c = (item - chunk * blocks) * 128 + lane;
+    float acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[j] = c + j * 32 < dim ? partial[(2 * chunk + 1) * dim + c + j * 32] : 0.f;
+#pragma unroll 4
+    for (int k = 1; k <= parts; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (c + j * 32 < dim) acc[j] += partial[2 * (chunk + k) * dim + c + j * 32];
+    float* to = dtable + static_cast<int64_t>(key) * ld_table + c;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (c + j * 32 < dim) to[j * 32] = add ? to[j * 32] + scale * acc[j] : scale * acc[j];
 }
 
-// One 16-byte block of y per item, a few items per thread for loads in flight. ALIGNED: all rows of the table
-// and of y start on 16 bytes; otherwise an item is one element.
-template <typename Tab, typename Out, typename Index, bool ALIGNED>
+// An item is one 16-byte block of y, or one element where a row of the table or of y does not start on 16 bytes. A
+// thread takes FLY of them a CTA's width apart, all their loads in flight before the first store.
+template <typename Tab, typename Out, typename Index, bool ALIGNED, int FLY>
 __global__ void __launch_bounds__(256)
 embedding_kernel(const Tab* __restrict__ table, const Index* __restrict__ index, Out* __restrict__ y, int64_t tokens,
                  int64_t vocab, int64_t dim, int64_t ld_table, int64_t ld_y, float scale) {
-    constexpr int VEC = ALIGNED ? Elem<Out>::VEC : 1;
-    const int64_t per_row = (dim + VEC - 1) / VEC;
-    const int64_t items = tokens * per_row;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-    for (int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; item < items; item += step) {
-        const int64_t t = item / per_row, c = (item - t * per_row) * VEC;
-        const int64_t v = static_cast<int64_t>(index[t]);
-        const bool inside = v >= 0 && v < vocab;
-        const Tab* from = table + (inside ? v : 0) * ld_table;
-        Out* to = y + t * ld_y;
-        if (ALIGNED) {
-            float f[Elem<Out>::VEC];
+    constexpr int VEC = ALIGNED ? Elem<Out>::VEC : 1, TV = ALIGNED ? Elem<Tab>::VEC : 1;
+    const uint32_t per_row = static_cast<uint32_t>((dim + VEC - 1) / VEC);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (256 * FLY) + threadIdx.x;
+    int64_t t = item >> 32 ? item / per_row : static_cast<uint32_t>(item) / per_row;
+    uint32_t b = static_cast<uint32_t>(item - t * per_row);
+    const uint32_t rows_on = 256 / per_row, blocks_on = 256 - rows_on * per_row;
+    uint4 u[FLY][VEC / TV];
+    Tab e[FLY];
+    Out* to[FLY];
+    int64_t col[FLY];
+    bool inside[FLY];
 #pragma unroll
-            for (int i = 0; i < Elem<Out>::VEC; i++) f[i] = 0.f;
-            if (inside) {
-                constexpr int TV = Elem<Tab>::VEC;
+    for (int f = 0; f < FLY; f++) {
+        col[f] = static_cast<int64_t>(b) * VEC;
+        to[f] = nullptr;
+        inside[f] = false;
+        if (t < tokens) {
+            to[f] = y + t * ld_y;
+            const int64_t v = static_cast<int64_t>(index[t]);
+            inside[f] = v >= 0 && v < vocab;
+            const Tab* from = table + (inside[f] ? v : 0) * ld_table;
+            if (inside[f]) {
+                if (ALIGNED) {
 #pragma unroll
-                for (int h = 0; h < Elem<Out>::VEC / TV; h++) {
-                    float part[TV];
-                    Elem<Tab>::unpack(load_block(from, c + h * TV, dim), part);
-#pragma unroll
-                    for (int i = 0; i < TV; i++) f[h * TV + i] = part[i] * scale;
+                    for (int h = 0; h < VEC / TV; h++) u[f][h] = load_block(from, col[f] + h * TV, dim);
+                } else {
+                    e[f] = from[b];
                 }
             }
-            store_block(to, c, dim, Elem<Out>::pack(f));
+        }
+        t += rows_on;
+        b += blocks_on;
+        if (b >= per_row) {
+            b -= per_row;
+            t++;
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < FLY; f++) {
+        if (!to[f]) continue;
+        if (ALIGNED) {
+            float v[Elem<Out>::VEC];
+#pragma unroll
+            for (int i = 0; i < Elem<Out>::VEC; i++) v[i] = 0.f;
+            if (inside[f]) {
+#pragma unroll
+                for (int h = 0; h < VEC / TV; h++) {
+                    float part[Elem<Tab>::VEC];
+                    Elem<Tab>::unpack(u[f][h], part);
+#pragma unroll
+                    for (int i = 0; i < TV; i++) v[h * TV + i] = part[i] * scale;
+                }
+            }
+            store_block(to[f], col[f], dim, Elem<Out>::pack(v));
         } else {
-            to[c] = Elem<Out>::from(inside ? Elem<Tab>::to(from[c]) * scale : 0.f);
+            to[f][col[f]] = Elem<Out>::from(inside[f] ? Elem<Tab>::to(e[f]) * scale : 0.f);
         }
     }
 }
@@ -381,10 +392,8 @@ static EmbeddingPlan plan_embedding(const nzb_embedding_desc* d) {
     if (pl.tiles < 1) pl.tiles = 1;
     pl.tiles_bytes = (size_t)round_up(pl.tiles * (int64_t)sizeof(SortTile), 256);
     pl.present_bytes = (size_t)round_up((d->vocab + 31) / 32 * 4, 256);
-    // a run has more than one piece from kPiece + 1 tokens on
-    int64_t slots = 2 * (d->tokens / kPiece);
-    if (slots > kMaxSlots) slots = kMaxSlots;
-    pl.partial_bytes = (size_t)round_up(slots * d->dim * 4, 256);
+    const int64_t most = d->tokens < kSortTile ? d->tokens : kSortTile;
+    pl.partial_bytes = (size_t)round_up((most + kChunk - 1) / kChunk * 2 * d->dim * 4, 256);  // two borders a chunk
     return pl;
 }
 
@@ -394,30 +403,40 @@ static int launch_embedding(const nzb_embedding_desc* d, const void* table, cons
     const bool aligned = aligned_to(table, 16) && aligned_to(y, 16) && d->ld_table * (int64_t)sizeof(Tab) % 16 == 0 &&
                          d->ld_y * (int64_t)sizeof(Out) % 16 == 0;
     const int64_t items = d->tokens * (aligned ? (d->dim + Elem<Out>::VEC - 1) / Elem<Out>::VEC : d->dim);
-    int64_t blocks = (items + 255) / 256;
-    if (blocks > (int64_t)sm_count * 64) blocks = (int64_t)sm_count * 64;
+    // few blocks: a thread for each, so that more SMs take part (32 rows of 4 KB: 2.2 us instead of 2.8)
+    const int fly = items <= (int64_t)sm_count * 2048 ? 1 : kEmbeddingFly;
+    const int64_t ctas = (items + 256 * fly - 1) / (256 * fly);
+    if (ctas > INT32_MAX) return fail(NZB_ERR_UNSUPPORTED, "more than 2^31 CTAs of rows");
     const Tab* tp = static_cast<const Tab*>(table);
     const Index* ip = static_cast<const Index*>(index);
     Out* yp = static_cast<Out*>(y);
-    if (aligned)
-        embedding_kernel<Tab, Out, Index, true><<<(unsigned)blocks, 256, 0, s>>>(tp, ip, yp, d->tokens, d->vocab, d->dim, d->ld_table, d->ld_y, d->scale);
-    else
-        embedding_kernel<Tab, Out, Index, false><<<(unsigned)blocks, 256, 0, s>>>(tp, ip, yp, d->tokens, d->vocab, d->dim, d->ld_table, d->ld_y, d->scale);
+    const auto kernel = aligned ? (fly == 1 ? embedding_kernel<Tab, Out, Index, true, 1> : embedding_kernel<Tab, Out, Index, true, kEmbeddingFly>)
+                                : (fly == 1 ? embedding_kernel<Tab, Out, Index, false, 1> : embedding_kernel<Tab, Out, Index, false, kEmbeddingFly>);
+    kernel<<<(unsigned)ctas, 256, 0, s>>>(tp, ip, yp, d->tokens, d->vocab, d->dim, d->ld_table, d->ld_y, d->scale);
     NZB_CUDA_TRY(cudaGetLastError());
     return NZB_OK;
 }
 
 template <typename Index>
 static int launch_sort(const nzb_embedding_desc* d, const void* index, const EmbeddingPlan& pl, SortTile* tiles,
-                       uint32_t* present, cudaStream_t s) {
+                       uint32_t* present, float* dtable, int sm_count, cudaStream_t s) {
     static std::atomic<uint64_t> smem_set{0};
     int rc = ensure_dynamic_smem(smem_set, reinterpret_cast<const void*>(embedding_sort_kernel<Index>), sizeof(SortSmem));
     if (rc != NZB_OK) return rc;
     int bits = 1;
     while (d->vocab >> bits) bits++;  // vocab itself stands for "no token"
     const int passes = (bits + 8) / 9, digit = (bits + passes - 1) / passes;
-    embedding_sort_kernel<Index><<<(unsigned)pl.tiles, kSortThreads, sizeof(SortSmem), s>>>(
-        static_cast<const Index*>(index), d->tokens, d->vocab, d->padding_index, digit, passes, tiles, present);
+    const Index* ip = static_cast<const Index*>(index);
+    unsigned grid = (unsigned)pl.tiles;
+    if (d->overwrite) {
+        const int64_t first = d->tokens < kSortTile ? d->tokens : kSortTile;
+        NZB_CUDA_TRY(cudaMemsetAsync(present, 0, pl.present_bytes, s));
+        if (first) embedding_mark_kernel<Index><<<(unsigned)((first + 255) / 256), 256, 0, s>>>(ip, first, d->vocab, d->padding_index, present);
+        // the sorting CTAs fill an SM each; the others share the rows to clear
+        grid += (unsigned)(sm_count - (pl.tiles < sm_count / 2 ? pl.tiles : 0));
+    }
+    embedding_sort_kernel<Index><<<grid, kSortThreads, sizeof(SortSmem), s>>>(ip, d->tokens, d->vocab, d->padding_index, digit, passes,
+                                                                            (int)pl.tiles, tiles, present, dtable, d->dim, d->ld_table);
     NZB_CUDA_TRY(cudaGetLastError());
     return NZB_OK;
 }
@@ -479,23 +498,26 @@ int nzb_embedding_backward(const nzb_embedding_desc* d, const void* dy, const vo
     SortTile* tiles = reinterpret_cast<SortTile*>(base);
     uint32_t* present = reinterpret_cast<uint32_t*>(base + pl.tiles_bytes);
     float* partial = reinterpret_cast<float*>(base + pl.tiles_bytes + pl.present_bytes);
-    NZB_CUDA_TRY(cudaMemsetAsync(present, 0, pl.present_bytes, s));
-    rc = d->index_type == NZB_I64 ? launch_sort<int64_t>(d, index, pl, tiles, present, s)
-                                  : launch_sort<int32_t>(d, index, pl, tiles, present, s);
+    rc = d->index_type == NZB_I64 ? launch_sort<int64_t>(d, index, pl, tiles, present, dtable, ds->sm_count, s)
+                                  : launch_sort<int32_t>(d, index, pl, tiles, present, dtable, ds->sm_count, s);
     if (rc != NZB_OK) return rc;
     const int vec_out = aligned_to(dtable, 16) && d->ld_table % 4 == 0;
-    const unsigned grid = (unsigned)ds->sm_count * 8;
     for (int64_t t = 0; t < pl.tiles; t++) {
-        const int add = t > 0 || !d->overwrite, zero_rest = t == 0 && d->overwrite;
+        const int add = t > 0 || !d->overwrite;
+        const int64_t n = d->tokens - t * kSortTile < kSortTile ? d->tokens - t * kSortTile : kSortTile;
+        const int64_t chunks = (n + kChunk - 1) / kChunk;
+        if (chunks == 0) break;
         NZB_DISPATCH_DTYPE(d->dtype, T, {
             const T* from = static_cast<const T*>(dy) + t * kSortTile * d->ld_y;
+            const int64_t warps = chunks * ((d->dim + 32 * Elem<T>::VEC - 1) / (32 * Elem<T>::VEC));
+            const unsigned grid = (unsigned)((warps + 7) / 8);
             if (aligned_to(dy, 16) && d->ld_y * (int64_t)sizeof(T) % 16 == 0)
-                embedding_sum_kernel<T, true><<<grid, 256, 0, s>>>(from, tiles + t, present, dtable, partial, d->vocab, d->dim, d->ld_table, d->ld_y, d->scale, add, zero_rest, vec_out);
+                embedding_sum_kernel<T, true><<<grid, 256, 0, s>>>(from, tiles + t, dtable, partial, d->dim, d->ld_table, d->ld_y, d->scale, add, vec_out);
             else
-                embedding_sum_kernel<T, false><<<grid, 256, 0, s>>>(from, tiles + t, present, dtable, partial, d->vocab, d->dim, d->ld_table, d->ld_y, d->scale, add, zero_rest, vec_out);
+                embedding_sum_kernel<T, false><<<grid, 256, 0, s>>>(from, tiles + t, dtable, partial, d->dim, d->ld_table, d->ld_y, d->scale, add, vec_out);
         });
-        if (d->tokens - t * kSortTile > kPiece)
-            embedding_join_kernel<<<grid, 256, 0, s>>>(tiles + t, partial, dtable, d->dim, d->ld_table, d->scale, add);
+        if (chunks > 1)
+            embedding_join_kernel<<<(unsigned)((chunks * ((d->dim + 127) / 128) + 7) / 8), 256, 0, s>>>(tiles + t, partial, dtable, d->dim, d->ld_table, d->scale, add);
         NZB_CUDA_TRY(cudaGetLastError());
     }
     return NZB_OK;
