@@ -13,80 +13,221 @@
 
 namespace nzb {
 
-template <int WARPS>
+// Sum over the CTA, the same bits in every thread. buf: a float per warp, not written again before the next barrier.
 __device__ __forceinline__ float block_sum(float v, float* buf) {
     v = warp_sum(v);
-    if (WARPS == 1) return v;
+    const int warps = blockDim.x >> 5;
+    if (warps == 1) return v;
     if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
     __syncthreads();
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < WARPS; i++) t += buf[i];
-    return t;
+    const int lane = threadIdx.x & 31;
+    return warp_sum(lane < warps ? buf[lane] : 0.f);
 }
 
-// NT threads per row; a warp per row (eight rows per CTA) when NT == 32.
-template <typename T, int NT, int VPT>
-__global__ void __launch_bounds__(NT == 32 ? 256 : NT)
+constexpr int kNormElems = 16;     // backward: columns per thread
+constexpr int kNormStages = 3;     // backward: rows on their way
+// Forward: 32 elements a thread need 80 registers, 16 and fewer 64.
+template <typename T, int ELEMS>
+constexpr int norm_max_threads() { return ELEMS == 32 ? 768 : 1024; }
+constexpr int kNormBackwardMaxThreads = 512;  // backward: 32 sums per thread beside the row
+constexpr int kNormSmem = 225 * 1024;          // dynamic shared memory of a CTA
+constexpr int kNormSms = 148;      // the workspace holds one pair of sums per CTA of a grid over this many SMs
+
+// A thread's share of a row: the blocks t, t + nt, ... of VPT. The same for every row of a residue.
+template <typename T, int VPT>
+struct RowShare {
+    static constexpr int VEC = Elem<T>::VEC;
+    int first0, pitch;      // first element of block 0; elements between two blocks
+    uint32_t some, whole;   // a bit per block: holds any of the row's elements; holds nothing else
+    float extra;            // elements of its cut blocks that lie outside the row
+    __device__ __forceinline__ RowShare(int t, int nt, int lead, int dim) : first0(t * VEC - lead), pitch(nt * VEC), some(0), whole(0) {
+        int in = 0;
+#pragma unroll
+        for (int k = 0; k < VPT; k++) {
+            if (first(k) < dim) some |= 1u << k;
+            if (first(k) >= 0 && first(k) + VEC <= dim) whole |= 1u << k;
+            in += max(0, min(first(k) + VEC, dim) - max(first(k), 0));
+        }
+        extra = static_cast<float>(__popc(some) * VEC - in);
+    }
+    __device__ __forceinline__ int first(int k) const { return first0 + k * pitch; }
+    __device__ __forceinline__ bool has(int k) const { return some >> k & 1; }
+    __device__ __forceinline__ float weight(int k) const { return has(k) ? 1.f : 0.f; }
+    __device__ __forceinline__ float count() const { return __popc(some) * static_cast<float>(VEC) - extra; }
+    // Gives the elements outside the row, in this thread's places in shared memory, the value of one inside it (so that
+    // they deviate from the mean like any other and can be subtracted from the sums without loss), or zero; returns that
+    // value. Only the threads at the row's ends have any, and nobody else pays for a mask.
+    __device__ __forceinline__ float patch(uint4* ring, int nt, int dim, bool zero) const {
+        if (extra == 0.f) return 0.f;
+        T value = Elem<T>::from(0.f);
+        for (int k = 0; k < VPT && !zero; k++)
+            if (has(k) && !(whole >> k & 1)) value = reinterpret_cast<T*>(ring + k * nt)[max(0, -first(k))];
+        for (int k = 0; k < VPT; k++)
+            if (has(k) && !(whole >> k & 1))
+                for (int i = 0; i < VEC; i++)
+                    if (first(k) + i < 0 || first(k) + i >= dim) reinterpret_cast<T*>(ring + k * nt)[i] = value;
+        return Elem<T>::to(value);
+    }
+    // Starts the copies of the row that begins at element `at` of a tensor of n to this thread's own places in shared
+    // memory, nt blocks apart; the same thread reads them after they have landed, so no barrier is needed. A block at
+    // the row's end brings elements of its neighbours, or of the gap between two rows, along, which patch() replaces;
+    // only blocks that reach beyond the tensor go element by element (waiting for them cost a memory latency per row).
+    __device__ __forceinline__ void fetch(uint4* ring, int nt, const T* base, int64_t at, int64_t n, bool border) const {
+        uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+        const T* from = base + at + first0;
+#pragma unroll
+        for (int k = 0; k < VPT; k++, to += nt * 16, from += pitch) {
+            if (!has(k)) continue;
+            if (border && (at + first(k) < 0 || at + first(k) + VEC > n)) ring[k * nt] = load_block(base, at + first(k), n);
+            else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        }
+    }
+    // Writes block k of a row that starts on the same offset from 16 bytes.
+    __device__ __forceinline__ void store(T* row, int k, int dim, const float (&f)[VEC]) const {
+        if (whole >> k & 1) *reinterpret_cast<uint4*>(row + first(k)) = Elem<T>::pack(f);
+        else if (has(k)) store_block(row, first(k), dim, Elem<T>::pack(f));
+    }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// A group of `nt` threads works on a row; the CTA's groups walk the rows of one residue, so that a thread's columns
+// stay the same: gamma and beta lie in shared memory as the threads read them, four at a time without bank conflicts
+// (read from memory unaligned for every row they cost more than the row: 8191 x 5003 fp16 113 us), and all groups
+// share them. STAGES rows per group are on their way while one is worked on. EXACT: rows start on 16 bytes and fill
+// the group's threads, so nothing is masked.
+// Statistics with one barrier: a warp's mean and its squares about that mean, then the warps' pairs joined,
+// M2 = sum_w (M2_w + n_w (mean_w - mean)^2); no difference of large numbers anywhere.
+template <typename T, int ELEMS, int STAGES, bool EXACT>
+__global__ void __launch_bounds__(norm_max_threads<T, ELEMS>())
 layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __restrict__ beta, T* y,
                  float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int dim, int64_t ld_x,
-                 int64_t ld_y, float eps) {
-    constexpr int VEC = Elem<T>::VEC, WARPS = NT / 32;
-    __shared__ float buf[2][WARPS];
-    const int t = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t r = NT == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-    if (r >= rows) return;
-    const T* xr = x + r * ld_x;
-    T* yr = y + r * ld_y;
-    const int lead = row_lead(xr);
-    float v[VPT][VEC];
-    float sum = 0.f;
+                 int64_t ld_y, float eps, int period, int y_together, int nt, int groups) {
+    constexpr int VEC = Elem<T>::VEC, VPT = ELEMS / VEC, Q = ELEMS / 4;
+    extern __shared__ uint4 smem_norm[];
+    __shared__ float2 buf[2][32];  // per warp of the CTA: mean and M2
+    const int group = threadIdx.x / nt, t = threadIdx.x - group * nt, lane = threadIdx.x & 31;
+    const int warps = nt >> 5, warp0 = group * warps, warp = threadIdx.x >> 5;
+    float4* params = reinterpret_cast<float4*>(smem_norm) + t;                          // [2][Q][nt]
+    uint4* ring = smem_norm + 2 * Q * nt + group * (STAGES * VPT * nt) + t;             // per group [STAGES][VPT][nt]
+    const int residue = blockIdx.x % period;
+    const int lead = EXACT ? 0 : row_lead(x + residue * ld_x);
+    const int64_t span = (rows - 1) * ld_x + dim;
+    const int64_t step = static_cast<int64_t>(gridDim.x / period) * groups * period;
+    const int64_t first_row = residue + static_cast<int64_t>(period) * (static_cast<int64_t>(blockIdx.x / period) * groups + group);
+    const RowShare<T, VPT> share(t, nt, lead, dim);
+    if (!EXACT) {
+        // blocks beyond the row are read as zeros, with weight zero
 #pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        const int first = (t + k * NT) * VEC - lead;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (first < dim) u = load_block(xr, first, dim);
-        Elem<T>::unpack(u, v[k]);
-#pragma unroll
-        for (int i = 0; i < VEC; i++) sum += v[k][i];
+        for (int k = 0; k < STAGES * VPT; k++)
+            if (!share.has(k % VPT)) ring[k * nt] = make_uint4(0, 0, 0, 0);
     }
-    const float mean = block_sum<WARPS>(sum, buf[0]) / dim;
-    float sq = 0.f;
+    const auto fetch = [&](int64_t r, int stage) {
+        if (r < rows) share.fetch(ring + stage * VPT * nt, nt, x, r * ld_x, span, !EXACT && (r == 0 || r == rows - 1));
+        copies_commit();
+    };
 #pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        const int first = (t + k * NT) * VEC - lead;
+    for (int s = 0; s < STAGES; s++) fetch(first_row + s * step, s);
+    for (int q = group; q < Q; q += groups) {
+        float g[4], b[4];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            v[k][i] -= mean;
-            if (first + i >= 0 && first + i < dim) sq += v[k][i] * v[k][i];
-        }
-    }
-    const float var = block_sum<WARPS>(sq, buf[1]) / dim;
-    const float rstd = 1.f / sqrtf(var + eps);
-    if (t == 0) {
-        if (mean_out) mean_out[r] = mean;
-        if (rstd_out) rstd_out[r] = rstd;
-    }
-    const bool same = row_lead(yr) == lead;
-#pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        const int first = (t + k * NT) * VEC - lead;
-        if (first >= dim) continue;
-        float o[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int c = first + i;
+        for (int i = 0; i < 4; i++) {
+            const int e = q * 4 + i, c = (t + e / VEC * nt) * VEC - lead + e % VEC;
             const bool in = c >= 0 && c < dim;
-            o[i] = v[k][i] * rstd * (gamma && in ? __ldg(gamma + c) : 1.f) + (beta && in ? __ldg(beta + c) : 0.f);
+            g[i] = in ? (gamma ? gamma[c] : 1.f) : 0.f;
+            b[i] = in && beta ? beta[c] : 0.f;
         }
-        if (same) {
-            store_block(yr, first, dim, Elem<T>::pack(o));
-        } else {
+        params[q * nt] = make_float4(g[0], g[1], g[2], g[3]);
+        params[(Q + q) * nt] = make_float4(b[0], b[1], b[2], b[3]);
+    }
+    __syncthreads();
+    // elements of this warp and, lane by lane, of the group's warps
+    const float n_warp = warp_sum(share.count()), inv_warp = n_warp > 0.f ? 1.f / n_warp : 0.f, inv = 1.f / dim;
+    float n_lane = 0.f;
+    if (warps > 1) {
+        if (lane == 0) buf[0][warp].x = n_warp;
+        __syncthreads();
+        n_lane = lane < warps ? buf[0][warp0 + lane].x : 0.f;
+        __syncthreads();
+    }
+    int turn = 0, stage = 0;
+    for (int64_t r = first_row; r < rows; r += step, turn ^= 1) {
+        copies_wait<STAGES - 1>();
+        const float extra_value = EXACT ? 0.f : share.patch(ring + stage * VPT * nt, nt, dim, false);
+        float2 v[VPT][VEC / 2];
+        float sum = 0.f, sq = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; i++)
-                if (first + i >= 0 && first + i < dim) yr[first + i] = Elem<T>::from(o[i]);
+        for (int k = 0; k < VPT; k++) {
+            float f[VEC];
+            Elem<T>::unpack(ring[(stage * VPT + k) * nt], f);
+            float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) {
+                v[k][i] = make_float2(f[2 * i], f[2 * i + 1]);
+                part = add2(part, v[k][i]);
+            }
+            sum = EXACT ? sum + (part.x + part.y) : fmaf(share.weight(k), part.x + part.y, sum);
+        }
+        if (!EXACT) sum = fmaf(-share.extra, extra_value, sum);
+        fetch(r + STAGES * step, stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        float mean = warp_sum(sum) * inv_warp;
+        const float2 minus = make_float2(-mean, -mean);
+#pragma unroll
+        for (int k = 0; k < VPT; k++) {
+            float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) {
+                const float2 d = add2(v[k][i], minus);
+                part = fma2(d, d, part);
+            }
+            sq = EXACT ? sq + (part.x + part.y) : fmaf(share.weight(k), part.x + part.y, sq);
+        }
+        if (!EXACT) {
+            const float d = extra_value - mean;
+            sq = fmaf(-share.extra * d, d, sq);
+        }
+        float m2 = warp_sum(sq);
+        if (warps > 1) {
+            if (lane == 0) buf[turn][warp] = make_float2(mean, m2);
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(nt) : "memory");
+            const float2 part = lane < warps ? buf[turn][warp0 + lane] : make_float2(0.f, 0.f);
+            mean = warp_sum(part.x * n_lane) * inv;
+            const float d = part.x - mean;
+            m2 = warp_sum(lane < warps ? fmaf(n_lane * d, d, part.y) : 0.f);
+        }
+        const float rstd = rsqrtf(fmaf(m2, inv, eps));
+        if (t == 0) {
+            if (mean_out) mean_out[r] = mean;
+            if (rstd_out) rstd_out[r] = rstd;
+        }
+        T* yr = y + r * ld_y;
+        const float2 rs = make_float2(rstd, rstd), shift = make_float2(-mean, -mean);
+#pragma unroll
+        for (int k = 0; k < VPT; k++) {
+            if (!EXACT && !share.has(k)) continue;
+            float o[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC / 4; q++) {
+                const float4 g = params[(k * (VEC / 4) + q) * nt], b = params[(Q + k * (VEC / 4) + q) * nt];
+                // (x - mean) rstd, then gamma and beta
+                const float2 lo = fma2(mul2(add2(v[k][2 * q], shift), rs), make_float2(g.x, g.y), make_float2(b.x, b.y));
+                const float2 hi = fma2(mul2(add2(v[k][2 * q + 1], shift), rs), make_float2(g.z, g.w), make_float2(b.z, b.w));
+                o[4 * q] = lo.x; o[4 * q + 1] = lo.y; o[4 * q + 2] = hi.x; o[4 * q + 3] = hi.y;
+            }
+            if (EXACT || y_together) {
+                share.store(yr, k, dim, o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    const int c = share.first(k) + i;
+                    if (c >= 0 && c < dim) yr[c] = Elem<T>::from(o[i]);
+                }
+            }
         }
     }
+    copies_wait<0>();
 }
 
 // Rows too long for the registers of a CTA: three walks over the row.
@@ -100,13 +241,13 @@ layernorm_long_kernel(const T* x, const float* __restrict__ gamma, const float* 
     T* yr = y + r * ld_y;
     float sum = 0.f;
     for (int c = threadIdx.x; c < dim; c += 1024) sum += Elem<T>::to(xr[c]);
-    const float mean = block_sum<32>(sum, buf[0]) / dim;
+    const float mean = block_sum(sum, buf[0]) / dim;
     float sq = 0.f;
     for (int c = threadIdx.x; c < dim; c += 1024) {
         const float d = Elem<T>::to(xr[c]) - mean;
         sq += d * d;
     }
-    const float rstd = 1.f / sqrtf(block_sum<32>(sq, buf[1]) / dim + eps);
+    const float rstd = 1.f / sqrtf(block_sum(sq, buf[1]) / dim + eps);
     if (threadIdx.x == 0) {
         if (mean_out) mean_out[r] = mean;
         if (rstd_out) rstd_out[r] = rstd;
@@ -115,113 +256,140 @@ layernorm_long_kernel(const T* x, const float* __restrict__ gamma, const float* 
         yr[c] = Elem<T>::from((Elem<T>::to(xr[c]) - mean) * rstd * (gamma ? gamma[c] : 1.f) + (beta ? beta[c] : 0.f));
 }
 
-constexpr int kNormElems = 16;     // columns per thread of the fused backward kernel
-constexpr int kNormMaxThreads = 512;
-constexpr int kNormSms = 148;      // the workspace holds one pair of sums per CTA of a grid over this many SMs
+// Two sums over the warp in one chain of shuffles: the lower half of the lanes ends with the first, the upper half with
+// the second.
+__device__ __forceinline__ float warp_sum_two(float a, float b, int lane) {
+    const bool upper = lane & 16;
+    float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
-// One CTA per residue of rows and slot; period: rows after which the start addresses repeat modulo 16 bytes.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT)
+// The same walk as the forward kernel's with a row per CTA, x and dy on their way together.
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(kNormBackwardMaxThreads)
 layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
                           const float* __restrict__ gamma, T* dx, float* __restrict__ partial, int64_t rows, int dim,
                           int64_t ld_x, int64_t ld_dy, int64_t ld_dx, int period, int add_dx) {
-    constexpr int VEC = Elem<T>::VEC, VPT = kNormElems / VEC, WARPS = NT / 32;
-    __shared__ float buf[2][2][WARPS];
-    const int t = threadIdx.x;
-    const int residue = blockIdx.x % period;
-    const int lead = row_lead(x + residue * ld_x);
-    float dg[VPT][VEC], db[VPT][VEC], ga[VPT][VEC];
+    constexpr int VEC = Elem<T>::VEC, VPT = kNormElems / VEC, Q = kNormElems / 4;
+    extern __shared__ uint4 smem_norm[];
+    __shared__ float buf[2][2][16];
+    const int t = threadIdx.x, NT = blockDim.x, lane = t & 31, warps = NT >> 5;
+    uint4* ring = smem_norm + t;  // [stage][x, dy][VPT][NT]
+    float4* params = reinterpret_cast<float4*>(smem_norm + kNormStages * 2 * VPT * NT) + t;  // [Q][NT]
+    const int lead = EXACT ? 0 : row_lead(x + (blockIdx.x % period) * ld_x);
+    const int64_t span_x = (rows - 1) * ld_x + dim, span_dy = (rows - 1) * ld_dy + dim;
+    const RowShare<T, VPT> share(t, NT, lead, dim);
+    if (!EXACT) {
+        // blocks beyond the row are read as zeros: a dy of zero adds nothing
 #pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        const int first = (t + k * NT) * VEC - lead;
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int c = first + i;
-            dg[k][i] = db[k][i] = 0.f;
-            ga[k][i] = c >= 0 && c < dim ? (gamma ? gamma[c] : 1.f) : 0.f;
-        }
+        for (int k = 0; k < kNormStages * 2 * VPT; k++)
+            if (!share.has(k % VPT)) ring[k * NT] = make_uint4(0, 0, 0, 0);
     }
-    int turn = 0;
-    const int64_t step = static_cast<int64_t>(gridDim.x / period) * period;
-    for (int64_t r = blockIdx.x; r < rows; r += step, turn ^= 1) {
-        const T* xr = x + r * ld_x;
-        const T* dyr = dy + r * ld_dy;
-        const float mu = mean[r], rs = rstd[r];
-        uint4 ux[VPT], ud[VPT];
-#pragma unroll
-        for (int k = 0; k < VPT; k++) {
-            const int first = (t + k * NT) * VEC - lead;
-            ux[k] = ud[k] = make_uint4(0, 0, 0, 0);
-            if (first < dim) {
-                ux[k] = load_block(xr, first, dim);
-                ud[k] = load_block(dyr, first, dim);
-            }
+    const auto fetch = [&](int64_t r, int stage) {
+        if (r < rows) {
+            const bool border = !EXACT && (r == 0 || r == rows - 1);
+            share.fetch(ring + stage * 2 * VPT * NT, NT, x, r * ld_x, span_x, border);
+            share.fetch(ring + (stage * 2 + 1) * VPT * NT, NT, dy, r * ld_dy, span_dy, border);
         }
-        float sg = 0.f, sgh = 0.f;
+        copies_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kNormStages; s++) fetch(blockIdx.x + static_cast<int64_t>(s) * gridDim.x, s);
+    float2 dg[VPT][VEC / 2], db[VPT][VEC / 2];
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        float g[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = q * 4 + i, c = (t + e / VEC * NT) * VEC - lead + e % VEC;
+            g[i] = c >= 0 && c < dim ? (gamma ? gamma[c] : 1.f) : 0.f;
+            dg[e / VEC][e % VEC / 2] = db[e / VEC][e % VEC / 2] = make_float2(0.f, 0.f);
+        }
+        params[q * NT] = make_float4(g[0], g[1], g[2], g[3]);
+    }
+    const float inv = 1.f / dim;
+    int turn = 0, stage = 0;
+    float next_mean = blockIdx.x < rows ? mean[blockIdx.x] : 0.f, next_rstd = blockIdx.x < rows ? rstd[blockIdx.x] : 0.f;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
+        const float2 rs = make_float2(next_rstd, next_rstd), minus = make_float2(-next_mean, -next_mean);
+        if (r + gridDim.x < rows) {
+            next_mean = mean[r + gridDim.x];
+            next_rstd = rstd[r + gridDim.x];
+        }
+        copies_wait<kNormStages - 1>();
+        if (!EXACT) {
+            // outside the row: an x of the row, whose h is finite where the row's are, and a dy of zero, which adds nothing
+            share.patch(ring + stage * 2 * VPT * NT, NT, dim, false);
+            share.patch(ring + (stage * 2 + 1) * VPT * NT, NT, dim, true);
+        }
+        float2 h[VPT][VEC / 2], g[VPT][VEC / 2];
+        float2 sg = make_float2(0.f, 0.f), sgh = sg;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             float fx[VEC], fd[VEC];
-            Elem<T>::unpack(ux[k], fx);
-            Elem<T>::unpack(ud[k], fd);
+            Elem<T>::unpack(ring[((stage * 2) * VPT + k) * NT], fx);
+            Elem<T>::unpack(ring[((stage * 2 + 1) * VPT + k) * NT], fd);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float h = (fx[i] - mu) * rs, g = fd[i] * ga[k][i];
-                sg += g;
-                sgh += g * h;
-                dg[k][i] += fd[i] * h;
-                db[k][i] += fd[i];
+            for (int i = 0; i < VEC / 2; i++) {
+                const float4 ga = params[(k * (VEC / 4) + i / 2) * NT];
+                const float2 d = make_float2(fd[2 * i], fd[2 * i + 1]);
+                h[k][i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
+                g[k][i] = mul2(d, i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
+                sg = add2(sg, g[k][i]);
+                sgh = fma2(g[k][i], h[k][i], sgh);
+                dg[k][i] = fma2(d, h[k][i], dg[k][i]);
+                db[k][i] = add2(db[k][i], d);
             }
         }
+        fetch(r + static_cast<int64_t>(kNormStages) * gridDim.x, stage);
+        stage = stage + 1 == kNormStages ? 0 : stage + 1;
         if (!dx) continue;
-        sg = warp_sum(sg);
-        sgh = warp_sum(sgh);
-        if (WARPS > 1) {
-            if ((t & 31) == 0) {
-                buf[turn][0][t >> 5] = sg;
-                buf[turn][1][t >> 5] = sgh;
-            }
+        float s = warp_sum_two(sg.x + sg.y, sgh.x + sgh.y, lane);
+        if (warps > 1) {
+            if ((lane & 15) == 0) buf[turn][lane >> 4][t >> 5] = s;
             __syncthreads();
-            sg = sgh = 0.f;
+            s = (lane & 15) < warps ? buf[turn][lane >> 4][lane & 15] : 0.f;
 #pragma unroll
-            for (int w = 0; w < WARPS; w++) {
-                sg += buf[turn][0][w];
-                sgh += buf[turn][1][w];
-            }
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         }
-        sg /= dim;
-        sgh /= dim;
+        // dx = rstd (g - mean g - h mean(g h))
+        s *= -rs.x * inv;
+        const float other = __shfl_xor_sync(0xffffffffu, s, 16);
+        const float m0 = lane & 16 ? other : s, m1 = lane & 16 ? s : other;
+        const float2 m0s = make_float2(m0, m0), m1s = make_float2(m1, m1);
         T* dxr = dx + r * ld_dx;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
-            const int first = (t + k * NT) * VEC - lead;
-            if (first >= dim) continue;
-            float fx[VEC], fd[VEC];
-            Elem<T>::unpack(ux[k], fx);
-            Elem<T>::unpack(ud[k], fd);
+            if (!EXACT && !share.has(k)) continue;
+            float o[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float h = (fx[i] - mu) * rs;
-                fd[i] = rs * (fd[i] * ga[k][i] - sg - h * sgh);
+            for (int i = 0; i < VEC / 2; i++) {
+                const float2 d = fma2(g[k][i], rs, fma2(h[k][i], m1s, m0s));
+                o[2 * i] = d.x;
+                o[2 * i + 1] = d.y;
             }
             if (add_dx) {
-                Elem<T>::unpack(load_block(dxr, first, dim), fx);
+                float old[VEC];
+                Elem<T>::unpack(load_block(dxr, share.first(k), dim), old);
 #pragma unroll
-                for (int i = 0; i < VEC; i++) fd[i] += fx[i];
+                for (int i = 0; i < VEC; i++) o[i] += old[i];
             }
-            store_block(dxr, first, dim, Elem<T>::pack(fd));
+            share.store(dxr, k, dim, o);
         }
     }
+    copies_wait<0>();
     if (!partial) return;
     float* pg = partial + static_cast<int64_t>(blockIdx.x) * 2 * dim;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
-        const int first = (t + k * NT) * VEC - lead;
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
-            const int c = first + i;
+            const int c = share.first(k) + i;
             if (c >= 0 && c < dim) {
-                pg[c] = dg[k][i];
-                pg[dim + c] = db[k][i];
+                pg[c] = i & 1 ? dg[k][i / 2].y : dg[k][i / 2].x;
+                pg[dim + c] = i & 1 ? db[k][i / 2].y : db[k][i / 2].x;
             }
         }
     }
@@ -233,7 +401,7 @@ template <typename T>
 __global__ void __launch_bounds__(512)
 layernorm_dx_kernel(const T* dy, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
                     const float* __restrict__ gamma, T* dx, int dim, int64_t ld_x, int64_t ld_dy, int64_t ld_dx, int add_dx) {
-    __shared__ float buf[2][16];
+    __shared__ float buf[2][32];
     const int64_t r = blockIdx.x;
     const T* xr = x + r * ld_x;
     const T* dyr = dy + r * ld_dy;
@@ -245,8 +413,8 @@ layernorm_dx_kernel(const T* dy, const T* x, const float* __restrict__ mean, con
         sg += g;
         sgh += g * ((Elem<T>::to(xr[c]) - mu) * rs);
     }
-    sg = block_sum<16>(sg, buf[0]) / dim;
-    sgh = block_sum<16>(sgh, buf[1]) / dim;
+    sg = block_sum(sg, buf[0]) / dim;
+    sgh = block_sum(sgh, buf[1]) / dim;
     for (int c = threadIdx.x; c < dim; c += 512) {
         const float g = Elem<T>::to(dyr[c]) * (gamma ? gamma[c] : 1.f);
         float d = rs * (g - sg - (Elem<T>::to(xr[c]) - mu) * rs * sgh);
@@ -283,7 +451,7 @@ layernorm_reduce_kernel(const float* __restrict__ partial, int parts, float* __r
     float s = 0.f;
     if (c < 2 * dim) {
         const int p1 = parts * (slice + 1) / 8;
-#pragma unroll 4
+#pragma unroll 8
         for (int p = parts * slice / 8; p < p1; p++) s += partial[static_cast<int64_t>(p) * 2 * dim + c];
     }
     buf[slice][lane] = s;
@@ -307,36 +475,20 @@ static int check_layernorm(const nzb_layernorm_desc* d) {
     return NZB_OK;
 }
 
-// CTAs of the fused backward kernel for this row length, threads per CTA; 0 threads: the row is too long.
-static int norm_threads(int64_t dim, int vec) {
-    const int64_t need = (dim + vec - 1 + kNormElems - 1) / kNormElems;  // the first block may be partly before the row
-    for (int nt = 32; nt <= kNormMaxThreads; nt *= 2)
-        if (need <= nt) return nt;
-    return 0;
+// Threads that hold a row of `dim` elements in registers, `elems` each; 0: more than `most`. lead: elements the row's
+// first block may share with what is before it.
+static int norm_threads(int64_t dim, int lead, int most, int elems) {
+    const int64_t nt = round_up((dim + lead + elems - 1) / elems, 32);
+    return nt <= most ? (int)nt : 0;
 }
+// CTAs of the backward kernel, at most; sized for rows that start anywhere, whatever the tensors' addresses. Its 100
+// registers a thread leave room for 640 threads on an SM.
 static int64_t norm_parts(const nzb_layernorm_desc* d) {
-    const int nt = norm_threads(d->dim, d->dtype == NZB_F32 ? 4 : 8);
+    const int nt = norm_threads(d->dim, 0, kNormBackwardMaxThreads, kNormElems);
     if (nt == 0) return d->rows < 64 ? d->rows : 64;
-    int64_t ctas = (int64_t)kNormSms * (1024 / nt);
+    int64_t ctas = (int64_t)kNormSms * (640 / nt);
     if (ctas > d->rows) ctas = d->rows;
     return ctas < 8 ? 8 : ctas;  // at least one per residue
-}
-
-template <typename T, int NT, int VPT>
-static void launch_norm(const nzb_layernorm_desc* d, const void* x, const float* gamma, const float* beta, void* y,
-                        float* mean, float* rstd, cudaStream_t s) {
-    const unsigned blocks = (unsigned)(NT == 32 ? (d->rows + 7) / 8 : d->rows);
-    layernorm_kernel<T, NT, VPT><<<blocks, NT == 32 ? 256 : NT, 0, s>>>(static_cast<const T*>(x), gamma, beta, static_cast<T*>(y),
-                                                                        mean, rstd, d->rows, (int)d->dim, d->ld_x, d->ld_y, d->eps);
-}
-
-template <typename T, int NT>
-static void launch_norm_backward(const nzb_layernorm_desc* d, const void* dy, const void* x, const float* mean,
-                                 const float* rstd, const float* gamma, void* dx, float* partial, int period, unsigned ctas,
-                                 cudaStream_t s) {
-    layernorm_backward_kernel<T, NT><<<ctas, NT, 0, s>>>(static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, gamma,
-                                                         static_cast<T*>(dx), partial, d->rows, (int)d->dim, d->ld_x, d->ld_y,
-                                                         d->ld_dx, period, !d->overwrite_dx);
 }
 
 }  // namespace nzb
@@ -359,17 +511,44 @@ int nzb_layernorm_forward(const nzb_layernorm_desc* d, const void* x, const floa
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     NZB_DISPATCH_DTYPE(d->dtype, T, {
         constexpr int VEC = Elem<T>::VEC;
-        const bool aligned = aligned_to(x, 16) && d->ld_x * size % 16 == 0;
-        const int64_t n = (d->dim + (aligned ? 0 : VEC - 1) + VEC - 1) / VEC;  // 16-byte blocks of a row
-        if (n <= 32) launch_norm<T, 32, 1>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 64) launch_norm<T, 32, 2>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 128) launch_norm<T, 32, 4>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 256) launch_norm<T, 128, 2>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 512) launch_norm<T, 128, 4>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 1024) launch_norm<T, 256, 4>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 2048) launch_norm<T, 512, 4>(d, x, gamma, beta, y, mean, rstd, s);
-        else if (n <= 4096) launch_norm<T, 1024, 4>(d, x, gamma, beta, y, mean, rstd, s);
-        else layernorm_long_kernel<T><<<(unsigned)d->rows, 1024, 0, s>>>(static_cast<const T*>(x), gamma, beta, static_cast<T*>(y), mean, rstd, (int)d->dim, d->ld_x, d->ld_y, d->eps);
+        const bool repeats = d->ld_x * size % 16 == 0;
+        const int period = repeats ? 1 : VEC;
+        // four blocks per thread: the instructions of the sums' joins are per thread
+        constexpr int WIDE = VEC * 4;
+        const int lead = repeats && aligned_to(x, 16) ? 0 : VEC - 1;
+        // rows for less than one round of the SMs: one block per thread shortens a row's way (64 x 1024 fp32: 2.8 us
+        // instead of 4.2)
+        int nt = d->rows <= ds->sm_count ? norm_threads(d->dim, lead, 1024, VEC) : 0;
+        const bool y_together = reinterpret_cast<uintptr_t>(x) % 16 == reinterpret_cast<uintptr_t>(y) % 16 && d->ld_x * size % 16 == d->ld_y * size % 16;
+        const int elems = nt ? VEC : WIDE, most = nt ? 1024 : norm_max_threads<T, WIDE>();
+        if (!nt) nt = norm_threads(d->dim, lead, most, elems);
+        const int params = nt * 2 * elems * 4, row = nt * elems / VEC * 16;
+        const int stages = elems == VEC || params + 2 * row > kNormSmem ? 1 : 2;
+        const T* xp = static_cast<const T*>(x);
+        T* yp = static_cast<T*>(y);
+        if (nt && params + stages * row <= kNormSmem) {
+            const bool exact = lead == 0 && d->dim == (int64_t)nt * elems && y_together;
+            // as many groups as threads, named barriers, shared memory and rows allow
+            int64_t groups = most / nt;
+            const int64_t fit = (kNormSmem - params) / (stages * row), spread = (d->rows + ds->sm_count - 1) / ds->sm_count;
+            if (groups > 15) groups = 15;
+            if (groups > fit) groups = fit;
+            if (groups > spread) groups = spread;
+            int64_t ctas = (d->rows + groups - 1) / groups;
+            if (ctas > ds->sm_count) ctas = ds->sm_count;
+            ctas = ctas / period * period;
+            if (ctas == 0) ctas = period;
+            const auto kernel = elems == VEC ? (exact ? layernorm_kernel<T, VEC, 1, true> : layernorm_kernel<T, VEC, 1, false>)
+                                : stages == 1 ? (exact ? layernorm_kernel<T, WIDE, 1, true> : layernorm_kernel<T, WIDE, 1, false>)
+                                              : (exact ? layernorm_kernel<T, WIDE, 2, true> : layernorm_kernel<T, WIDE, 2, false>);
+            static std::atomic<uint64_t> smem_set[6];
+            rc = ensure_dynamic_smem(smem_set[(elems == VEC ? 0 : 2 * stages) + exact], reinterpret_cast<const void*>(kernel), kNormSmem);
+            if (rc != NZB_OK) return rc;
+            kernel<<<(unsigned)ctas, (unsigned)(groups * nt), (size_t)(params + groups * stages * row), s>>>(
+                xp, gamma, beta, yp, mean, rstd, d->rows, (int)d->dim, d->ld_x, d->ld_y, d->eps, period, y_together, nt, (int)groups);
+        } else {
+            layernorm_long_kernel<T><<<(unsigned)d->rows, 1024, 0, s>>>(xp, gamma, beta, yp, mean, rstd, (int)d->dim, d->ld_x, d->ld_y, d->eps);
+        }
     });
     NZB_CUDA_TRY(cudaGetLastError());
     return NZB_OK;
@@ -416,16 +595,19 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
     const auto offset = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; };
     const bool together = offset(x) == offset(dy) && d->ld_x * size % 16 == d->ld_y * size % 16 &&
                           (!dx || (offset(x) == offset(dx) && d->ld_x * size % 16 == d->ld_dx * size % 16));
-    const int nt = together ? norm_threads(d->dim, d->dtype == NZB_F32 ? 4 : 8) : 0;
+    const int period = d->ld_x * size % 16 == 0 ? 1 : (int)(16 / size);
+    const int lead = period == 1 && aligned_to(x, 16) ? 0 : (int)(16 / size) - 1;
+    const int nt = together ? norm_threads(d->dim, lead, kNormBackwardMaxThreads, kNormElems) : 0;
     if (nt) {
-        const int period = d->ld_x * size % 16 == 0 ? 1 : (int)(16 / size);
         parts = parts / period * period;  // whole rounds of the residues: norm_parts gives eight at least
         NZB_DISPATCH_DTYPE(d->dtype, T, {
-            if (nt == 32) launch_norm_backward<T, 32>(d, dy, x, mean, rstd, gamma, dx, partial, period, (unsigned)parts, s);
-            else if (nt == 64) launch_norm_backward<T, 64>(d, dy, x, mean, rstd, gamma, dx, partial, period, (unsigned)parts, s);
-            else if (nt == 128) launch_norm_backward<T, 128>(d, dy, x, mean, rstd, gamma, dx, partial, period, (unsigned)parts, s);
-            else if (nt == 256) launch_norm_backward<T, 256>(d, dy, x, mean, rstd, gamma, dx, partial, period, (unsigned)parts, s);
-            else launch_norm_backward<T, 512>(d, dy, x, mean, rstd, gamma, dx, partial, period, (unsigned)parts, s);
+            constexpr int per_thread = kNormStages * 2 * (int)(kNormElems / Elem<T>::VEC) * 16 + kNormElems * 4;
+            const bool exact = period == 1 && lead == 0 && d->dim == (int64_t)nt * kNormElems;
+            const auto kernel = exact ? layernorm_backward_kernel<T, true> : layernorm_backward_kernel<T, false>;
+            static std::atomic<uint64_t> smem_set[2];
+            rc = ensure_dynamic_smem(smem_set[exact], reinterpret_cast<const void*>(kernel), kNormBackwardMaxThreads * per_thread);
+            if (rc != NZB_OK) return rc;
+            kernel<<<(unsigned)parts, nt, nt * per_thread, s>>>(static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, gamma, static_cast<T*>(dx), partial, d->rows, (int)d->dim, d->ld_x, d->ld_y, d->ld_dx, period, !d->overwrite_dx);
         });
     } else {
         NZB_DISPATCH_DTYPE(d->dtype, T, {
