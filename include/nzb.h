@@ -544,9 +544,9 @@ NZB_API int nzb_layernorm_backward(const nzb_layernorm_desc* desc, const void* d
  *   top_logprob / top_index {rows, top_k}: the top_k largest logits' log probabilities and columns, largest
  *   first, equal ones by the lower column (top_k <= 32 and <= vocab).
  * Any output may be null. Targets and top_index have the type index_type. A target outside [0, vocab) stands
- * for a position without one: its logprob is 0. Logits of -inf (or of the type's lowest value) are masked:
- * probability 0. A row without a z above -1e30 is empty: lse and its log probabilities are -inf, its entropy
- * is 0. A NaN in a row makes the row's results NaN; it ranks last among the alternatives.
+ * for a position without one: its logprob is 0. Logits of -2^27 and less (-inf, -1e9, the lowest fp32 or bf16
+ * number) are masked: probability 0 beside any other. A row of masked logits is empty: lse and its log
+ * probabilities are -inf, its entropy is 0. A NaN or +inf in a row makes the row's results NaN; a NaN ranks with -inf among the alternatives.
  * Backward: dlogits = scale * (dlogprob * (1[target] - p) - dentropy * p * (ln p + entropy)), from lse and
  * entropy of the forward pass; dlogprob or dentropy may be null (0), entropy too when dentropy is. Rows that
  * are empty get zeros; positions without a target only the entropy's part. dlogits may be logits.

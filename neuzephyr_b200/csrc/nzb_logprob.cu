@@ -1,19 +1,23 @@
 // Log probabilities of given tokens with entropy and the top alternatives, and their gradient. Beside the softmax
 // and binary-cross-entropy head: the loss of a model whose answer is one of `vocab` tokens.
 //
-// With z = scale x over a row: lse = ln sum exp z, logprob = z_t - lse, H = lse - sum p z.
-// One walk over the row: every thread keeps the running maximum m of its logits, s = sum e and w = sum e u with
-// u = (x - m) scale and e = exp u; when m grows by d, w = f (w + d s) and s = f s with f = exp(d), d < 0. Two such
-// triples join the same way, so ln s and H = ln s - w / s need no second walk and cancel nothing (w <= 0).
-#include "nzb_internal.h"
+// With z = scale x over a row: lse = ln sum exp z, logprob = z_t - lse, H = lse - sum p z. Everything is in powers of
+// two, k = scale log2(e). One walk over the row: every thread keeps its largest logit m, s = sum e and w = sum e u with
+// u = (x - m) k and e = 2^u; when m grows by d / k, u falls by d: w = f (w - d s), s = f s with f = 2^-d. Two such
+// triples join the same way, so log2 s and H = (log2 s - w / s) ln 2 need no second walk and cancel nothing (w <= 0).
+// Logits are read as no less than -2^27, so that a masked one (-inf, -1e9, the type's lowest) has e = 0 and e u = 0.
+#include <cooperative_groups.h>
+
 #include "nzb_elem.cuh"
+#include "nzb_internal.h"
 
 namespace nzb {
 
-constexpr float kEmptyRow = -1e30f;  // a row without a z above this has nothing left to choose from
+namespace cg = cooperative_groups;
+
+constexpr float kEmpty = -134217728.f;  // -2^27, exact in bf16: a row without a logit above it has nothing left to choose from
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -26,22 +30,67 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return y;
 }
 
-// Running sums of a part of a row. u is in units of ln 2 / scale: u2 = (x - m) scale log2(e).
+// A 16-byte block of logits: -inf beyond the row.
+template <typename T>
+__device__ __forceinline__ uint4 load_logits(const T* row, int first, int n) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (first >= 0 && first + VEC <= n) return __ldcs(reinterpret_cast<const uint4*>(row + first));
+    union { uint4 u; T e[VEC]; } b;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) b.e[i] = first + i >= 0 && first + i < n ? row[first + i] : Elem<T>::from(-INFINITY);
+    return b.u;
+}
+// Largest element of a block, NaN left out.
+__device__ __forceinline__ float block_max(const uint4& u, float) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+__device__ __forceinline__ float block_max(const uint4& u, __half) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float block_max(const uint4& u, __nv_bfloat16) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+// The elements of a block as floats no less than kEmpty, NaN kept. bf16 has the range, so two are raised at once.
+__device__ __forceinline__ void unpack_raised(const uint4& u, float (&f)[4], float) {
+    Elem<float>::unpack(u, f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = max_nan(f[i], kEmpty);
+}
+__device__ __forceinline__ void unpack_raised(const uint4& u, float (&f)[8], __half) {
+    Elem<__half>::unpack(u, f);
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = max_nan(f[i], kEmpty);
+}
+__device__ __forceinline__ void unpack_raised(const uint4& u, float (&f)[8], __nv_bfloat16) {
+    uint4 r = u;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&r);
+    const __nv_bfloat162 low = __float2bfloat162_rn(kEmpty);
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = __hmax2_nan(h[i], low);
+    Elem<__nv_bfloat16>::unpack(r, f);
+}
+
+// Running sums of a part of a row.
 struct RowSums {
-    float m, s, w;  // m: largest logit (unscaled); w = sum e * u2
+    float top;   // largest logit, raised
+    float s, w;  // sum e, sum e u
 };
 __device__ __forceinline__ RowSums join(const RowSums& a, const RowSums& b, float k) {
-    RowSums r;
-    r.m = fmaxf(a.m, b.m);
-    // differences of finite numbers, at worst -inf; clamped so that 0 * u stays 0
-    const float ua = fmaxf((a.m - r.m) * k, -1000.f), ub = fmaxf((b.m - r.m) * k, -1000.f);
-    const float fa = exp2_fast(ua), fb = exp2_fast(ub);
-    r.s = a.s * fa + b.s * fb;
-    r.w = fa * (a.w + ua * a.s) + fb * (b.w + ub * b.s);
-    return r;
+    RowSums j;
+    j.top = fmaxf(a.top, b.top);
+    const float ua = (a.top - j.top) * k, ub = (b.top - j.top) * k, fa = exp2_fast(ua), fb = exp2_fast(ub);
+    j.s = fa * a.s + fb * b.s;
+    j.w = fa * fmaf(ua, a.s, a.w) + fb * fmaf(ub, b.s, b.w);
+    return j;
 }
 
 constexpr int kLogprobThreads = 256;
+constexpr int kLogprobFly = 4;    // blocks in flight per thread
+constexpr int kLogprobCluster = 8;
 constexpr int kTopMax = 32;
 constexpr int kTopBuffer = 1024;  // candidates for the alternatives held in shared memory
 
@@ -65,11 +114,40 @@ struct TopSmem {
     int best_i[kLogprobThreads / 32];
 };
 
-// The top_k largest logits of a row into s.value / s.column [0, top_k), in order. lane_max[t] holds the largest
-// logit among the blocks t, t + threads, ... of the row: the top_k-th largest of these is a lower bound of the
-// top_k-th largest logit, so only the blocks of threads whose maximum reaches the bound are looked at again.
+// Orders the first `count` candidates (at most kTopBuffer) and leaves the top_k best in front.
+__device__ __forceinline__ void rank_candidates(TopSmem& s, int count, int top_k) {
+    constexpr int NT = kLogprobThreads, PER = kTopBuffer / NT;
+    const int t = threadIdx.x;
+    float v[PER];
+    int col[PER], at[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int i = t + j * NT;
+        at[j] = kTopBuffer;
+        if (i >= count) continue;
+        v[j] = s.value[i];
+        col[j] = s.column[i];
+        int before = 0;
+        for (int o = 0; o < count; o++) before += ranks_before(s.value[o], s.column[o], v[j], col[j]);
+        at[j] = before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        if (at[j] < top_k) {
+            s.value[at[j]] = v[j];
+            s.column[at[j]] = col[j];
+        }
+    }
+    __syncthreads();
+}
+
+// The top_k largest logits among the blocks [b0, b1) of a row into s.value / s.column [0, top_k), in order; fewer than
+// top_k elements are filled up with -inf in columns behind the row. lane_max[t] holds the largest logit of the blocks
+// b0 + t, b0 + t + threads, ...: the top_k-th largest of these is a lower bound of the top_k-th largest logit, so
+// only the blocks of threads whose maximum reaches the bound are looked at again.
 template <typename T>
-__device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int blocks, int top_k) {
+__device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int b0, int b1, int top_k) {
     constexpr int VEC = Elem<T>::VEC, NT = kLogprobThreads;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     if (t == 0) {
@@ -86,7 +164,7 @@ __device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int blocks
     if (mine >= bound) s.chosen[atomicAdd(&s.n_chosen, 1)] = t;
     __syncthreads();
     for (int c = warp; c < s.n_chosen; c += NT / 32) {
-        for (int b = s.chosen[c] + lane * NT; b < blocks; b += 32 * NT) {
+        for (int b = b0 + s.chosen[c] + lane * NT; b < b1; b += 32 * NT) {
             const int first = b * VEC - lead;
             union { uint4 u; T e[VEC]; } x;
             x.u = load_block(row, first, n);
@@ -105,32 +183,19 @@ __device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int blocks
         }
     }
     __syncthreads();
-    const int count = s.count;
+    const int c0 = max(0, b0 * VEC - lead), c1 = min(n, b1 * VEC - lead);
+    int count = s.count;
     if (count <= kTopBuffer) {
-        // at least top_k candidates: each finds its rank among them
-        constexpr int PER = kTopBuffer / NT;
-        float v[PER];
-        int col[PER], at[PER];
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = t + j * NT;
-            at[j] = kTopBuffer;
-            if (i >= count) continue;
-            v[j] = s.value[i];
-            col[j] = s.column[i];
-            int before = 0;
-            for (int o = 0; o < count; o++) before += ranks_before(s.value[o], s.column[o], v[j], col[j]);
-            at[j] = before;
-        }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            if (at[j] < top_k) {
-                s.value[at[j]] = v[j];
-                s.column[at[j]] = col[j];
+        if (count < top_k) {
+            if (t < top_k - count) {
+                s.value[count + t] = -INFINITY;
+                s.column[count + t] = n + count + t;
             }
+            count = top_k;
+            __syncthreads();
         }
-        __syncthreads();
+        rank_candidates(s, count, top_k);
         return;
     }
     // Too many logits reach the bound (long runs of equal ones): take the alternatives one after the other, each the
@@ -140,7 +205,7 @@ __device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int blocks
     for (int k = 0; k < top_k; k++) {
         float bv = -INFINITY;
         int bi = n;
-        for (int c = t; c < n; c += NT) {
+        for (int c = c0 + t; c < c1; c += NT) {
             const float v = rank_value(row[c]);
             if (ranks_before(last_v, last_i, v, c) && ranks_before(v, c, bv, bi)) {
                 bv = v;
@@ -178,55 +243,69 @@ __device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int blocks
     }
 }
 
-template <typename T, typename Index>
+// A row per CTA, or per cluster of CTAs when there are few rows: each takes a stretch of the row, and the first one
+// joins what the others left in their shared memory.
+template <typename T, typename Index, bool CLUSTER>
 __global__ void __launch_bounds__(kLogprobThreads)
 token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ targets, float* __restrict__ logprob,
                      float* __restrict__ entropy, float* __restrict__ lse_out, float* __restrict__ top_logprob,
-                     Index* __restrict__ top_index, int vocab, int64_t ld, float scale, int top_k) {
-    constexpr int VEC = Elem<T>::VEC, NT = kLogprobThreads;
+                     Index* __restrict__ top_index, int vocab, int64_t ld, float scale, int top_k, int parts) {
+    constexpr int VEC = Elem<T>::VEC, NT = kLogprobThreads, FLY = kLogprobFly;
     __shared__ RowSums warp_sums[NT / 32];
-    __shared__ RowSums row_sums;
+    __shared__ RowSums cta_sums;
     __shared__ TopSmem top;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int64_t r = blockIdx.x;
+    const int part = CLUSTER ? blockIdx.x % parts : 0;
+    const int64_t r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
     const T* row = logits + r * ld;
     const int lead = row_lead(row);
     const int blocks = (vocab + lead + VEC - 1) / VEC;
+    const int per = CLUSTER ? (blocks + parts - 1) / parts : blocks;
+    const int b0 = min(blocks, part * per), b1 = min(blocks, b0 + per);
     const float k = scale * kLog2e;
-    RowSums a = {kLowest, 0.f, 0.f};
+    const float2 k2 = make_float2(k, k);
+    RowSums a = {kEmpty, 0.f, 0.f};
     float seen = -INFINITY;  // largest logit of this thread's, NaN left out
-    for (int b = t; b < blocks; b += NT) {
-        const int first = b * VEC - lead;
-        float f[VEC];
-        if (first >= 0 && first + VEC <= vocab) {
-            Elem<T>::unpack(*reinterpret_cast<const uint4*>(row + first), f);
-        } else {
+    float2 s2 = make_float2(0.f, 0.f), w2 = s2;
+    for (int b = b0 + t; b < b1; b += NT * FLY) {
+        uint4 u[FLY];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) f[i] = first + i >= 0 && first + i < vocab ? Elem<T>::to(row[first + i]) : -INFINITY;
+        for (int f = 0; f < FLY; f++) {
+            // past the end of the stretch: the first block's place, given no weight below
+            const int at = b + f * NT;
+            u[f] = at < b1 ? load_logits(row, at * VEC - lead, vocab) : load_logits(row, vocab, vocab);
         }
-        float mx = f[0];
+        float mx = block_max(u[0], T());
 #pragma unroll
-        for (int i = 1; i < VEC; i++) mx = fmaxf(mx, f[i]);
+        for (int f = 1; f < FLY; f++) mx = fmaxf(mx, block_max(u[f], T()));
         seen = fmaxf(seen, mx);
-        if (mx > a.m) {
-            const float u = fmaxf((a.m - mx) * k, -1000.f), fac = exp2_fast(u);
-            a.w = fac * (a.w + u * a.s);
-            a.s *= fac;
-            a.m = mx;
+        if (mx > a.top) {
+            const float d = (a.top - mx) * k, fac = exp2_fast(d);
+            w2 = make_float2(fac * fmaf(d, s2.x, w2.x), fac * fmaf(d, s2.y, w2.y));
+            s2 = make_float2(fac * s2.x, fac * s2.y);
+            a.top = mx;
         }
+        const float2 minus = make_float2(-a.top, -a.top);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const float u = max_nan((f[i] - a.m) * k, -1000.f);
-            const float e = exp2_fast(u);
-            a.s += e;
-            a.w = fmaf(e, u, a.w);
+        for (int f = 0; f < FLY; f++) {
+            float x[VEC];
+            unpack_raised(u[f], x, T());
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+                const float2 v = mul2(add2(make_float2(x[i], x[i + 1]), minus), k2);
+                const float2 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+                s2 = add2(s2, e);
+                w2 = fma2(e, v, w2);
+            }
         }
     }
+    a.s = s2.x + s2.y;
+    a.w = w2.x + w2.y;
     if (top_k) top.lane_max[t] = seen;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         RowSums b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+        b.top = __shfl_xor_sync(0xffffffffu, a.top, o);
         b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
         b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
         // both lanes of a pair join in the same order, so that they agree
@@ -236,66 +315,130 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
     __syncthreads();
     if (t == 0) {
         for (int w = 1; w < NT / 32; w++) a = join(a, warp_sums[w], k);
-        row_sums = a;
-        const bool empty = a.m * scale <= kEmptyRow || a.s == 0.f;
-        const float log_s = logf(a.s);
-        if (lse_out) lse_out[r] = empty ? (a.s == a.s ? -INFINITY : a.s) : a.m * scale + log_s;
-        if (entropy) entropy[r] = empty ? (a.s == a.s ? 0.f : a.s) : log_s - a.w / a.s * kLn2;
+        cta_sums = a;
+    }
+    if (top_k) top_of_row(top, row, vocab, lead, b0, b1, top_k);
+    if (CLUSTER) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (part == 0) {
+            if (t == 0) {
+                for (int p = 1; p < parts; p++) a = join(a, *cluster.map_shared_rank(&cta_sums, p), k);
+                cta_sums = a;
+            }
+            if (top_k) {
+                for (int i = top_k + t; i < top_k * parts; i += NT) {
+                    const int p = i / top_k, j = i - p * top_k;
+                    top.value[i] = *cluster.map_shared_rank(&top.value[j], p);
+                    top.column[i] = *cluster.map_shared_rank(&top.column[j], p);
+                }
+                __syncthreads();
+                rank_candidates(top, top_k * parts, top_k);
+            }
+        }
+        cluster.sync();  // nobody leaves while the first CTA may still read
+        if (part) return;
+    }
+    __syncthreads();
+    const RowSums all = cta_sums;
+    const bool empty = all.top <= kEmpty && all.s == all.s;
+    const float log_s = log2f(all.s);
+    if (t == 0) {
+        if (lse_out) lse_out[r] = empty ? -INFINITY : fmaf(all.top, scale, log_s * kLn2);
+        if (entropy) entropy[r] = empty ? 0.f : (log_s - all.w / all.s) * kLn2;
         if (logprob) {
             const int64_t tgt = static_cast<int64_t>(targets[r]);
             float lp = 0.f;
-            if (tgt >= 0 && tgt < vocab) lp = empty ? (a.s == a.s ? -INFINITY : a.s) : (Elem<T>::to(row[tgt]) - a.m) * scale - log_s;
+            if (tgt >= 0 && tgt < vocab) lp = empty ? -INFINITY : fmaf(Elem<T>::to(row[tgt]) - all.top, scale, -log_s * kLn2);
             logprob[r] = lp;
         }
     }
-    if (!top_k) return;
-    __syncthreads();
-    top_of_row(top, row, vocab, lead, blocks, top_k);
-    const RowSums all = row_sums;
     if (t < top_k) {
-        const bool empty = all.m * scale <= kEmptyRow || all.s == 0.f;
-        if (top_logprob) top_logprob[r * top_k + t] = empty && all.s == all.s ? -INFINITY : (top.value[t] - all.m) * scale - logf(all.s);
+        if (top_logprob) top_logprob[r * top_k + t] = empty ? -INFINITY : fmaf(top.value[t] - all.top, scale, -log_s * kLn2);
         if (top_index) top_index[r * top_k + t] = static_cast<Index>(top.column[t]);
     }
 }
 
-// dlogits = scale (dl (1[target] - p) - dH p (ln p + H)), p = exp(z - lse).
-template <typename T, typename Index>
+// dlogits = scale (dl (1[target] - p) - dH p (ln p + H)), p = e^q with q = z - lse in one rounding (ln p near 0 counts).
+template <typename T, typename Index, bool ENTROPY>
 __global__ void __launch_bounds__(256)
 token_logprob_backward_kernel(const T* logits, const Index* __restrict__ targets, const float* __restrict__ lse,
                               const float* __restrict__ entropy, const float* __restrict__ dlogprob,
                               const float* __restrict__ dentropy, T* dlogits, int vocab, int64_t ld, int64_t ld_d, float scale) {
-    constexpr int VEC = Elem<T>::VEC;
+    constexpr int VEC = Elem<T>::VEC, FLY = kLogprobFly;
     const int64_t r = blockIdx.y;
     const T* row = logits + r * ld;
     T* out = dlogits + r * ld_d;
     const int lead = row_lead(row);
-    const bool same = row_lead(out) == lead;
     const int blocks = (vocab + lead + VEC - 1) / VEC;
+    const int b0 = blockIdx.x * (256 * FLY) + threadIdx.x;
+    uint4 u[FLY];
+#pragma unroll
+    for (int f = 0; f < FLY; f++)
+        if (b0 + f * 256 < blocks) u[f] = load_logits(row, (b0 + f * 256) * VEC - lead, vocab);
+    const bool same = row_lead(out) == lead;
     const int64_t tgt = static_cast<int64_t>(targets[r]);
     const bool has = tgt >= 0 && tgt < vocab;
-    const float l = lse[r], dl = dlogprob && has ? dlogprob[r] : 0.f, dh = dentropy ? dentropy[r] : 0.f, H = dentropy ? entropy[r] : 0.f;
-    const bool empty = l <= kEmptyRow;
-    const float c0 = -scale * (dl + dh * H), c1 = -scale * dh;
-    for (int b = blockIdx.x * 256 + threadIdx.x; b < blocks; b += gridDim.x * 256) {
-        const int first = b * VEC - lead;
-        float f[VEC];
-        Elem<T>::unpack(load_block(row, first, vocab), f);
+    const float l = lse[r], dl = dlogprob && has ? dlogprob[r] : 0.f, dh = ENTROPY ? dentropy[r] : 0.f, H = ENTROPY ? entropy[r] : 0.f;
+    const bool empty = l == -INFINITY;
+    const float c0 = empty ? 0.f : -scale * (dl + dh * H), c1 = empty ? 0.f : -scale * dh;
+    const float base = empty ? 0.f : -l;
+    const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base), log2e2 = make_float2(kLog2e, kLog2e), c02 = make_float2(c0, c0), c12 = make_float2(c1, c1);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const float q = max_nan(fmaf(f[i], scale, -l), -1000.f);  // ln p
-            const float p = exp2_fast(q * kLog2e);
-            f[i] = empty ? 0.f : p * fmaf(c1, q, c0);
-            if (first + i == tgt && has && !empty) f[i] += scale * dl;
+    for (int f = 0; f < FLY; f++) {
+        const int b = b0 + f * 256, first = b * VEC - lead;
+        if (b >= blocks) break;
+        float x[VEC];
+        if (ENTROPY) unpack_raised(u[f], x, T());  // p ln p of a masked logit is 0
+        else Elem<T>::unpack(u[f], x);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const float2 q = fma2(make_float2(x[i], x[i + 1]), scale2, base2), q2 = mul2(q, log2e2);
+            const float2 p = make_float2(exp2_fast(q2.x), exp2_fast(q2.y));
+            const float2 d = mul2(p, ENTROPY ? fma2(c12, q, c02) : c02);
+            x[i] = d.x;
+            x[i + 1] = d.y;
+        }
+        if (empty) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) x[i] = 0.f;
+        } else if (has && tgt >= first && tgt < first + VEC) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++)
+                if (first + i == tgt) x[i] = fmaf(scale, dl, x[i]);
         }
         if (same) {
-            store_block(out, first, vocab, Elem<T>::pack(f));
+            store_block(out, first, vocab, Elem<T>::pack(x));
         } else {
 #pragma unroll
             for (int i = 0; i < VEC; i++)
-                if (first + i >= 0 && first + i < vocab) out[first + i] = Elem<T>::from(f[i]);
+                if (first + i >= 0 && first + i < vocab) out[first + i] = Elem<T>::from(x[i]);
         }
     }
+}
+
+template <typename T, typename Index>
+static int launch_logprob(const nzb_token_logprob_desc* d, const void* logits, const void* targets, float* logprob, float* entropy,
+                          float* lse, float* top_logprob, void* top_index, int top_k, int sm_count, cudaStream_t s) {
+    const int64_t blocks = (d->vocab + Elem<T>::VEC - 1) / Elem<T>::VEC;
+    // few rows: more CTAs share one, as long as each thread keeps a round of blocks
+    int parts = 1;
+    while (parts < kLogprobCluster && d->rows * parts < 2 * sm_count && blocks >= (int64_t)parts * 2 * kLogprobThreads * kLogprobFly) parts *= 2;
+    cudaLaunchConfig_t cfg = {};
+    if (d->rows * parts > INT32_MAX) return fail(NZB_ERR_UNSUPPORTED, "too many rows");
+    cfg.gridDim = dim3((unsigned)(d->rows * parts));
+    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    const auto kernel = parts > 1 ? token_logprob_kernel<T, Index, true> : token_logprob_kernel<T, Index, false>;
+    NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<const Index*>(targets), logprob, entropy,
+                                    lse, top_logprob, static_cast<Index*>(top_index), (int)d->vocab, d->ld_logits, d->scale, top_k, parts));
+    return NZB_OK;
 }
 
 static int check_logprob(const nzb_token_logprob_desc* d) {
@@ -330,16 +473,10 @@ int nzb_token_logprob_forward(const nzb_token_logprob_desc* d, const void* logit
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int top_k = top_logprob || top_index ? d->top_k : 0;
     NZB_DISPATCH_DTYPE(d->dtype, T, {
-        const T* x = static_cast<const T*>(logits);
-        if (d->index_type == NZB_I64)
-            token_logprob_kernel<T, int64_t><<<(unsigned)d->rows, kLogprobThreads, 0, s>>>(
-                x, static_cast<const int64_t*>(targets), logprob, entropy, lse, top_logprob, static_cast<int64_t*>(top_index), (int)d->vocab, d->ld_logits, d->scale, top_k);
-        else
-            token_logprob_kernel<T, int32_t><<<(unsigned)d->rows, kLogprobThreads, 0, s>>>(
-                x, static_cast<const int32_t*>(targets), logprob, entropy, lse, top_logprob, static_cast<int32_t*>(top_index), (int)d->vocab, d->ld_logits, d->scale, top_k);
+        rc = d->index_type == NZB_I64 ? launch_logprob<T, int64_t>(d, logits, targets, logprob, entropy, lse, top_logprob, top_index, top_k, ds->sm_count, s)
+                                      : launch_logprob<T, int32_t>(d, logits, targets, logprob, entropy, lse, top_logprob, top_index, top_k, ds->sm_count, s);
     });
-    NZB_CUDA_TRY(cudaGetLastError());
-    return NZB_OK;
+    return rc;
 }
 
 int nzb_token_logprob_backward(const nzb_token_logprob_desc* d, const void* logits, const void* targets, const float* lse,
@@ -358,7 +495,7 @@ int nzb_token_logprob_backward(const nzb_token_logprob_desc* d, const void* logi
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     NZB_DISPATCH_DTYPE(d->dtype, T, {
         const int64_t blocks = (d->vocab + Elem<T>::VEC - 1) / Elem<T>::VEC + 1;
-        int64_t gx = (blocks + 1023) / 1024;
+        const int64_t gx = (blocks + 256 * kLogprobFly - 1) / (256 * kLogprobFly);
         for (int64_t r0 = 0; r0 < d->rows; r0 += 65535) {
             const int64_t n = d->rows - r0 < 65535 ? d->rows - r0 : 65535;
             const dim3 grid((unsigned)gx, (unsigned)n);
@@ -367,10 +504,11 @@ int nzb_token_logprob_backward(const nzb_token_logprob_desc* d, const void* logi
             const float* ent = dentropy ? entropy + r0 : nullptr;
             const float* dlp = dlogprob ? dlogprob + r0 : nullptr;
             const float* dent = dentropy ? dentropy + r0 : nullptr;
-            if (d->index_type == NZB_I64)
-                token_logprob_backward_kernel<T, int64_t><<<grid, 256, 0, s>>>(x, static_cast<const int64_t*>(targets) + r0, lse + r0, ent, dlp, dent, o, (int)d->vocab, d->ld_logits, d->ld_dlogits, d->scale);
-            else
-                token_logprob_backward_kernel<T, int32_t><<<grid, 256, 0, s>>>(x, static_cast<const int32_t*>(targets) + r0, lse + r0, ent, dlp, dent, o, (int)d->vocab, d->ld_logits, d->ld_dlogits, d->scale);
+            const auto launch = [&](auto kernel, auto index) {
+                kernel<<<grid, 256, 0, s>>>(x, static_cast<const decltype(index)*>(targets) + r0, lse + r0, ent, dlp, dent, o, (int)d->vocab, d->ld_logits, d->ld_dlogits, d->scale);
+            };
+            if (d->index_type == NZB_I64) launch(dentropy ? token_logprob_backward_kernel<T, int64_t, true> : token_logprob_backward_kernel<T, int64_t, false>, int64_t());
+            else launch(dentropy ? token_logprob_backward_kernel<T, int32_t, true> : token_logprob_backward_kernel<T, int32_t, false>, int32_t());
         }
     });
     NZB_CUDA_TRY(cudaGetLastError());
