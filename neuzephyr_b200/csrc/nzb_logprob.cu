@@ -90,7 +90,7 @@ __device__ __forceinline__ RowSums join(const RowSums& a, const RowSums& b, floa
 
 constexpr int kLogprobThreads = 256;
 constexpr int kLogprobFly = 4;    // blocks in flight per thread
-constexpr int kLogprobCluster = 8;
+constexpr int kLogprobCluster = 8;  // CTAs that share a row, at most; lanes of a join too
 constexpr int kTopMax = 32;
 constexpr int kTopBuffer = 1024;  // candidates for the alternatives held in shared memory
 
@@ -142,48 +142,100 @@ __device__ __forceinline__ void rank_candidates(TopSmem& s, int count, int top_k
     __syncthreads();
 }
 
-// The top_k largest logits among the blocks [b0, b1) of a row into s.value / s.column [0, top_k), in order; fewer than
-// top_k elements are filled up with -inf in columns behind the row. lane_max[t] holds the largest logit of the blocks
-// b0 + t, b0 + t + threads, ...: the top_k-th largest of these is a lower bound of the top_k-th largest logit, so
-// only the blocks of threads whose maximum reaches the bound are looked at again.
+// The part of a row that a CTA looks at. Whole 16-byte blocks [w0, w1) go round the threads: thread t has w0 + t,
+// w0 + t + threads, ...; a first block that starts before the row is thread 0's too, a last one that ends behind it thread
+// 1's (-1: there is none).
+struct Stretch {
+    int w0, w1, head, tail;
+    int lead;
+};
+__device__ __forceinline__ Stretch make_stretch(int vocab, int lead, int vec, int part, int parts) {
+    Stretch st;
+    st.lead = lead;
+    const int blocks = (vocab + lead + vec - 1) / vec, per = (blocks + parts - 1) / parts;
+    const int b0 = min(blocks, part * per), b1 = min(blocks, b0 + per);
+    const int first = lead ? 1 : 0, last = (vocab + lead) / vec;  // the row's whole blocks
+    st.w0 = max(b0, first);
+    st.w1 = max(st.w0, min(b1, last));
+    st.head = b0 == 0 && b1 > 0 && (lead || last == 0) ? 0 : -1;
+    st.tail = b1 == blocks && b1 > b0 && last < blocks && last > 0 ? last : -1;
+    return st;
+}
+
+// The top_k-th largest of a CTA's 256 values, by one warp: rounds of the largest one left.
+__device__ __forceinline__ float kth_largest(const float* value, int top_k, int lane) {
+    uint32_t key[kLogprobThreads / 32], mine = 0;
+#pragma unroll
+    for (int j = 0; j < kLogprobThreads / 32; j++) {
+        const uint32_t u = __float_as_uint(value[lane + 32 * j]);
+        key[j] = u & 0x80000000u ? ~u : u | 0x80000000u;  // unsigned numbers in the floats' order
+        mine = max(mine, key[j]);
+    }
+    uint32_t best = 0;
+    for (int i = 0; i < top_k; i++) {
+        best = __reduce_max_sync(0xffffffffu, mine);
+        const uint32_t holders = __ballot_sync(0xffffffffu, mine == best);
+        if (lane == __ffs(holders) - 1) {
+            bool taken = false;
+            mine = 0;
+#pragma unroll
+            for (int j = 0; j < kLogprobThreads / 32; j++) {
+                if (!taken && key[j] == best) {
+                    key[j] = 0;
+                    taken = true;
+                }
+                mine = max(mine, key[j]);
+            }
+        }
+    }
+    return __uint_as_float(best & 0x80000000u ? best & 0x7fffffffu : ~best);
+}
+
+// The top_k largest logits of a stretch into s.value / s.column [0, top_k), in order; fewer than top_k elements are
+// filled up with -inf in columns behind the row. lane_max[t] holds the largest of thread t's logits: the top_k-th
+// largest of these is a lower bound of the top_k-th largest logit, so only the blocks of threads whose maximum
+// reaches the bound are looked at again.
 template <typename T>
-__device__ void top_of_row(TopSmem& s, const T* row, int n, int lead, int b0, int b1, int top_k) {
+__device__ void top_of_row(TopSmem& s, const T* row, int n, const Stretch& st, int top_k) {
     constexpr int VEC = Elem<T>::VEC, NT = kLogprobThreads;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    if (t == 0) {
-        s.count = s.n_chosen = 0;
-        s.bound = -INFINITY;
-    }
+    const int lead = st.lead;
+    if (t == 0) s.count = s.n_chosen = 0;
     __syncthreads();
     const float mine = s.lane_max[t];
-    int rank = 0;
-    for (int i = 0; i < NT; i++) rank += ranks_before(s.lane_max[i], i, mine, t);
-    if (rank == top_k - 1) s.bound = mine;
+    if (warp == 0) {
+        const float bound = kth_largest(s.lane_max, top_k, lane);
+        if (lane == 0) s.bound = bound;
+    }
     __syncthreads();
     const float bound = s.bound;
     if (mine >= bound) s.chosen[atomicAdd(&s.n_chosen, 1)] = t;
     __syncthreads();
-    for (int c = warp; c < s.n_chosen; c += NT / 32) {
-        for (int b = b0 + s.chosen[c] + lane * NT; b < b1; b += 32 * NT) {
-            const int first = b * VEC - lead;
-            union { uint4 u; T e[VEC]; } x;
-            x.u = load_block(row, first, n);
+    const auto look = [&](int b) {
+        const int first = b * VEC - lead;
+        union { uint4 u; T e[VEC]; } x;
+        x.u = load_logits(row, first, n);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const int col = first + i;
-                const float v = rank_value(x.e[i]);
-                if (col >= 0 && col < n && v >= bound) {
-                    const int at = atomicAdd(&s.count, 1);
-                    if (at < kTopBuffer) {
-                        s.value[at] = v;
-                        s.column[at] = col;
-                    }
+        for (int i = 0; i < VEC; i++) {
+            const int col = first + i;
+            const float v = rank_value(x.e[i]);
+            if (v >= bound && col >= 0 && col < n) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kTopBuffer) {
+                    s.value[at] = v;
+                    s.column[at] = col;
                 }
             }
         }
+    };
+    for (int c = warp; c < s.n_chosen; c += NT / 32) {
+        const int who = s.chosen[c];
+        for (int b = st.w0 + who + lane * NT; b < st.w1; b += 32 * NT) look(b);
+        if (lane == 0 && who == 0 && st.head >= 0) look(st.head);
+        if (lane == 1 && who == 1 && st.tail >= 0) look(st.tail);
     }
     __syncthreads();
-    const int c0 = max(0, b0 * VEC - lead), c1 = min(n, b1 * VEC - lead);
+    const int c0 = st.head >= 0 ? 0 : st.w0 * VEC - lead, c1 = st.tail >= 0 || st.w1 <= st.w0 ? n : st.w1 * VEC - lead;
     int count = s.count;
     if (count <= kTopBuffer) {
         __syncthreads();
@@ -259,25 +311,17 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
     const int64_t r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
     const T* row = logits + r * ld;
     const int lead = row_lead(row);
-    const int blocks = (vocab + lead + VEC - 1) / VEC;
-    const int per = CLUSTER ? (blocks + parts - 1) / parts : blocks;
-    const int b0 = min(blocks, part * per), b1 = min(blocks, b0 + per);
+    const Stretch st = make_stretch(vocab, lead, VEC, part, CLUSTER ? parts : 1);
     const float k = scale * kLog2e;
     const float2 k2 = make_float2(k, k);
     RowSums a = {kEmpty, 0.f, 0.f};
     float seen = -INFINITY;  // largest logit of this thread's, NaN left out
     float2 s2 = make_float2(0.f, 0.f), w2 = s2;
-    for (int b = b0 + t; b < b1; b += NT * FLY) {
-        uint4 u[FLY];
-#pragma unroll
-        for (int f = 0; f < FLY; f++) {
-            // past the end of the stretch: the first block's place, given no weight below
-            const int at = b + f * NT;
-            u[f] = at < b1 ? load_logits(row, at * VEC - lead, vocab) : load_logits(row, vocab, vocab);
-        }
+    const auto take = [&](const auto& u) {
+        constexpr int N = sizeof(u) / sizeof(uint4);
         float mx = block_max(u[0], T());
 #pragma unroll
-        for (int f = 1; f < FLY; f++) mx = fmaxf(mx, block_max(u[f], T()));
+        for (int f = 1; f < N; f++) mx = fmaxf(mx, block_max(u[f], T()));
         seen = fmaxf(seen, mx);
         if (mx > a.top) {
             const float d = (a.top - mx) * k, fac = exp2_fast(d);
@@ -287,7 +331,7 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
         }
         const float2 minus = make_float2(-a.top, -a.top);
 #pragma unroll
-        for (int f = 0; f < FLY; f++) {
+        for (int f = 0; f < N; f++) {
             float x[VEC];
             unpack_raised(u[f], x, T());
 #pragma unroll
@@ -298,6 +342,24 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
                 w2 = fma2(e, v, w2);
             }
         }
+    };
+    // whole blocks without any check, FLY of them in flight; what is left, one by one
+    const uint4* at = reinterpret_cast<const uint4*>(row + st.w0 * VEC - lead) + t;
+    int left = (st.w1 - st.w0 - t + NT - 1) / NT;  // of this thread
+    for (; left >= FLY; left -= FLY, at += FLY * NT) {
+        uint4 u[FLY];
+#pragma unroll
+        for (int f = 0; f < FLY; f++) u[f] = __ldcs(at + f * NT);
+        take(u);
+    }
+    for (; left > 0; left--, at += NT) {
+        const uint4 u[1] = {__ldcs(at)};
+        take(u);
+    }
+    const int cut = t == 0 ? st.head : t == 1 ? st.tail : -1;
+    if (cut >= 0) {
+        const uint4 u[1] = {load_logits(row, cut * VEC - lead, vocab)};
+        take(u);
     }
     a.s = s2.x + s2.y;
     a.w = w2.x + w2.y;
@@ -313,18 +375,32 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
     }
     if (lane == 0) warp_sums[warp] = a;
     __syncthreads();
-    if (t == 0) {
-        for (int w = 1; w < NT / 32; w++) a = join(a, warp_sums[w], k);
-        cta_sums = a;
+    // lanes 0..7 of the first warp hold the warps' (or, below, the CTAs') sums and join in pairs
+    const auto join_eight = [&](RowSums a) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            RowSums b;
+            b.top = __shfl_down_sync(0xffu, a.top, o);
+            b.s = __shfl_down_sync(0xffu, a.s, o);
+            b.w = __shfl_down_sync(0xffu, a.w, o);
+            a = join(a, b, k);
+        }
+        return a;
+    };
+    if (t < 8) {
+        a = join_eight(warp_sums[t]);
+        if (t == 0) cta_sums = a;
     }
-    if (top_k) top_of_row(top, row, vocab, lead, b0, b1, top_k);
+    if (top_k) top_of_row(top, row, vocab, st, top_k);
     if (CLUSTER) {
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         if (part == 0) {
-            if (t == 0) {
-                for (int p = 1; p < parts; p++) a = join(a, *cluster.map_shared_rank(&cta_sums, p), k);
-                cta_sums = a;
+            if (t < 8) {
+                const RowSums none = {kEmpty, 0.f, 0.f};
+                a = join_eight(t < parts ? *cluster.map_shared_rank(&cta_sums, t) : none);
+                __syncwarp(0xffu);
+                if (t == 0) cta_sums = a;
             }
             if (top_k) {
                 for (int i = top_k + t; i < top_k * parts; i += NT) {
