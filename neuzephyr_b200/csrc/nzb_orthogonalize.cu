@@ -55,11 +55,13 @@ struct NsCfg {
     static constexpr bool PAIR = PAIR_;
     static constexpr int BM = 128;                    // rows per CTA
     static constexpr int TILE = PAIR ? 256 : 128;     // the tile of a CTA, or of a pair, is square
-    static constexpr int STAGES = 6;
+    static constexpr int STAGES = 5;
+    static constexpr int EPI_WARPS = 8;               // two per quarter of the tensor-memory lanes, half the columns each
+    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int OPERAND_BYTES = 128 * 64 * 2;  // per CTA and operand: 128 rows x 64 k
     static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
     static constexpr int EPI_STRIDE = 36;
-    static constexpr int EPI_BYTES = 4 * 32 * EPI_STRIDE * 4;
+    static constexpr int EPI_BYTES = EPI_WARPS * 32 * EPI_STRIDE * 4;
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
     static constexpr int TMEM_COLS = 2 * TILE;
     static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB shared memory of an sm_100 CTA");
@@ -84,18 +86,28 @@ __device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32
     }
 }
 
-// Drains a quarter (32 rows) of a finished A or B tile: every lane holds one row, 32 columns at a time. Writes
-// the fp16 entries and, off the diagonal tiles, their mirror image.
-template <class Cfg, int MODE>
-__device__ __forceinline__ void ns_drain_symmetric(const NsParams& p, uint32_t tmem, int lane, int32_t b, int32_t row0,
-                                                   int32_t col_tile, bool mirror) {
+// Drains 32 rows x half the columns of a finished A or B tile: every lane holds one row, 32 columns at a time. Writes the
+// fp16 entries and, off the diagonal tiles, their mirror image. `ready` waits for the accumulator; what else a group of
+// columns needs is loaded before that, and for the next group before this one is written.
+template <class Cfg, int MODE, class Ready>
+__device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t tmem, int lane, int32_t b, int32_t row0,
+                                                   int32_t col_first, bool mirror, Ready ready) {
     using namespace ptx;
     __half* out = p.out16 + b * p.stride16;
     const int32_t row = row0 + lane;
     const bool row_ok = row < p.M;
+    const __half* gram = p.gram + b * p.stride16 + static_cast<int64_t>(row) * p.ld16;
+    uint4 g[4];
+    const auto fetch = [&](int32_t col0) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            g[j] = row_ok && col0 < p.N ? *reinterpret_cast<const uint4*>(gram + col0 + 8 * j) : make_uint4(0, 0, 0, 0);
+    };
+    if (MODE == NS_POLY) fetch(col_first);
+    if (!ready()) return false;
 #pragma unroll 1
-    for (int c0 = 0; c0 < Cfg::TILE; c0 += 32) {
-        const int32_t col0 = col_tile + c0;
+    for (int c0 = 0; c0 < Cfg::TILE / 2; c0 += 32) {
+        const int32_t col0 = col_first + c0;
         if (col0 >= p.N) break;  // warp-uniform; the padded leading dimension covers a started group of 32
         uint32_t v[32];
         tmem_ld_32x32(tmem + c0, v);
@@ -106,11 +118,6 @@ __device__ __forceinline__ void ns_drain_symmetric(const NsParams& p, uint32_t t
             for (int j = 0; j < 16; j++)
                 h[j] = __floats2half2_rn(__uint_as_float(v[2 * j]) * kNsUnscale, __uint_as_float(v[2 * j + 1]) * kNsUnscale);
         } else {
-            uint4 g[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                g[j] = row_ok ? *reinterpret_cast<const uint4*>(p.gram + b * p.stride16 + static_cast<int64_t>(row) * p.ld16 + col0 + 8 * j)
-                              : make_uint4(0, 0, 0, 0);
             const __half2* gh = reinterpret_cast<const __half2*>(g);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
@@ -123,6 +130,7 @@ __device__ __forceinline__ void ns_drain_symmetric(const NsParams& p, uint32_t t
                     p.diag[b * p.short_side + row] = p.c0 + (row == c ? x : y) * kNsUnscale;
                 h[j] = __floats2half2_rn(row == c ? 0.f : x, row == c + 1 ? 0.f : y);
             }
+            if (c0 + 32 < Cfg::TILE / 2) fetch(col0 + 32);
         }
         if (row_ok) {
             uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * p.ld16 + col0);
@@ -144,6 +152,7 @@ __device__ __forceinline__ void ns_drain_symmetric(const NsParams& p, uint32_t t
             }
         }
     }
+    return true;
 }
 
 __device__ __forceinline__ void ns_put_half4(__half* at, const float4& x) {
@@ -169,83 +178,103 @@ __device__ __forceinline__ void ns_put4(T* at, const float4& x, int n, bool vec)
         if (i < n) at[i] = Elem<T>::from(f[i]);
 }
 
-// Drains a quarter of a finished B X tile through shared memory, so that eight lanes share 128 bytes of a row of
-// X32, and completes the step: x = diag * x + product, or the result's element.
-template <class Cfg>
-__device__ __forceinline__ void ns_drain_apply(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b,
-                                               int32_t row0, int32_t col_tile) {
+// Drains 32 rows x half the columns of a finished B X tile through shared memory, so that eight lanes share 128 bytes of a
+// row of X32, and completes the step: x = diag * x + product, or the result's element. X32 does not depend on the
+// product, so a group's part is on its way before the accumulator is ready, the next group's before this one is
+// written (loaded where they are used they made the epilogue as long as the product).
+template <class Cfg, class Ready>
+__device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b,
+                                               int32_t row0, int32_t col_first, Ready ready) {
     using namespace ptx;
     const float* diag = p.diag + b * p.short_side;
-#pragma unroll 1
-    for (int c0 = 0; c0 < Cfg::TILE; c0 += 32) {
-        const int32_t col0 = col_tile + c0;
-        if (col0 >= p.N) break;  // warp-uniform
-        uint32_t v[32];
-        tmem_ld_32x32(tmem + c0, v);
-        tmem_ld_wait();
-        float4* dst = reinterpret_cast<float4*>(stage + lane * Cfg::EPI_STRIDE);
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
-                                 __uint_as_float(v[4 * j + 3]));
-        __syncwarp();
-        const int cl = (lane & 7) * 4;
+    const int cl = (lane & 7) * 4, rl = lane >> 3;  // this lane's columns within a group, and its first row
+    float* X = p.X32 + b * p.stridex + static_cast<int64_t>(row0 + rl) * p.ldx + cl;
+    float4 old[8], dc;
+    float dr[8];
+    const auto fetch = [&](int32_t col0) {
         const int32_t gc = col0 + cl;
-        float4 dc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (row0 + rl + 4 * i < p.M && gc < p.N) old[i] = *reinterpret_cast<const float4*>(X + static_cast<int64_t>(4 * i) * p.ldx + col0);
         if (p.by_column) {
             dc.x = gc < p.N ? diag[gc] : 0.f;
             dc.y = gc + 1 < p.N ? diag[gc + 1] : 0.f;
             dc.z = gc + 2 < p.N ? diag[gc + 2] : 0.f;
             dc.w = gc + 3 < p.N ? diag[gc + 3] : 0.f;
         }
+    };
+    fetch(col_first);
+    if (!p.by_column) {
 #pragma unroll
-        for (int rr = 0; rr < 32; rr += 4) {
-            const int r = rr + (lane >> 3);
-            const int32_t gr = row0 + r;
-            if (gr < p.M && gc < p.N) {
-                float4 x = *reinterpret_cast<const float4*>(stage + r * Cfg::EPI_STRIDE + cl);
-                float* xp = p.X32 + b * p.stridex + static_cast<int64_t>(gr) * p.ldx + gc;
-                const float4 o = *reinterpret_cast<const float4*>(xp);
-                if (!p.by_column) dc.x = dc.y = dc.z = dc.w = diag[gr];
-                constexpr float k = kNsUnscale * kNsUnscale;
-                x.x = fmaf(dc.x, o.x, x.x * k);
-                x.y = fmaf(dc.y, o.y, x.y * k);
-                x.z = fmaf(dc.z, o.z, x.z * k);
-                x.w = fmaf(dc.w, o.w, x.w * k);
-                if (p.out_kind == NS_OUT_STATE) {
-                    *reinterpret_cast<float4*>(xp) = x;  // the padded row holds whole groups of four
-                    x.x *= kNsScale; x.y *= kNsScale; x.z *= kNsScale; x.w *= kNsScale;
-                    ns_put_half4(p.out16 + b * p.stride16 + static_cast<int64_t>(gr) * p.ld16 + gc, x);
+        for (int i = 0; i < 8; i++) dr[i] = row0 + rl + 4 * i < p.M ? diag[row0 + rl + 4 * i] : 0.f;
+    }
+    if (!ready()) return false;
+#pragma unroll 1
+    for (int c0 = 0; c0 < Cfg::TILE / 2; c0 += 32) {
+        const int32_t col0 = col_first + c0;
+        if (col0 >= p.N) break;  // warp-uniform
+        {
+            uint32_t v[32];
+            tmem_ld_32x32(tmem + c0, v);
+            tmem_ld_wait();
+            float4* dst = reinterpret_cast<float4*>(stage + lane * Cfg::EPI_STRIDE);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                                     __uint_as_float(v[4 * j + 3]));
+        }
+        __syncwarp();
+        const int32_t gc = col0 + cl;
+        float4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = *reinterpret_cast<const float4*>(stage + (rl + 4 * i) * Cfg::EPI_STRIDE + cl);
+            constexpr float k = kNsUnscale * kNsUnscale;
+            const float4 d = p.by_column ? dc : make_float4(dr[i], dr[i], dr[i], dr[i]);
+            x[i].x = fmaf(d.x, old[i].x, x[i].x * k);
+            x[i].y = fmaf(d.y, old[i].y, x[i].y * k);
+            x[i].z = fmaf(d.z, old[i].z, x[i].z * k);
+            x[i].w = fmaf(d.w, old[i].w, x[i].w * k);
+        }
+        __syncwarp();
+        if (c0 + 32 < Cfg::TILE / 2) fetch(col0 + 32);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int32_t gr = row0 + rl + 4 * i;
+            if (gr >= p.M || gc >= p.N) continue;
+            if (p.out_kind == NS_OUT_STATE) {
+                *reinterpret_cast<float4*>(X + static_cast<int64_t>(4 * i) * p.ldx + col0) = x[i];  // the padded row holds whole groups of four
+                x[i].x *= kNsScale; x[i].y *= kNsScale; x[i].z *= kNsScale; x[i].w *= kNsScale;
+                ns_put_half4(p.out16 + b * p.stride16 + static_cast<int64_t>(gr) * p.ld16 + gc, x[i]);
+            } else {
+                const int64_t at = b * p.stride_out + static_cast<int64_t>(gr) * p.ld_out + gc;
+                const int n = p.N - gc;
+                if (p.out_kind == NS_OUT_F32) {
+                    ns_put4(static_cast<float*>(p.out) + at, x[i], n, p.out_vec);
+                } else if (p.out_kind == NS_OUT_F16) {
+                    ns_put4(static_cast<__half*>(p.out) + at, x[i], n, p.out_vec);
+                } else if (p.out_kind == NS_OUT_BF16) {
+                    ns_put4(static_cast<__nv_bfloat16*>(p.out) + at, x[i], n, p.out_vec);
                 } else {
-                    const int64_t at = b * p.stride_out + static_cast<int64_t>(gr) * p.ld_out + gc;
-                    const int n = p.N - gc;
-                    if (p.out_kind == NS_OUT_F32) {
-                        ns_put4(static_cast<float*>(p.out) + at, x, n, p.out_vec);
-                    } else if (p.out_kind == NS_OUT_F16) {
-                        ns_put4(static_cast<__half*>(p.out) + at, x, n, p.out_vec);
-                    } else if (p.out_kind == NS_OUT_BF16) {
-                        ns_put4(static_cast<__nv_bfloat16*>(p.out) + at, x, n, p.out_vec);
-                    } else {
-                        float* w = static_cast<float*>(p.out) + at;
-                        const float f[4] = {x.x, x.y, x.z, x.w};
+                    float* w = static_cast<float*>(p.out) + at;
+                    const float f[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (i < n) w[i] = fmaf(-p.w_step, f[i], p.w_keep * w[i]);
-                    }
+                    for (int j = 0; j < 4; j++)
+                        if (j < n) w[j] = fmaf(-p.w_step, f[j], p.w_keep * w[j]);
                 }
             }
         }
-        __syncwarp();
     }
+    return true;
 }
 
-// One product of all matrices. CTA layout (192 threads, persistent over the tiles): warp 0 TMA producer, warp 1
-// tensor-memory allocator and MMA issuer, warps 2-5 epilogue; two accumulators, so that a tile's epilogue runs
+// One product of all matrices. CTA layout (320 threads, persistent over the tiles): warp 0 TMA producer, warp 1
+// tensor-memory allocator and MMA issuer, warps 2-9 epilogue; two accumulators, so that a tile's epilogue runs
 // under the next tile's products. PAIR: two CTAs share a 256 x 256 tile (each loads its 128 rows of both operands).
 // Every wait is bounded; on expiry the CTA raises its abort flag, waits for its copies in flight, frees its tensor
 // memory and returns with NZB_ERR_DEVICE_TIMEOUT in the status word.
 template <class Cfg, int MODE>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
 ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsParams p) {
     using namespace ptx;
     constexpr bool PAIR = Cfg::PAIR;
@@ -274,7 +303,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(&tfull[a], 1);
-            mbar_init(&tempty[a], PAIR ? 8 : 4);
+            mbar_init(&tempty[a], (PAIR ? 2 : 1) * Cfg::EPI_WARPS);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -388,13 +417,18 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             int32_t mt, nt, b;
             ns_decode<MODE>(p, tile, mt, nt, b);
             const uint32_t acc = tcount & 1, aph = (tcount >> 1) & 1;
-            if (!mbar_wait_bounded(&tfull[acc], aph, abort_flag)) break;
-            __syncwarp();
-            tc_fence_after();
-            const int32_t row0 = mt * Cfg::TILE + (int32_t)rank * 128 + q * 32;
-            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::TILE;
-            if constexpr (MODE == NS_APPLY) ns_drain_apply<Cfg>(p, tmem, stage, lane, b, row0, nt * Cfg::TILE);
-            else ns_drain_symmetric<Cfg, MODE>(p, tmem, lane, b, row0, nt * Cfg::TILE, mt != nt);
+            const auto ready = [&] {
+                if (!mbar_wait_warp(&tfull[acc], aph, abort_flag)) return false;
+                tc_fence_after();
+                return true;
+            };
+            const int half = (warp - 2) >> 2;
+            const int32_t row0 = mt * Cfg::TILE + (int32_t)rank * 128 + q * 32, col_first = nt * Cfg::TILE + half * (Cfg::TILE / 2);
+            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::TILE + half * (Cfg::TILE / 2);
+            bool ok;
+            if constexpr (MODE == NS_APPLY) ok = ns_drain_apply<Cfg>(p, tmem, stage, lane, b, row0, col_first, ready);
+            else ok = ns_drain_symmetric<Cfg, MODE>(p, tmem, lane, b, row0, col_first, mt != nt, ready);
+            if (!ok) break;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -421,29 +455,78 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 }
 
 // ---- Frobenius norm and first state ---------------------------------------------------------------------------
-constexpr int kNormParts = 256;  // partial sums per matrix
+constexpr int kNormParts = 592;  // partial sums per matrix, at most
+
+// Both elementwise passes go over groups of eight elements of a row, a thread over every gridDim.x * 256-th group.
+struct NsGroups {
+    int64_t item, items;
+    uint32_t per_row;
+    __device__ __forceinline__ NsGroups(int64_t rows, int64_t cols)
+        : item(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x), per_row(static_cast<uint32_t>((cols + 7) / 8)) {
+        items = rows * per_row;
+    }
+    __device__ __forceinline__ bool more() const { return item < items; }
+    __device__ __forceinline__ void next() { item += static_cast<int64_t>(gridDim.x) * 256; }
+    __device__ __forceinline__ void at(int64_t& r, int64_t& c) const {
+        r = items >> 32 ? item / per_row : static_cast<uint32_t>(item) / per_row;
+        c = (item - r * per_row) * 8;
+    }
+};
+template <typename T>
+__device__ __forceinline__ void ns_load8(const T* row, int64_t c, int64_t cols, bool vec, float (&f)[8]) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (vec && c + 8 <= cols) {
+#pragma unroll
+        for (int h = 0; h < 8 / VEC; h++) {
+            float part[VEC];
+            Elem<T>::unpack(reinterpret_cast<const uint4*>(row + c)[h], part);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) f[h * VEC + i] = part[i];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = c + i < cols ? Elem<T>::to(row[c + i]) : 0.f;
+}
 
 // Sums of squares in 64 bits (fp32 squares leave the range from 1.8e19 on). For the Muon step the pass also updates
 // the momentum and leaves the matrix to orthogonalise in X32.
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256)
 ns_norm_kernel(const T* __restrict__ g, float* __restrict__ momentum, float* __restrict__ X32, double* __restrict__ partial,
-               int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float mu, int nesterov) {
+               int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float mu, int nesterov, int vec) {
     __shared__ double buf[8];
-    const int64_t b = blockIdx.y, n = rows * cols;
-    const T* from = g + b * stride_g;
+    const int64_t b = blockIdx.y;
     double sum = 0.0;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / cols, c = i - r * cols;
-        float v = Elem<T>::to(from[r * ld_g + c]);
+#pragma unroll 4
+    for (NsGroups it(rows, cols); it.more(); it.next()) {
+        int64_t r, c;
+        it.at(r, c);
+        float v[8];
+        ns_load8(g + b * stride_g + r * ld_g, c, cols, vec, v);
         if (MUON) {
-            float* m = momentum + b * n + i;
-            const float moved = fmaf(mu, *m, v);
-            *m = moved;
-            v = nesterov ? fmaf(mu, moved, v) : moved;
-            X32[(b * rows + r) * ldx + c] = v;
+            float m[8];
+            float* mp = momentum + (b * rows + r) * cols + c;
+            ns_load8(const_cast<const float*>(mp - c), c, cols, vec, m);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                m[i] = fmaf(mu, m[i], v[i]);
+                v[i] = nesterov ? fmaf(mu, m[i], v[i]) : m[i];
+            }
+            if (vec && c + 8 <= cols) {
+                reinterpret_cast<float4*>(mp)[0] = make_float4(m[0], m[1], m[2], m[3]);
+                reinterpret_cast<float4*>(mp)[1] = make_float4(m[4], m[5], m[6], m[7]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (c + i < cols) mp[i] = m[i];
+            }
+            float4* xp = reinterpret_cast<float4*>(X32 + (b * rows + r) * ldx + c);  // padded rows: whole groups
+            xp[0] = make_float4(v[0], v[1], v[2], v[3]);
+            xp[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
-        sum += static_cast<double>(v) * v;
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum += static_cast<double>(v[i]) * v[i];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -458,10 +541,11 @@ ns_norm_kernel(const T* __restrict__ g, float* __restrict__ momentum, float* __r
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256)
 ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __restrict__ X16, const double* __restrict__ partial,
-                int parts, int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float eps) {
+                int parts, int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float eps, int vec) {
     __shared__ double buf[8];
-    const int64_t b = blockIdx.y, n = rows * cols;
-    double sum = threadIdx.x < parts ? partial[b * kNormParts + threadIdx.x] : 0.0;
+    const int64_t b = blockIdx.y;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) sum += partial[b * kNormParts + i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = sum;
@@ -469,11 +553,26 @@ ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __rest
     sum = 0.0;
     for (int w = 0; w < 8; w++) sum += buf[w];
     const float div = static_cast<float>(sqrt(sum) + eps);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / cols, c = i - r * cols, at = (b * rows + r) * ldx + c;
-        const float x = (MUON ? X32[at] : Elem<T>::to(g[b * stride_g + r * ld_g + c])) / div;
-        X32[at] = x;
-        X16[at] = __float2half_rn(x * kNsScale);
+#pragma unroll 2
+    for (NsGroups it(rows, cols); it.more(); it.next()) {
+        int64_t r, c;
+        it.at(r, c);
+        float v[8];
+        const int64_t at = (b * rows + r) * ldx + c;
+        if (MUON) ns_load8(const_cast<const float*>(X32 + at - c), c, ldx, true, v);
+        else ns_load8(g + b * stride_g + r * ld_g, c, cols, vec, v);
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = v[i] / div;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 two = __floats2half2_rn(v[2 * i] * kNsScale, v[2 * i + 1] * kNsScale);
+            h[i] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+        float4* xp = reinterpret_cast<float4*>(X32 + at);
+        xp[0] = make_float4(v[0], v[1], v[2], v[3]);
+        xp[1] = make_float4(v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<uint4*>(X16 + at) = make_uint4(h[0], h[1], h[2], h[3]);
     }
 }
 
@@ -521,7 +620,7 @@ static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, NsPara
     if (p.tiles < workers) workers = p.tiles;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(Cfg::PAIR ? 2 * workers : workers));
-    cfg.blockDim = dim3(192);
+    cfg.blockDim = dim3(Cfg::THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -532,6 +631,20 @@ static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, NsPara
     cfg.numAttrs = 1;
     NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, p));
     return NZB_OK;
+}
+
+// Pairs of CTAs on 256 x 256 tiles read half the operand bytes per product from shared memory; single CTAs on 128 x 128
+// tiles fill the SMs better when there are few. A pair's tile keeps two SMs busy for twice as long as a small one,
+// and a small one takes a sixth longer than its share (8192 x 4096 fp32 with small tiles only: 1.95 ms, pairs 1.75).
+template <int MODE>
+static int launch_best(const CUtensorMap& tmA, const CUtensorMap& tmB, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
+    const auto count = [&](int64_t tile) {
+        const int64_t m = (p.M + tile - 1) / tile, n = (p.N + tile - 1) / tile;
+        return batch * (MODE == NS_APPLY ? m * n : m * (m + 1) / 2);
+    };
+    const int64_t pairs = ds.sm_count / 2, rounds_pair = (count(256) + pairs - 1) / pairs, rounds_single = (count(128) + ds.sm_count - 1) / ds.sm_count;
+    return 12 * rounds_pair <= 7 * rounds_single ? launch_product<NsCfg<true>, MODE>(tmA, tmB, p, batch, ds, s)
+                                                : launch_product<NsCfg<false>, MODE>(tmA, tmB, p, batch, ds, s);
 }
 
 // A product's operand of the whole batch: `rows` x `cols` halves, the contraction along the row or down the rows.
@@ -580,14 +693,14 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         p.ld16 = pl.lda;
         p.stride16 = pl.S * pl.lda;
         const CUtensorMap& x = pl.tall ? x_mn[cur] : x_k[cur];
-        rc = launch_product<NsCfg<false>, NS_GRAM>(x, x, p, d->batch, ds, s);
+        rc = launch_best<NS_GRAM>(x, x, p, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
         // B = c1 A + c2 A A; A is symmetric, so both operands are read along its rows
         contraction(p, pl.S);
         p.a_mn = p.b_mn = 0;
         p.out16 = B16;
         p.gram = A16;
-        rc = launch_product<NsCfg<false>, NS_POLY>(gram_k, gram_k, p, d->batch, ds, s);
+        rc = launch_best<NS_POLY>(gram_k, gram_k, p, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
         // X = c0 X + B X, or c0 X + X B
         p.M = (int32_t)d->rows;
@@ -608,7 +721,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
             p.w_keep = target.w_keep;
             p.w_step = target.w_step;
         }
-        rc = launch_product<NsCfg<false>, NS_APPLY>(pl.tall ? x_k[cur] : poly_k, pl.tall ? poly_k : x_mn[cur], p, d->batch, ds, s);
+        rc = launch_best<NS_APPLY>(pl.tall ? x_k[cur] : poly_k, pl.tall ? poly_k : x_mn[cur], p, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
     }
     return NZB_OK;
@@ -620,9 +733,9 @@ static int check_ws(const NsPlan& pl, const void* ws, size_t bytes) {
     return NZB_OK;
 }
 
-// CTAs of the two elementwise passes: at least eight elements per thread.
+// CTAs of the two elementwise passes: two groups per thread at least.
 static unsigned elementwise_ctas(int64_t n, int64_t most) {
-    int64_t ctas = (n + 2047) / 2048;
+    int64_t ctas = (n + 4095) / 4096;
     return (unsigned)(ctas < 1 ? 1 : ctas > most ? most : ctas);
 }
 
@@ -664,10 +777,12 @@ int nzb_orthogonalize(const nzb_orthogonalize_desc* d, const void* g, void* out,
     double* partial = reinterpret_cast<double*>(ws + pl.total() - pl.norm);
     const int64_t n = d->rows * d->cols;
     const unsigned parts = elementwise_ctas(n, kNormParts);
+    const int64_t size = dtype_size(d->dtype);
+    const int vec = aligned_to(g, 16) && d->ld_g * size % 16 == 0 && (d->batch == 1 || d->stride_g * size % 16 == 0);
     NZB_DISPATCH_DTYPE(d->dtype, T, {
         const T* from = static_cast<const T*>(g);
-        ns_norm_kernel<T, false><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(from, nullptr, nullptr, partial, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, 0.f, 0);
-        ns_start_kernel<T, false><<<dim3(elementwise_ctas(n, 2048), (unsigned)d->batch), 256, 0, s>>>(from, X32, X16, partial, (int)parts, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, d->eps);
+        ns_norm_kernel<T, false><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(from, nullptr, nullptr, partial, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, 0.f, 0, vec);
+        ns_start_kernel<T, false><<<dim3(elementwise_ctas(n, 4096), (unsigned)d->batch), 256, 0, s>>>(from, X32, X16, partial, (int)parts, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, d->eps, vec);
     });
     NZB_CUDA_TRY(cudaGetLastError());
     const int kind = d->out_dtype == NZB_F32 ? NS_OUT_F32 : d->out_dtype == NZB_F16 ? NS_OUT_F16 : NS_OUT_BF16;
@@ -699,8 +814,9 @@ int nzb_muon(const nzb_orthogonalize_desc* d, float* w, float* momentum, const f
     double* partial = reinterpret_cast<double*>(ws + pl.total() - pl.norm);
     const int64_t n = d->rows * d->cols;
     const unsigned parts = elementwise_ctas(n, kNormParts);
-    ns_norm_kernel<float, true><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(grad, momentum, X32, partial, d->rows, d->cols, d->cols, n, pl.ldx, mu, nesterov);
-    ns_start_kernel<float, true><<<dim3(elementwise_ctas(n, 2048), (unsigned)d->batch), 256, 0, s>>>(nullptr, X32, X16, partial, (int)parts, d->rows, d->cols, 0, 0, pl.ldx, d->eps);
+    const int vec = aligned_to(grad, 16) && aligned_to(momentum, 16) && d->cols % 4 == 0;
+    ns_norm_kernel<float, true><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(grad, momentum, X32, partial, d->rows, d->cols, d->cols, n, pl.ldx, mu, nesterov, vec);
+    ns_start_kernel<float, true><<<dim3(elementwise_ctas(n, 4096), (unsigned)d->batch), 256, 0, s>>>(nullptr, X32, X16, partial, (int)parts, d->rows, d->cols, 0, 0, pl.ldx, d->eps, vec);
     NZB_CUDA_TRY(cudaGetLastError());
     return run_ns(d, pl, ws, NsTarget{NS_OUT_WEIGHT, w, d->cols, n, 1.f - lr * weight_decay, lr * scale}, *ds, s);
 }
