@@ -33,6 +33,7 @@ struct NsParams {
     int32_t k_blocks, last_ksteps;
     int32_t tiles_m, tiles_n, group_m;
     int32_t a_mn, b_mn;
+    int32_t symmetric;         // A and B by their lower triangle of (square) tiles, mirrored; 0: every tile
     int32_t by_column;         // NS_APPLY of a tall matrix: the diagonal belongs to the columns
     int32_t out_kind, out_vec; // NS_APPLY
     int64_t tiles, tiles_per_matrix;
@@ -50,20 +51,21 @@ struct NsParams {
     int* status;
 };
 
-template <bool PAIR_>
+// A tile is BM x BN per CTA (PAIR: two CTAs share one of twice the rows).
+template <bool PAIR_, int BN_>
 struct NsCfg {
     static constexpr bool PAIR = PAIR_;
-    static constexpr int BM = 128;                    // rows per CTA
-    static constexpr int TILE = PAIR ? 256 : 128;     // the tile of a CTA, or of a pair, is square
-    static constexpr int STAGES = 5;
+    static constexpr int BM = PAIR ? 256 : 128, BN = BN_;
+    static constexpr int STAGES = 6;
     static constexpr int EPI_WARPS = 8;               // two per quarter of the tensor-memory lanes, half the columns each
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static constexpr int OPERAND_BYTES = 128 * 64 * 2;  // per CTA and operand: 128 rows x 64 k
-    static constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-    static constexpr int EPI_STRIDE = 36;
-    static constexpr int EPI_BYTES = EPI_WARPS * 32 * EPI_STRIDE * 4;
+    static constexpr int B_ROWS = PAIR ? BN / 2 : BN; // rows of B that a CTA loads
+    static constexpr int A_BYTES = 128 * 64 * 2;      // per k block of 64
+    static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * 64 * 2;
+    static constexpr int EPI_BYTES = EPI_WARPS * 4096;  // 32 x 32 floats per warp
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
-    static constexpr int TMEM_COLS = 2 * TILE;
+    static constexpr int TMEM_COLS = 2 * BN;
+    static_assert(BN >= 64, "an MN-major operand is loaded in boxes of 64 columns");
     static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB shared memory of an sm_100 CTA");
 };
 
@@ -72,7 +74,7 @@ template <int MODE>
 __device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32_t& mt, int32_t& nt, int32_t& b) {
     b = static_cast<int32_t>(tile / p.tiles_per_matrix);
     const int32_t rem = static_cast<int32_t>(tile - b * p.tiles_per_matrix);
-    if (MODE == NS_APPLY) {
+    if (MODE == NS_APPLY || !p.symmetric) {
         const int32_t group = p.group_m * p.tiles_n, g = rem / group, first = g * p.group_m;
         const int32_t gm = min(p.tiles_m - first, p.group_m), within = rem - g * group;
         mt = first + within % gm;
@@ -86,27 +88,35 @@ __device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32
     }
 }
 
+// 32 x 32 fp16 entries in shared memory, 64 bytes a row: 16-byte piece j of row r lies at j ^ (r / 2 & 3), so that a lane per
+// row and four lanes per row both go without bank conflicts.
+__device__ __forceinline__ uint4* ns_piece(float* stage, int r, int j) { return reinterpret_cast<uint4*>(stage) + r * 4 + (j ^ (r >> 1 & 3)); }
+
 // Drains 32 rows x half the columns of a finished A or B tile: every lane holds one row, 32 columns at a time. Writes the
 // fp16 entries and, off the diagonal tiles, their mirror image. `ready` waits for the accumulator; what else a group of
-// columns needs is loaded before that, and for the next group before this one is written.
+// columns needs is loaded before that, and for the next group before this one is written. Rows go to and from memory
+// four lanes to 64 bytes, by way of shared memory (a lane per row touches 32 lines an instruction: 19000 cycles for a
+// 256 x 256 tile of B).
 template <class Cfg, int MODE, class Ready>
-__device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t tmem, int lane, int32_t b, int32_t row0,
+__device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b, int32_t row0,
                                                    int32_t col_first, bool mirror, Ready ready) {
     using namespace ptx;
     __half* out = p.out16 + b * p.stride16;
     const int32_t row = row0 + lane;
-    const bool row_ok = row < p.M;
-    const __half* gram = p.gram + b * p.stride16 + static_cast<int64_t>(row) * p.ld16;
+    const int pr = lane >> 2, pj = lane & 3;  // this lane's row (of eight) and piece
+    const __half* gram = p.gram + b * p.stride16;
     uint4 g[4];
     const auto fetch = [&](int32_t col0) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            g[j] = row_ok && col0 < p.N ? *reinterpret_cast<const uint4*>(gram + col0 + 8 * j) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; i++) {
+            const int32_t r = row0 + 8 * i + pr;
+            g[i] = r < p.M && col0 < p.N ? *reinterpret_cast<const uint4*>(gram + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj) : make_uint4(0, 0, 0, 0);
+        }
     };
     if (MODE == NS_POLY) fetch(col_first);
     if (!ready()) return false;
 #pragma unroll 1
-    for (int c0 = 0; c0 < Cfg::TILE / 2; c0 += 32) {
+    for (int c0 = 0; c0 < Cfg::BN / 2; c0 += 32) {
         const int32_t col0 = col_first + c0;
         if (col0 >= p.N) break;  // warp-uniform; the padded leading dimension covers a started group of 32
         uint32_t v[32];
@@ -118,7 +128,14 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
             for (int j = 0; j < 16; j++)
                 h[j] = __floats2half2_rn(__uint_as_float(v[2 * j]) * kNsUnscale, __uint_as_float(v[2 * j + 1]) * kNsUnscale);
         } else {
-            const __half2* gh = reinterpret_cast<const __half2*>(g);
+#pragma unroll
+            for (int i = 0; i < 4; i++) *ns_piece(stage, 8 * i + pr, pj) = g[i];
+            __syncwarp();
+            uint4 mine[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) mine[j] = *ns_piece(stage, lane, j);
+            __syncwarp();
+            const __half2* gh = reinterpret_cast<const __half2*>(mine);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const float2 a = __half22float2(gh[j]);
@@ -126,18 +143,23 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
                 const float x = p.c1 * a.x + p.c2 * (__uint_as_float(v[2 * j]) * kNsUnscale);
                 const float y = p.c1 * a.y + p.c2 * (__uint_as_float(v[2 * j + 1]) * kNsUnscale);
                 const int32_t c = col0 + 2 * j;
-                if (row_ok && (row == c || row == c + 1))
+                if (row < p.M && (row == c || row == c + 1))
                     p.diag[b * p.short_side + row] = p.c0 + (row == c ? x : y) * kNsUnscale;
                 h[j] = __floats2half2_rn(row == c ? 0.f : x, row == c + 1 ? 0.f : y);
             }
-            if (c0 + 32 < Cfg::TILE / 2) fetch(col0 + 32);
+            if (c0 + 32 < Cfg::BN / 2) fetch(col0 + 32);
         }
-        if (row_ok) {
-            uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * p.ld16 + col0);
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(h);
+        const uint4* own = reinterpret_cast<const uint4*>(h);
 #pragma unroll
-            for (int j = 0; j < 4; j++) to[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = own[j];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int32_t r = row0 + 8 * i + pr;
+            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
+            if (r < p.M) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj) = u;
         }
+        __syncwarp();
         if (mirror) {
             // entry (row, col) to (col, row): the lanes' rows are neighbours there. Two lanes trade halves so that
             // each writes a pair of rows: the even lane of column 2j, the odd one of column 2j + 1.
@@ -180,7 +202,7 @@ __device__ __forceinline__ void ns_put4(T* at, const float4& x, int n, bool vec)
 
 // Drains 32 rows x half the columns of a finished B X tile through shared memory, so that eight lanes share 128 bytes of a
 // row of X32, and completes the step: x = diag * x + product, or the result's element. X32 does not depend on the
-// product, so a group's part is on its way before the accumulator is ready, the next group's before this one is
+// product, so two groups' parts are on their way before the accumulator is ready, the next ones before a group is
 // written (loaded where they are used they made the epilogue as long as the product).
 template <class Cfg, class Ready>
 __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b,
@@ -189,55 +211,56 @@ __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem,
     const float* diag = p.diag + b * p.short_side;
     const int cl = (lane & 7) * 4, rl = lane >> 3;  // this lane's columns within a group, and its first row
     float* X = p.X32 + b * p.stridex + static_cast<int64_t>(row0 + rl) * p.ldx + cl;
-    float4 old[8], dc;
+    // 32 x 32 floats: the four of a lane's columns, lane & 7 within the row, lie at (lane & 7) ^ (row & 7)
+    const auto spot = [&](int r, int j) { return reinterpret_cast<float4*>(stage) + r * 8 + (j ^ (r & 7)); };
+    float4 old[2][8], dc[2];
     float dr[8];
-    const auto fetch = [&](int32_t col0) {
+    const auto fetch = [&](int32_t col0, float4 (&o)[8], float4& d) {
         const int32_t gc = col0 + cl;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (row0 + rl + 4 * i < p.M && gc < p.N) old[i] = *reinterpret_cast<const float4*>(X + static_cast<int64_t>(4 * i) * p.ldx + col0);
+            if (row0 + rl + 4 * i < p.M && gc < p.N) o[i] = *reinterpret_cast<const float4*>(X + static_cast<int64_t>(4 * i) * p.ldx + col0);
         if (p.by_column) {
-            dc.x = gc < p.N ? diag[gc] : 0.f;
-            dc.y = gc + 1 < p.N ? diag[gc + 1] : 0.f;
-            dc.z = gc + 2 < p.N ? diag[gc + 2] : 0.f;
-            dc.w = gc + 3 < p.N ? diag[gc + 3] : 0.f;
+            d.x = gc < p.N ? diag[gc] : 0.f;
+            d.y = gc + 1 < p.N ? diag[gc + 1] : 0.f;
+            d.z = gc + 2 < p.N ? diag[gc + 2] : 0.f;
+            d.w = gc + 3 < p.N ? diag[gc + 3] : 0.f;
         }
     };
-    fetch(col_first);
+    fetch(col_first, old[0], dc[0]);
+    if (Cfg::BN / 2 > 32) fetch(col_first + 32, old[1], dc[1]);
     if (!p.by_column) {
 #pragma unroll
         for (int i = 0; i < 8; i++) dr[i] = row0 + rl + 4 * i < p.M ? diag[row0 + rl + 4 * i] : 0.f;
     }
     if (!ready()) return false;
-#pragma unroll 1
-    for (int c0 = 0; c0 < Cfg::TILE / 2; c0 += 32) {
+    const auto group = [&](int c0, float4 (&o)[8], float4& d4) {
         const int32_t col0 = col_first + c0;
-        if (col0 >= p.N) break;  // warp-uniform
+        if (col0 >= p.N) return;  // warp-uniform
         {
             uint32_t v[32];
             tmem_ld_32x32(tmem + c0, v);
             tmem_ld_wait();
-            float4* dst = reinterpret_cast<float4*>(stage + lane * Cfg::EPI_STRIDE);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
-                                     __uint_as_float(v[4 * j + 3]));
+                *spot(lane, j) = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                                             __uint_as_float(v[4 * j + 3]));
         }
         __syncwarp();
         const int32_t gc = col0 + cl;
         float4 x[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            x[i] = *reinterpret_cast<const float4*>(stage + (rl + 4 * i) * Cfg::EPI_STRIDE + cl);
+            x[i] = *spot(rl + 4 * i, lane & 7);
             constexpr float k = kNsUnscale * kNsUnscale;
-            const float4 d = p.by_column ? dc : make_float4(dr[i], dr[i], dr[i], dr[i]);
-            x[i].x = fmaf(d.x, old[i].x, x[i].x * k);
-            x[i].y = fmaf(d.y, old[i].y, x[i].y * k);
-            x[i].z = fmaf(d.z, old[i].z, x[i].z * k);
-            x[i].w = fmaf(d.w, old[i].w, x[i].w * k);
+            const float4 d = p.by_column ? d4 : make_float4(dr[i], dr[i], dr[i], dr[i]);
+            x[i].x = fmaf(d.x, o[i].x, x[i].x * k);
+            x[i].y = fmaf(d.y, o[i].y, x[i].y * k);
+            x[i].z = fmaf(d.z, o[i].z, x[i].z * k);
+            x[i].w = fmaf(d.w, o[i].w, x[i].w * k);
         }
         __syncwarp();
-        if (c0 + 32 < Cfg::TILE / 2) fetch(col0 + 32);
+        if (c0 + 64 < Cfg::BN / 2) fetch(col0 + 64, o, d4);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int32_t gr = row0 + rl + 4 * i;
@@ -264,9 +287,19 @@ __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem,
                 }
             }
         }
+    };
+#pragma unroll 1
+    for (int c0 = 0; c0 < Cfg::BN / 2; c0 += 64) {
+        group(c0, old[0], dc[0]);
+        if (Cfg::BN / 2 > 32) group(c0 + 32, old[1], dc[1]);
     }
     return true;
 }
+
+// Programmatic launch: a kernel may start while the one before it on the stream ends, and waits here until that one has
+// ended and its writes are visible.
+__device__ __forceinline__ void kernel_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void kernel_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // One product of all matrices. CTA layout (320 threads, persistent over the tiles): warp 0 TMA producer, warp 1
 // tensor-memory allocator and MMA issuer, warps 2-9 epilogue; two accumulators, so that a tile's epilogue runs
@@ -322,6 +355,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    // everything above ran under the previous kernel's end; its results are there from here on
+    kernel_wait_previous();
+    kernel_allow_next();
 
     if (warp == 0) {
         uint32_t it = 0;
@@ -329,7 +365,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         for (int64_t tile = first_tile; tile < p.tiles && ok; tile += step) {
             int32_t mt, nt, b;
             ns_decode<MODE>(p, tile, mt, nt, b);
-            const int32_t row_a = mt * Cfg::TILE + (int32_t)rank * 128, row_b = nt * Cfg::TILE + (int32_t)rank * 128;
+            const int32_t row_a = mt * Cfg::BM + (int32_t)rank * 128, row_b = nt * Cfg::BN + (int32_t)rank * Cfg::B_ROWS;
             for (int32_t kb = 0; kb < p.k_blocks; kb++, it++) {
                 const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
                 if (!mbar_wait_warp(&empty[s], ph ^ 1, abort_flag)) {
@@ -342,11 +378,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                         const uint32_t leader_full = map_to_cta(smem_u32(&full[s]), 0);
                         if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
                         load_operand_pair<128>(sa, &tmA, p.a_mn, kb * 64, row_a, b, leader_full);
-                        load_operand_pair<128>(sa + Cfg::OPERAND_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, leader_full);
+                        load_operand_pair<Cfg::B_ROWS>(sa + Cfg::A_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, leader_full);
                     } else {
                         mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
                         load_operand<128>(sa, &tmA, p.a_mn, kb * 64, row_a, b, &full[s]);
-                        load_operand<128>(sa + Cfg::OPERAND_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, &full[s]);
+                        load_operand<Cfg::B_ROWS>(sa + Cfg::A_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, &full[s]);
                     }
                 }
                 __syncwarp();
@@ -364,7 +400,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            const uint32_t idesc = make_idesc_f16_f32(Cfg::TILE, Cfg::TILE) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
+            const uint32_t idesc = make_idesc_f16_f32(Cfg::BM, Cfg::BN) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
             const uint64_t hi_a = desc_high_bits(p.a_mn), hi_b = desc_high_bits(p.b_mn);
             const uint32_t ka = desc_kstep(p.a_mn), kb_step = desc_kstep(p.b_mn);
             uint32_t it = 0, tcount = 0;
@@ -373,7 +409,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 const uint32_t acc = tcount & 1, aph = (tcount >> 1) & 1;
                 if (!mbar_wait_warp(&tempty[acc], aph ^ 1, abort_flag)) break;
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * Cfg::TILE;
+                const uint32_t d_tmem = tmem_base + acc * Cfg::BN;
                 for (int32_t kb = 0; kb < p.k_blocks; kb++, it++) {
                     const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
                     if (!mbar_wait_warp(&full[s], ph, abort_flag)) {
@@ -383,7 +419,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + s * Cfg::STAGE_BYTES);
                     const uint64_t da = hi_a | ((sa & 0x3ffff) >> 4);
-                    const uint64_t db = hi_b | (((sa + Cfg::OPERAND_BYTES) & 0x3ffff) >> 4);
+                    const uint64_t db = hi_b | (((sa + Cfg::A_BYTES) & 0x3ffff) >> 4);
                     const int32_t ksteps = kb == p.k_blocks - 1 ? p.last_ksteps : 4;
                     if (elect_one()) {
                         if constexpr (PAIR) {
@@ -411,7 +447,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
     } else {
         const int q = warp & 3;
-        float* stage = epi + (warp - 2) * 32 * Cfg::EPI_STRIDE;
+        float* stage = epi + (warp - 2) * 1024;
         uint32_t tcount = 0;
         for (int64_t tile = first_tile; tile < p.tiles; tile += step, tcount++) {
             int32_t mt, nt, b;
@@ -423,11 +459,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 return true;
             };
             const int half = (warp - 2) >> 2;
-            const int32_t row0 = mt * Cfg::TILE + (int32_t)rank * 128 + q * 32, col_first = nt * Cfg::TILE + half * (Cfg::TILE / 2);
-            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::TILE + half * (Cfg::TILE / 2);
+            const int32_t row0 = mt * Cfg::BM + (int32_t)rank * 128 + q * 32, col_first = nt * Cfg::BN + half * (Cfg::BN / 2);
+            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::BN + half * (Cfg::BN / 2);
             bool ok;
             if constexpr (MODE == NS_APPLY) ok = ns_drain_apply<Cfg>(p, tmem, stage, lane, b, row0, col_first, ready);
-            else ok = ns_drain_symmetric<Cfg, MODE>(p, tmem, lane, b, row0, col_first, mt != nt, ready);
+            else ok = ns_drain_symmetric<Cfg, MODE>(p, tmem, stage, lane, b, row0, col_first, p.symmetric && mt != nt, ready);
             if (!ok) break;
             tc_fence_before();
             __syncwarp();
@@ -611,10 +647,11 @@ static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, NsPara
     const auto kernel = ns_product_kernel<Cfg, MODE>;
     int rc = ensure_dynamic_smem(smem_set, reinterpret_cast<const void*>(kernel), Cfg::SMEM_BYTES);
     if (rc != NZB_OK) return rc;
-    p.tiles_m = (p.M + Cfg::TILE - 1) / Cfg::TILE;
-    p.tiles_n = (p.N + Cfg::TILE - 1) / Cfg::TILE;
+    p.tiles_m = (p.M + Cfg::BM - 1) / Cfg::BM;
+    p.tiles_n = (p.N + Cfg::BN - 1) / Cfg::BN;
     p.group_m = 8;
-    p.tiles_per_matrix = MODE == NS_APPLY ? (int64_t)p.tiles_m * p.tiles_n : (int64_t)p.tiles_m * (p.tiles_m + 1) / 2;
+    p.symmetric = MODE != NS_APPLY && Cfg::BM == Cfg::BN;
+    p.tiles_per_matrix = p.symmetric ? (int64_t)p.tiles_m * (p.tiles_m + 1) / 2 : (int64_t)p.tiles_m * p.tiles_n;
     p.tiles = p.tiles_per_matrix * batch;
     int64_t workers = Cfg::PAIR ? ds.sm_count / 2 : ds.sm_count;
     if (p.tiles < workers) workers = p.tiles;
@@ -623,33 +660,55 @@ static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, NsPara
     cfg.blockDim = dim3(Cfg::THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = Cfg::PAIR ? 2 : 1;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = Cfg::PAIR ? 2 : 1;
     NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, p));
     return NZB_OK;
 }
 
-// Pairs of CTAs on 256 x 256 tiles read half the operand bytes per product from shared memory; single CTAs on 128 x 128
-// tiles fill the SMs better when there are few. A pair's tile keeps two SMs busy for twice as long as a small one,
-// and a small one takes a sixth longer than its share (8192 x 4096 fp32 with small tiles only: 1.95 ms, pairs 1.75).
-template <int MODE>
-static int launch_best(const CUtensorMap& tmA, const CUtensorMap& tmB, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
-    const auto count = [&](int64_t tile) {
-        const int64_t m = (p.M + tile - 1) / tile, n = (p.N + tile - 1) / tile;
-        return batch * (MODE == NS_APPLY ? m * n : m * (m + 1) / 2);
-    };
-    const int64_t pairs = ds.sm_count / 2, rounds_pair = (count(256) + pairs - 1) / pairs, rounds_single = (count(128) + ds.sm_count - 1) / ds.sm_count;
-    return 12 * rounds_pair <= 7 * rounds_single ? launch_product<NsCfg<true>, MODE>(tmA, tmB, p, batch, ds, s)
-                                                : launch_product<NsCfg<false>, MODE>(tmA, tmB, p, batch, ds, s);
+// A product's operand of the whole batch: `rows` x `cols` halves, the contraction along the row or down the rows;
+// `box`: rows of the tile that a load brings (K-major).
+static int operand(CUtensorMap* map, const __half* base, bool mn, int64_t rows, int64_t cols, int64_t ld, int64_t batch, int box) {
+    return mn ? make_operand_map_mn(map, base, rows, cols, ld, batch) : make_operand_map(map, base, cols, ld, rows, batch, box);
+}
+struct NsOperand {
+    const __half* base;
+    bool mn;
+    int64_t rows, cols, ld;
+};
+template <class Cfg, int MODE>
+static int launch_product_of(const NsOperand& a, const NsOperand& b, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
+    CUtensorMap tmA, tmB;
+    int rc = operand(&tmA, a.base, a.mn, a.rows, a.cols, a.ld, batch, 128);
+    if (rc == NZB_OK) rc = operand(&tmB, b.base, b.mn, b.rows, b.cols, b.ld, batch, Cfg::B_ROWS);
+    p.a_mn = a.mn;
+    p.b_mn = b.mn;
+    return rc == NZB_OK ? launch_product<Cfg, MODE>(tmA, tmB, p, batch, ds, s) : rc;
 }
 
-// A product's operand of the whole batch: `rows` x `cols` halves, the contraction along the row or down the rows.
-static int operand(CUtensorMap* map, const __half* base, bool mn, int64_t rows, int64_t cols, int64_t ld, int64_t batch) {
-    return mn ? make_operand_map_mn(map, base, rows, cols, ld, batch) : make_operand_map(map, base, cols, ld, rows, batch, 128);
+// Three tile sizes. A k block of 64 takes a pair of CTAs 560 cycles on its 256 x 256 tile, a CTA 460 on 128 x 128 (bound
+// by shared memory, which holds both operands) and 390 on 128 x 64; a tile's epilogue, exposed at the end, about 5000 /
+// 3500 / 2500 cycles (of X twice that). Large products are fastest by pairs, products of few tiles by the size that
+// gives every SM one, the smallest by the tile with the shortest way (8192 x 4096: 2.4 ms by pairs, 3.4 by 128 x 128;
+// 256 x 512: 125 us by 128 x 128).
+template <int MODE>
+static int launch_best(const NsOperand& a, const NsOperand& b, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
+    const auto cycles = [&](int64_t bm, int64_t bn, int64_t workers, int64_t block, int64_t epilogue) {
+        const int64_t m = (p.M + bm - 1) / bm, n = (p.N + bn - 1) / bn;
+        const int64_t tiles = batch * (MODE != NS_APPLY && bm == bn ? m * (m + 1) / 2 : m * n);
+        return (tiles + workers - 1) / workers * p.k_blocks * block + epilogue * (MODE == NS_APPLY ? 2 : 1);
+    };
+    const int64_t pair = cycles(256, 256, ds.sm_count / 2, 560, 5000), single = cycles(128, 128, ds.sm_count, 460, 3500);
+    const int64_t small = cycles(128, 64, ds.sm_count, 390, 2500);
+    if (pair <= single && pair <= small) return launch_product_of<NsCfg<true, 256>, MODE>(a, b, p, batch, ds, s);
+    if (single <= small) return launch_product_of<NsCfg<false, 128>, MODE>(a, b, p, batch, ds, s);
+    return launch_product_of<NsCfg<false, 64>, MODE>(a, b, p, batch, ds, s);
 }
 
 struct NsTarget {
@@ -666,14 +725,8 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
     __half* A16 = reinterpret_cast<__half*>(ws + pl.x32 + 2 * pl.x16);
     __half* B16 = reinterpret_cast<__half*>(ws + pl.x32 + 2 * pl.x16 + pl.gram);
     float* diag = reinterpret_cast<float*>(ws + pl.x32 + 2 * pl.x16 + 2 * pl.gram);
-    CUtensorMap x_k[2], x_mn[2], gram_k, poly_k;
+    const NsOperand gram{A16, false, pl.S, pl.S, pl.lda}, poly{B16, false, pl.S, pl.S, pl.lda};
     int rc;
-    for (int i = 0; i < 2; i++) {
-        if ((rc = operand(&x_k[i], X16[i], false, d->rows, d->cols, pl.ldx, d->batch)) != NZB_OK) return rc;
-        if ((rc = operand(&x_mn[i], X16[i], true, d->rows, d->cols, pl.ldx, d->batch)) != NZB_OK) return rc;
-    }
-    if ((rc = operand(&gram_k, A16, false, pl.S, pl.S, pl.lda, d->batch)) != NZB_OK) return rc;
-    if ((rc = operand(&poly_k, B16, false, pl.S, pl.S, pl.lda, d->batch)) != NZB_OK) return rc;
     const auto contraction = [](NsParams& p, int64_t k) {
         p.k_blocks = (int32_t)((k + 63) / 64);
         p.last_ksteps = (int32_t)((k - (int64_t)(p.k_blocks - 1) * 64 + 15) / 16);
@@ -688,25 +741,22 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         // A = X X^T, or X^T X of a tall matrix
         p.M = p.N = (int32_t)pl.S;
         contraction(p, pl.L);
-        p.a_mn = p.b_mn = pl.tall;
         p.out16 = A16;
         p.ld16 = pl.lda;
         p.stride16 = pl.S * pl.lda;
-        const CUtensorMap& x = pl.tall ? x_mn[cur] : x_k[cur];
-        rc = launch_best<NS_GRAM>(x, x, p, d->batch, ds, s);
+        const NsOperand x_k{X16[cur], false, d->rows, d->cols, pl.ldx}, x_mn{X16[cur], true, d->rows, d->cols, pl.ldx};
+        rc = launch_best<NS_GRAM>(pl.tall ? x_mn : x_k, pl.tall ? x_mn : x_k, p, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
         // B = c1 A + c2 A A; A is symmetric, so both operands are read along its rows
         contraction(p, pl.S);
-        p.a_mn = p.b_mn = 0;
         p.out16 = B16;
         p.gram = A16;
-        rc = launch_best<NS_POLY>(gram_k, gram_k, p, d->batch, ds, s);
+        rc = launch_best<NS_POLY>(gram, gram, p, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
         // X = c0 X + B X, or c0 X + X B
         p.M = (int32_t)d->rows;
         p.N = (int32_t)d->cols;
         p.by_column = pl.tall;
-        p.b_mn = !pl.tall;
         p.out16 = X16[cur ^ 1];
         p.ld16 = p.ldx = pl.ldx;
         p.stride16 = p.stridex = d->rows * pl.ldx;
@@ -721,7 +771,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
             p.w_keep = target.w_keep;
             p.w_step = target.w_step;
         }
-        rc = launch_best<NS_APPLY>(pl.tall ? x_k[cur] : poly_k, pl.tall ? poly_k : x_mn[cur], p, d->batch, ds, s);
+        rc = launch_best<NS_APPLY>(pl.tall ? x_k : poly, pl.tall ? poly : x_mn, p, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
     }
     return NZB_OK;
