@@ -8,8 +8,9 @@
 //
 // Precision. The recurrence multiplies small singular values by c0 (3.4) a step, and with them whatever noise the
 // roundings put there, so X itself is held in fp32: X = (c0 + B_ii) X32 + (B - diag B) X16. Only the products'
-// operands are fp16 (rounding 2^-12 relative), stored times 2^12 so that entries down to 2^-26 keep all bits, and
-// B's diagonal, which carries most of B once X is near orthogonal, multiplies the fp32 X. Simulated against 64 bits
+// operands are fp16 (rounding 2^-12 relative); X and A are stored times 2^12, so that entries down to 2^-26 keep all
+// bits, B as it is (entries below 2^-14 lose relative precision there, where c0 X outweighs them by far), and B's
+// diagonal, which carries most of B once X is near orthogonal, multiplies the fp32 X. Simulated against 64 bits
 // on full-rank, decaying and nearly low-rank matrices: 3e-4 .. 1e-3 for sides of 128 and more; with X rounded
 // to bf16 in every step 1e-2 .. 3e-1.
 #include <cuda_bf16.h>
@@ -22,7 +23,7 @@
 
 namespace nzb {
 
-constexpr float kNsScale = 4096.f;            // 2^12: what the fp16 copies of X, A and B are multiplied by
+constexpr float kNsScale = 4096.f;            // 2^12: what X (both copies) and A are multiplied by
 constexpr float kNsUnscale = 1.f / 4096.f;
 
 enum { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2 };
@@ -38,7 +39,7 @@ struct NsParams {
     int32_t out_kind, out_vec; // NS_APPLY
     int64_t tiles, tiles_per_matrix;
     float c0, c1, c2;
-    __half* out16;             // A, B or the next X, times 2^12
+    __half* out16;             // 2^12 A, B or the next 2^12 X
     int64_t ld16, stride16;
     const __half* gram;        // NS_POLY: A times 2^12, same layout as out16
     float* diag;               // c0 + B_ii, `short_side` per matrix
@@ -57,12 +58,15 @@ struct NsCfg {
     static constexpr bool PAIR = PAIR_;
     static constexpr int BM = PAIR ? 256 : 128, BN = BN_;
     static constexpr int STAGES = 6;
-    static constexpr int EPI_WARPS = 8;               // two per quarter of the tensor-memory lanes, half the columns each
+    // two or four per quarter of the tensor-memory lanes. The epilogue of a 256-wide tile is a long chain per warp (tensor
+    // memory, shared memory, memory): eight warps took 15000 cycles, whatever they left out
+    static constexpr int EPI_WARPS = BN == 256 ? 16 : 8;
+    static constexpr int COLS = BN * 4 / EPI_WARPS;   // columns of a warp
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN; // rows of B that a CTA loads
     static constexpr int A_BYTES = 128 * 64 * 2;      // per k block of 64
     static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * 64 * 2;
-    static constexpr int EPI_BYTES = EPI_WARPS * 4096;  // 32 x 32 floats per warp
+    static constexpr int EPI_BYTES = EPI_WARPS * 2048;  // 32 x 32 fp16 entries per warp
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
     static constexpr int TMEM_COLS = 2 * BN;
     static_assert(BN >= 64, "an MN-major operand is loaded in boxes of 64 columns");
@@ -113,10 +117,21 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
             g[i] = r < p.M && col0 < p.N ? *reinterpret_cast<const uint4*>(gram + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj) : make_uint4(0, 0, 0, 0);
         }
     };
+    // Rows r0 .. r0 + 31 (below `rows`) of the 32 x 32 entries in shared memory, to columns c0 .. of the matrix.
+    const auto put = [&](int32_t r0, int32_t rows, int32_t c0, int32_t cols) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
+            if (r0 + 8 * i + pr < rows && c0 + 8 * pj < cols) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r0 + 8 * i + pr) * p.ld16 + c0 + 8 * pj) = u;
+        }
+        __syncwarp();
+    };
+    const float k1 = p.c1 * kNsUnscale, k2 = p.c2 * kNsUnscale * kNsUnscale;
     if (MODE == NS_POLY) fetch(col_first);
     if (!ready()) return false;
 #pragma unroll 1
-    for (int c0 = 0; c0 < Cfg::BN / 2; c0 += 32) {
+    for (int c0 = 0; c0 < Cfg::COLS; c0 += 32) {
         const int32_t col0 = col_first + c0;
         if (col0 >= p.N) break;  // warp-uniform; the padded leading dimension covers a started group of 32
         uint32_t v[32];
@@ -135,163 +150,161 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
 #pragma unroll
             for (int j = 0; j < 4; j++) mine[j] = *ns_piece(stage, lane, j);
             __syncwarp();
+            if (c0 + 32 < Cfg::COLS) fetch(col0 + 32);
             const __half2* gh = reinterpret_cast<const __half2*>(mine);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const float2 a = __half22float2(gh[j]);
-                // 2^12 B
-                const float x = p.c1 * a.x + p.c2 * (__uint_as_float(v[2 * j]) * kNsUnscale);
-                const float y = p.c1 * a.y + p.c2 * (__uint_as_float(v[2 * j + 1]) * kNsUnscale);
+                const float x = fmaf(k1, a.x, k2 * __uint_as_float(v[2 * j])), y = fmaf(k1, a.y, k2 * __uint_as_float(v[2 * j + 1]));
                 const int32_t c = col0 + 2 * j;
-                if (row < p.M && (row == c || row == c + 1))
-                    p.diag[b * p.short_side + row] = p.c0 + (row == c ? x : y) * kNsUnscale;
+                if (row < p.M && (row == c || row == c + 1)) p.diag[b * p.short_side + row] = p.c0 + (row == c ? x : y);
                 h[j] = __floats2half2_rn(row == c ? 0.f : x, row == c + 1 ? 0.f : y);
             }
-            if (c0 + 32 < Cfg::BN / 2) fetch(col0 + 32);
         }
         const uint4* own = reinterpret_cast<const uint4*>(h);
 #pragma unroll
         for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = own[j];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int32_t r = row0 + 8 * i + pr;
-            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
-            if (r < p.M) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj) = u;
-        }
-        __syncwarp();
+        put(row0, p.M, col0, p.ld16);
         if (mirror) {
-            // entry (row, col) to (col, row): the lanes' rows are neighbours there. Two lanes trade halves so that
-            // each writes a pair of rows: the even lane of column 2j, the odd one of column 2j + 1.
-            const int32_t pair_row = row0 + (lane & ~1);
+            // entry (row, col) to (col, row). Two lanes trade halves so that each holds a pair of rows: the even lane of
+            // column 2j, the odd one of column 2j + 1; a column's 32 rows become a row of 64 bytes.
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const __half give = lane & 1 ? __low2half(h[j]) : __high2half(h[j]);
                 const __half got = __ushort_as_half(__shfl_xor_sync(0xffffffffu, __half_as_ushort(give), 1));
                 const __half2 two = lane & 1 ? __halves2half2(got, __high2half(h[j])) : __halves2half2(__low2half(h[j]), got);
-                const int32_t c = col0 + 2 * j + (lane & 1);
-                if (c < p.N && pair_row < p.M) *reinterpret_cast<__half2*>(out + static_cast<int64_t>(c) * p.ld16 + pair_row) = two;
+                reinterpret_cast<__half2*>(ns_piece(stage, 2 * j + (lane & 1), lane >> 3))[lane >> 1 & 3] = two;
             }
+            put(col0, p.N, row0, p.ld16);
         }
     }
     return true;
 }
 
-__device__ __forceinline__ void ns_put_half4(__half* at, const float4& x) {
-    const __half2 lo = __floats2half2_rn(x.x, x.y), hi = __floats2half2_rn(x.z, x.w);
-    uint2 u;
-    u.x = *reinterpret_cast<const uint32_t*>(&lo);
-    u.y = *reinterpret_cast<const uint32_t*>(&hi);
-    *reinterpret_cast<uint2*>(at) = u;
-}
-template <typename T>
-__device__ __forceinline__ void ns_put4(T* at, const float4& x, int n, bool vec) {
-    const float f[4] = {x.x, x.y, x.z, x.w};
-    if (vec && n >= 4) {
-        union { T e[4]; uint2 two; uint4 four; } u;
-#pragma unroll
-        for (int i = 0; i < 4; i++) u.e[i] = Elem<T>::from(f[i]);
-        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(at) = u.four;
-        else *reinterpret_cast<uint2*>(at) = u.two;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (i < n) at[i] = Elem<T>::from(f[i]);
+// X32 (2^12 X) in the order the epilogue holds it: blocks of 32 x 32, in each the rows' first four columns, then the rows' next
+// four, so that a lane per row reads and writes 512 contiguous bytes an instruction. Offset of row r's columns c .. c + 3.
+__host__ __device__ __forceinline__ int64_t ns_state_at(int64_t r, int64_t c, int64_t ldx) {
+    return ((r >> 5) * (ldx >> 5) + (c >> 5)) * 1024 + (c >> 2 & 7) * 128 + (r & 31) * 4;
 }
 
-// Drains 32 rows x half the columns of a finished B X tile through shared memory, so that eight lanes share 128 bytes of a
-// row of X32, and completes the step: x = diag * x + product, or the result's element. X32 does not depend on the
-// product, so two groups' parts are on their way before the accumulator is ready, the next ones before a group is
-// written (loaded where they are used they made the epilogue as long as the product).
+// Drains 32 rows x a warp's columns of a finished B X tile and completes the step, x = diag * x + product, or writes the
+// result's elements. X32 does not depend on the product, so a group's part is on its way before the accumulator is
+// ready, the next group's before this one is written. Shared memory, which the products keep busy, only turns the fp16
+// rows around.
 template <class Cfg, class Ready>
 __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b,
                                                int32_t row0, int32_t col_first, Ready ready) {
     using namespace ptx;
     const float* diag = p.diag + b * p.short_side;
-    const int cl = (lane & 7) * 4, rl = lane >> 3;  // this lane's columns within a group, and its first row
-    float* X = p.X32 + b * p.stridex + static_cast<int64_t>(row0 + rl) * p.ldx + cl;
-    // 32 x 32 floats: the four of a lane's columns, lane & 7 within the row, lie at (lane & 7) ^ (row & 7)
-    const auto spot = [&](int r, int j) { return reinterpret_cast<float4*>(stage) + r * 8 + (j ^ (r & 7)); };
-    float4 old[2][8], dc[2];
-    float dr[8];
-    const auto fetch = [&](int32_t col0, float4 (&o)[8], float4& d) {
-        const int32_t gc = col0 + cl;
+    const int32_t row = row0 + lane;
+    const bool row_ok = row < p.M;
+    float* X = p.X32 + b * p.stridex;
+    const int pr = lane >> 2, pj = lane & 3;
+    float4 old[8];
+    float dcol = 0.f;  // by column: this lane's of the group
+    const auto fetch = [&](int32_t col0) {
+        if (p.by_column) dcol = col0 + lane < p.N ? diag[col0 + lane] : 0.f;
+        if (!row_ok || col0 >= p.N) return;
+        const float4* from = reinterpret_cast<const float4*>(X + ns_state_at(row, col0, p.ldx));
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (row0 + rl + 4 * i < p.M && gc < p.N) o[i] = *reinterpret_cast<const float4*>(X + static_cast<int64_t>(4 * i) * p.ldx + col0);
-        if (p.by_column) {
-            d.x = gc < p.N ? diag[gc] : 0.f;
-            d.y = gc + 1 < p.N ? diag[gc + 1] : 0.f;
-            d.z = gc + 2 < p.N ? diag[gc + 2] : 0.f;
-            d.w = gc + 3 < p.N ? diag[gc + 3] : 0.f;
-        }
+        for (int j = 0; j < 8; j++) old[j] = from[j * 32];
     };
-    fetch(col_first, old[0], dc[0]);
-    if (Cfg::BN / 2 > 32) fetch(col_first + 32, old[1], dc[1]);
-    if (!p.by_column) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) dr[i] = row0 + rl + 4 * i < p.M ? diag[row0 + rl + 4 * i] : 0.f;
-    }
+    fetch(col_first);
+    const float dr = !p.by_column && row_ok ? diag[row] : 0.f;
     if (!ready()) return false;
-    const auto group = [&](int c0, float4 (&o)[8], float4& d4) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < Cfg::COLS; c0 += 32) {
         const int32_t col0 = col_first + c0;
-        if (col0 >= p.N) return;  // warp-uniform
-        {
-            uint32_t v[32];
-            tmem_ld_32x32(tmem + c0, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                *spot(lane, j) = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
-                                             __uint_as_float(v[4 * j + 3]));
+        if (col0 >= p.N) break;  // warp-uniform
+        if (p.by_column) {
+            stage[lane] = dcol;
+            __syncwarp();
         }
-        __syncwarp();
-        const int32_t gc = col0 + cl;
+        uint32_t v[32];
+        tmem_ld_32x32(tmem + c0, v);
+        tmem_ld_wait();
         float4 x[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = *spot(rl + 4 * i, lane & 7);
-            constexpr float k = kNsUnscale * kNsUnscale;
-            const float4 d = p.by_column ? d4 : make_float4(dr[i], dr[i], dr[i], dr[i]);
-            x[i].x = fmaf(d.x, o[i].x, x[i].x * k);
-            x[i].y = fmaf(d.y, o[i].y, x[i].y * k);
-            x[i].z = fmaf(d.z, o[i].z, x[i].z * k);
-            x[i].w = fmaf(d.w, o[i].w, x[i].w * k);
+        for (int j = 0; j < 8; j++) {
+            const float4 d = p.by_column ? reinterpret_cast<const float4*>(stage)[j] : make_float4(dr, dr, dr, dr);
+            x[j].x = fmaf(d.x, old[j].x, __uint_as_float(v[4 * j]));
+            x[j].y = fmaf(d.y, old[j].y, __uint_as_float(v[4 * j + 1]));
+            x[j].z = fmaf(d.z, old[j].z, __uint_as_float(v[4 * j + 2]));
+            x[j].w = fmaf(d.w, old[j].w, __uint_as_float(v[4 * j + 3]));
         }
-        __syncwarp();
-        if (c0 + 64 < Cfg::BN / 2) fetch(col0 + 64, o, d4);
+        if (p.by_column) __syncwarp();
+        if (c0 + 32 < Cfg::COLS) fetch(col0 + 32);
+        if (p.out_kind == NS_OUT_STATE) {
+            if (row_ok) {
+                float4* to = reinterpret_cast<float4*>(X + ns_state_at(row, col0, p.ldx));
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int32_t gr = row0 + rl + 4 * i;
-            if (gr >= p.M || gc >= p.N) continue;
-            if (p.out_kind == NS_OUT_STATE) {
-                *reinterpret_cast<float4*>(X + static_cast<int64_t>(4 * i) * p.ldx + col0) = x[i];  // the padded row holds whole groups of four
-                x[i].x *= kNsScale; x[i].y *= kNsScale; x[i].z *= kNsScale; x[i].w *= kNsScale;
-                ns_put_half4(p.out16 + b * p.stride16 + static_cast<int64_t>(gr) * p.ld16 + gc, x[i]);
-            } else {
-                const int64_t at = b * p.stride_out + static_cast<int64_t>(gr) * p.ld_out + gc;
-                const int n = p.N - gc;
-                if (p.out_kind == NS_OUT_F32) {
-                    ns_put4(static_cast<float*>(p.out) + at, x[i], n, p.out_vec);
-                } else if (p.out_kind == NS_OUT_F16) {
-                    ns_put4(static_cast<__half*>(p.out) + at, x[i], n, p.out_vec);
-                } else if (p.out_kind == NS_OUT_BF16) {
-                    ns_put4(static_cast<__nv_bfloat16*>(p.out) + at, x[i], n, p.out_vec);
-                } else {
-                    float* w = static_cast<float*>(p.out) + at;
-                    const float f[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                for (int j = 0; j < 8; j++) to[j * 32] = x[j];
+            }
+        } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (j < n) w[j] = fmaf(-p.w_step, f[j], p.w_keep * w[j]);
-                }
+            for (int j = 0; j < 8; j++) {
+                x[j].x *= kNsUnscale; x[j].y *= kNsUnscale; x[j].z *= kNsUnscale; x[j].w *= kNsUnscale;
             }
         }
-    };
-#pragma unroll 1
-    for (int c0 = 0; c0 < Cfg::BN / 2; c0 += 64) {
-        group(c0, old[0], dc[0]);
-        if (Cfg::BN / 2 > 32) group(c0 + 32, old[1], dc[1]);
+        if (p.out_kind == NS_OUT_F32 || p.out_kind == NS_OUT_WEIGHT) {
+            // once per pass, so a lane writes its row's 128 bytes itself
+            float* to = static_cast<float*>(p.out) + b * p.stride_out + static_cast<int64_t>(row) * p.ld_out + col0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float f[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+                if (!row_ok) continue;
+                if (p.out_vec && col0 + 4 * j + 4 <= p.N) {
+                    float4* at = reinterpret_cast<float4*>(to) + j;
+                    if (p.out_kind == NS_OUT_WEIGHT) {
+                        const float4 w = *at;
+                        *at = make_float4(fmaf(-p.w_step, f[0], p.w_keep * w.x), fmaf(-p.w_step, f[1], p.w_keep * w.y),
+                                          fmaf(-p.w_step, f[2], p.w_keep * w.z), fmaf(-p.w_step, f[3], p.w_keep * w.w));
+                    } else {
+                        *at = x[j];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (col0 + 4 * j + i < p.N) to[4 * j + i] = p.out_kind == NS_OUT_WEIGHT ? fmaf(-p.w_step, f[i], p.w_keep * to[4 * j + i]) : f[i];
+                }
+            }
+            continue;
+        }
+        uint32_t h[16];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (p.out_kind == NS_OUT_BF16) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[j].x, x[j].y), hi = __floats2bfloat162_rn(x[j].z, x[j].w);
+                h[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
+                h[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+            } else {
+                const __half2 lo = __floats2half2_rn(x[j].x, x[j].y), hi = __floats2half2_rn(x[j].z, x[j].w);
+                h[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
+                h[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+        __syncwarp();
+        const bool state = p.out_kind == NS_OUT_STATE;
+        const int64_t ld = state ? p.ld16 : p.ld_out;
+        uint16_t* out = (state ? reinterpret_cast<uint16_t*>(p.out16) + b * p.stride16 : static_cast<uint16_t*>(p.out) + b * p.stride_out) +
+                        static_cast<int64_t>(row0 + pr) * ld + col0 + 8 * pj;
+        const bool vec = state || (p.out_vec && col0 + 8 * pj + 8 <= p.N);  // the state's padded rows hold whole groups
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
+            if (row0 + 8 * i + pr >= p.M) continue;
+            if (vec) {
+                *reinterpret_cast<uint4*>(out + 8 * i * ld) = u;
+            } else {
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (col0 + 8 * pj + k < p.N) out[8 * i * ld + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+            }
+        }
+        __syncwarp();
     }
     return true;
 }
@@ -301,8 +314,8 @@ __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem,
 __device__ __forceinline__ void kernel_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void kernel_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// One product of all matrices. CTA layout (320 threads, persistent over the tiles): warp 0 TMA producer, warp 1
-// tensor-memory allocator and MMA issuer, warps 2-9 epilogue; two accumulators, so that a tile's epilogue runs
+// One product of all matrices. CTA layout (persistent over the tiles): warp 0 TMA producer, warp 1 tensor-memory
+// allocator and MMA issuer, the others epilogue; two accumulators, so that a tile's epilogue runs
 // under the next tile's products. PAIR: two CTAs share a 256 x 256 tile (each loads its 128 rows of both operands).
 // Every wait is bounded; on expiry the CTA raises its abort flag, waits for its copies in flight, frees its tensor
 // memory and returns with NZB_ERR_DEVICE_TIMEOUT in the status word.
@@ -447,7 +460,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
     } else {
         const int q = warp & 3;
-        float* stage = epi + (warp - 2) * 1024;
+        float* stage = epi + (warp - 2) * 512;
         uint32_t tcount = 0;
         for (int64_t tile = first_tile; tile < p.tiles; tile += step, tcount++) {
             int32_t mt, nt, b;
@@ -458,9 +471,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 tc_fence_after();
                 return true;
             };
-            const int half = (warp - 2) >> 2;
-            const int32_t row0 = mt * Cfg::BM + (int32_t)rank * 128 + q * 32, col_first = nt * Cfg::BN + half * (Cfg::BN / 2);
-            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::BN + half * (Cfg::BN / 2);
+            const int col_part = ((warp - 2) >> 2) * Cfg::COLS;
+            const int32_t row0 = mt * Cfg::BM + (int32_t)rank * 128 + q * 32, col_first = nt * Cfg::BN + col_part;
+            const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::BN + col_part;
             bool ok;
             if constexpr (MODE == NS_APPLY) ok = ns_drain_apply<Cfg>(p, tmem, stage, lane, b, row0, col_first, ready);
             else ok = ns_drain_symmetric<Cfg, MODE>(p, tmem, stage, lane, b, row0, col_first, p.symmetric && mt != nt, ready);
@@ -493,19 +506,27 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 // ---- Frobenius norm and first state ---------------------------------------------------------------------------
 constexpr int kNormParts = 592;  // partial sums per matrix, at most
 
-// Both elementwise passes go over groups of eight elements of a row, a thread over every gridDim.x * 256-th group.
+// Both elementwise passes go over groups of eight columns. ROWS: neighbouring threads take a row's neighbouring groups
+// (reading is all there is); otherwise a warp takes 32 rows of a group, the order of X32, and its CTA the eight groups of 64
+// columns.
+template <bool ROWS>
 struct NsGroups {
     int64_t item, items;
     uint32_t per_row;
-    __device__ __forceinline__ NsGroups(int64_t rows, int64_t cols)
-        : item(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x), per_row(static_cast<uint32_t>((cols + 7) / 8)) {
-        items = rows * per_row;
+    __device__ __forceinline__ NsGroups(int64_t rows, int64_t cols) {
+        per_row = static_cast<uint32_t>(ROWS ? (cols + 7) / 8 : (cols + 63) / 64);
+        item = ROWS ? static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x : blockIdx.x;
+        items = (ROWS ? rows : (rows + 31) / 32) * per_row;
     }
     __device__ __forceinline__ bool more() const { return item < items; }
-    __device__ __forceinline__ void next() { item += static_cast<int64_t>(gridDim.x) * 256; }
+    __device__ __forceinline__ void next() { item += static_cast<int64_t>(gridDim.x) * (ROWS ? 256 : 1); }
     __device__ __forceinline__ void at(int64_t& r, int64_t& c) const {
         r = items >> 32 ? item / per_row : static_cast<uint32_t>(item) / per_row;
-        c = (item - r * per_row) * 8;
+        c = (item - r * per_row) * (ROWS ? 8 : 64);
+        if (!ROWS) {
+            r = r * 32 + (threadIdx.x & 31);
+            c += (threadIdx.x >> 5) * 8;
+        }
     }
 };
 template <typename T>
@@ -530,14 +551,15 @@ __device__ __forceinline__ void ns_load8(const T* row, int64_t c, int64_t cols, 
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256)
 ns_norm_kernel(const T* __restrict__ g, float* __restrict__ momentum, float* __restrict__ X32, double* __restrict__ partial,
-               int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float mu, int nesterov, int vec) {
+               int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, int64_t stridex, float mu, int nesterov, int vec) {
     __shared__ double buf[8];
     const int64_t b = blockIdx.y;
     double sum = 0.0;
 #pragma unroll 4
-    for (NsGroups it(rows, cols); it.more(); it.next()) {
+    for (NsGroups<!MUON> it(rows, cols); it.more(); it.next()) {
         int64_t r, c;
         it.at(r, c);
+        if (r >= rows || c >= cols) continue;
         float v[8];
         ns_load8(g + b * stride_g + r * ld_g, c, cols, vec, v);
         if (MUON) {
@@ -557,9 +579,9 @@ ns_norm_kernel(const T* __restrict__ g, float* __restrict__ momentum, float* __r
                 for (int i = 0; i < 8; i++)
                     if (c + i < cols) mp[i] = m[i];
             }
-            float4* xp = reinterpret_cast<float4*>(X32 + (b * rows + r) * ldx + c);  // padded rows: whole groups
+            float4* xp = reinterpret_cast<float4*>(X32 + b * stridex + ns_state_at(r, c, ldx));
             xp[0] = make_float4(v[0], v[1], v[2], v[3]);
-            xp[1] = make_float4(v[4], v[5], v[6], v[7]);
+            xp[32] = make_float4(v[4], v[5], v[6], v[7]);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) sum += static_cast<double>(v[i]) * v[i];
@@ -577,7 +599,7 @@ ns_norm_kernel(const T* __restrict__ g, float* __restrict__ momentum, float* __r
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256)
 ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __restrict__ X16, const double* __restrict__ partial,
-                int parts, int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, float eps, int vec) {
+                int parts, int64_t rows, int64_t cols, int64_t ld_g, int64_t stride_g, int64_t ldx, int64_t stridex, float eps, int vec) {
     __shared__ double buf[8];
     const int64_t b = blockIdx.y;
     double sum = 0.0;
@@ -590,32 +612,37 @@ ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __rest
     for (int w = 0; w < 8; w++) sum += buf[w];
     const float div = static_cast<float>(sqrt(sum) + eps);
 #pragma unroll 2
-    for (NsGroups it(rows, cols); it.more(); it.next()) {
+    for (NsGroups<false> it(rows, cols); it.more(); it.next()) {
         int64_t r, c;
         it.at(r, c);
+        if (r >= rows || c >= cols) continue;
         float v[8];
-        const int64_t at = (b * rows + r) * ldx + c;
-        if (MUON) ns_load8(const_cast<const float*>(X32 + at - c), c, ldx, true, v);
-        else ns_load8(g + b * stride_g + r * ld_g, c, cols, vec, v);
+        float4* xp = reinterpret_cast<float4*>(X32 + b * stridex + ns_state_at(r, c, ldx));
+        if (MUON) {
+            const float4 lo = xp[0], hi = xp[32];
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+        } else {
+            ns_load8(g + b * stride_g + r * ld_g, c, cols, vec, v);
+        }
         uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = v[i] / div;
+        for (int i = 0; i < 8; i++) v[i] = v[i] / div * kNsScale;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const __half2 two = __floats2half2_rn(v[2 * i] * kNsScale, v[2 * i + 1] * kNsScale);
+            const __half2 two = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
             h[i] = *reinterpret_cast<const uint32_t*>(&two);
         }
-        float4* xp = reinterpret_cast<float4*>(X32 + at);
         xp[0] = make_float4(v[0], v[1], v[2], v[3]);
-        xp[1] = make_float4(v[4], v[5], v[6], v[7]);
-        *reinterpret_cast<uint4*>(X16 + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        xp[32] = make_float4(v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<uint4*>(X16 + (b * rows + r) * ldx + c) = make_uint4(h[0], h[1], h[2], h[3]);  // padded rows: whole groups
     }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
 struct NsPlan {
     bool tall;
-    int64_t S, L, ldx, lda;
+    int64_t S, L, ldx, lda, stridex;  // stridex: floats of a matrix's X32, whole blocks of 32 rows
     size_t x32, x16, gram, diag, norm;
     size_t total() const { return x32 + 2 * x16 + 2 * gram + diag + norm; }
 };
@@ -632,7 +659,8 @@ static int plan_ns(const nzb_orthogonalize_desc* d, NsPlan* pl) {
     if (pl->S > (1 << 20)) return fail(NZB_ERR_UNSUPPORTED, "the short side is at most 2^20");
     pl->ldx = round_up(d->cols > 0 ? d->cols : 1, kOperandKAlign);
     pl->lda = round_up(pl->S > 0 ? pl->S : 1, kOperandKAlign);
-    pl->x32 = (size_t)round_up(d->batch * d->rows * pl->ldx * 4, 256);
+    pl->stridex = round_up(d->rows, 32) * pl->ldx;
+    pl->x32 = (size_t)round_up(d->batch * pl->stridex * 4, 256);
     pl->x16 = (size_t)round_up(d->batch * d->rows * pl->ldx * 2, 256);
     pl->gram = (size_t)round_up(d->batch * pl->S * pl->lda * 2, 256);
     pl->diag = (size_t)round_up(d->batch * pl->S * 4, 256);
@@ -759,7 +787,8 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         p.by_column = pl.tall;
         p.out16 = X16[cur ^ 1];
         p.ld16 = p.ldx = pl.ldx;
-        p.stride16 = p.stridex = d->rows * pl.ldx;
+        p.stride16 = d->rows * pl.ldx;
+        p.stridex = pl.stridex;
         p.X32 = X32;
         if (step == d->steps - 1) {
             const int64_t size = target.kind == NS_OUT_F16 || target.kind == NS_OUT_BF16 ? 2 : 4;
@@ -767,7 +796,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
             p.out = target.out;
             p.ld_out = target.ld;
             p.stride_out = target.stride;
-            p.out_vec = aligned_to(target.out, 4 * size) && target.ld % 4 == 0 && target.stride % 4 == 0;
+            p.out_vec = aligned_to(target.out, 16) && target.ld * size % 16 == 0 && target.stride * size % 16 == 0;
             p.w_keep = target.w_keep;
             p.w_step = target.w_step;
         }
@@ -783,9 +812,9 @@ static int check_ws(const NsPlan& pl, const void* ws, size_t bytes) {
     return NZB_OK;
 }
 
-// CTAs of the two elementwise passes: two groups per thread at least.
+// CTAs of the two elementwise passes, 2048 elements a turn.
 static unsigned elementwise_ctas(int64_t n, int64_t most) {
-    int64_t ctas = (n + 4095) / 4096;
+    int64_t ctas = (n + 2047) / 2048;
     return (unsigned)(ctas < 1 ? 1 : ctas > most ? most : ctas);
 }
 
@@ -831,8 +860,8 @@ int nzb_orthogonalize(const nzb_orthogonalize_desc* d, const void* g, void* out,
     const int vec = aligned_to(g, 16) && d->ld_g * size % 16 == 0 && (d->batch == 1 || d->stride_g * size % 16 == 0);
     NZB_DISPATCH_DTYPE(d->dtype, T, {
         const T* from = static_cast<const T*>(g);
-        ns_norm_kernel<T, false><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(from, nullptr, nullptr, partial, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, 0.f, 0, vec);
-        ns_start_kernel<T, false><<<dim3(elementwise_ctas(n, 4096), (unsigned)d->batch), 256, 0, s>>>(from, X32, X16, partial, (int)parts, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, d->eps, vec);
+        ns_norm_kernel<T, false><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(from, nullptr, nullptr, partial, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, pl.stridex, 0.f, 0, vec);
+        ns_start_kernel<T, false><<<dim3(elementwise_ctas(n, 4096), (unsigned)d->batch), 256, 0, s>>>(from, X32, X16, partial, (int)parts, d->rows, d->cols, d->ld_g, d->stride_g, pl.ldx, pl.stridex, d->eps, vec);
     });
     NZB_CUDA_TRY(cudaGetLastError());
     const int kind = d->out_dtype == NZB_F32 ? NS_OUT_F32 : d->out_dtype == NZB_F16 ? NS_OUT_F16 : NS_OUT_BF16;
@@ -865,8 +894,8 @@ int nzb_muon(const nzb_orthogonalize_desc* d, float* w, float* momentum, const f
     const int64_t n = d->rows * d->cols;
     const unsigned parts = elementwise_ctas(n, kNormParts);
     const int vec = aligned_to(grad, 16) && aligned_to(momentum, 16) && d->cols % 4 == 0;
-    ns_norm_kernel<float, true><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(grad, momentum, X32, partial, d->rows, d->cols, d->cols, n, pl.ldx, mu, nesterov, vec);
-    ns_start_kernel<float, true><<<dim3(elementwise_ctas(n, 4096), (unsigned)d->batch), 256, 0, s>>>(nullptr, X32, X16, partial, (int)parts, d->rows, d->cols, 0, 0, pl.ldx, d->eps, vec);
+    ns_norm_kernel<float, true><<<dim3(parts, (unsigned)d->batch), 256, 0, s>>>(grad, momentum, X32, partial, d->rows, d->cols, d->cols, n, pl.ldx, pl.stridex, mu, nesterov, vec);
+    ns_start_kernel<float, true><<<dim3(elementwise_ctas(n, 4096), (unsigned)d->batch), 256, 0, s>>>(nullptr, X32, X16, partial, (int)parts, d->rows, d->cols, 0, 0, pl.ldx, pl.stridex, d->eps, vec);
     NZB_CUDA_TRY(cudaGetLastError());
     return run_ns(d, pl, ws, NsTarget{NS_OUT_WEIGHT, w, d->cols, n, 1.f - lr * weight_decay, lr * scale}, *ds, s);
 }
