@@ -58,9 +58,9 @@ struct NsCfg {
     static constexpr bool PAIR = PAIR_;
     static constexpr int BM = PAIR ? 256 : 128, BN = BN_;
     static constexpr int STAGES = 6;
-    // two or four per quarter of the tensor-memory lanes. The epilogue of a 256-wide tile is a long chain per warp (tensor
-    // memory, shared memory, memory): eight warps took 15000 cycles, whatever they left out
-    static constexpr int EPI_WARPS = BN == 256 ? 16 : 8;
+    // two or four per quarter of the tensor-memory lanes. The epilogue is a long chain per warp (tensor memory, shared
+    // memory, memory): on a 256-wide tile eight warps took 15000 cycles, whatever they left out, sixteen 7500
+    static constexpr int EPI_WARPS = BN >= 128 ? 16 : 8;
     static constexpr int COLS = BN * 4 / EPI_WARPS;   // columns of a warp
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN; // rows of B that a CTA loads
@@ -507,8 +507,8 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 constexpr int kNormParts = 592;  // partial sums per matrix, at most
 
 // Both elementwise passes go over groups of eight columns. ROWS: neighbouring threads take a row's neighbouring groups
-// (reading is all there is); otherwise a warp takes 32 rows of a group, the order of X32, and its CTA the eight groups of 64
-// columns.
+// (reading is all there is); otherwise a CTA takes 32 rows x 64 columns and a warp 8 x 32 of them: 64 bytes and more of
+// every row, and whole lines of X32's order.
 template <bool ROWS>
 struct NsGroups {
     int64_t item, items;
@@ -524,8 +524,9 @@ struct NsGroups {
         r = items >> 32 ? item / per_row : static_cast<uint32_t>(item) / per_row;
         c = (item - r * per_row) * (ROWS ? 8 : 64);
         if (!ROWS) {
-            r = r * 32 + (threadIdx.x & 31);
-            c += (threadIdx.x >> 5) * 8;
+            const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            r = r * 32 + (warp & 3) * 8 + (lane >> 2);
+            c += (warp >> 2) * 32 + (lane & 3) * 8;
         }
     }
 };
@@ -720,20 +721,22 @@ static int launch_product_of(const NsOperand& a, const NsOperand& b, NsParams& p
     return rc == NZB_OK ? launch_product<Cfg, MODE>(tmA, tmB, p, batch, ds, s) : rc;
 }
 
-// Three tile sizes. A k block of 64 takes a pair of CTAs 560 cycles on its 256 x 256 tile, a CTA 460 on 128 x 128 (bound
-// by shared memory, which holds both operands) and 390 on 128 x 64; a tile's epilogue, exposed at the end, about 5000 /
-// 3500 / 2500 cycles (of X twice that). Large products are fastest by pairs, products of few tiles by the size that
-// gives every SM one, the smallest by the tile with the shortest way (8192 x 4096: 2.4 ms by pairs, 3.4 by 128 x 128;
-// 256 x 512: 125 us by 128 x 128).
+// Three tile sizes. A k block of 64 takes a pair of CTAs 565 cycles on its 256 x 256 tile, a CTA 455 on 128 x 128 (bound
+// by shared memory, which holds both operands) and 390 on 128 x 64. Between two tiles of a CTA the epilogue of the
+// first slows the second down (by about half its own length when it is X's, which moves ten bytes an entry); the last
+// epilogue stands alone. Large products are fastest by pairs, products of few tiles by the size that gives every SM one, the
+// smallest by the tile with the shortest way (8192 x 4096: 2.4 ms by pairs, 3.4 by 128 x 128; 256 x 512: 71 us by 128 x 64,
+// 125 by 128 x 128).
 template <int MODE>
 static int launch_best(const NsOperand& a, const NsOperand& b, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
     const auto cycles = [&](int64_t bm, int64_t bn, int64_t workers, int64_t block, int64_t epilogue) {
         const int64_t m = (p.M + bm - 1) / bm, n = (p.N + bn - 1) / bn;
         const int64_t tiles = batch * (MODE != NS_APPLY && bm == bn ? m * (m + 1) / 2 : m * n);
-        return (tiles + workers - 1) / workers * p.k_blocks * block + epilogue * (MODE == NS_APPLY ? 2 : 1);
+        const int64_t rounds = (tiles + workers - 1) / workers;
+        return rounds * p.k_blocks * block + (rounds - 1) * (MODE == NS_APPLY ? epilogue / 2 : 0) + epilogue;
     };
-    const int64_t pair = cycles(256, 256, ds.sm_count / 2, 560, 5000), single = cycles(128, 128, ds.sm_count, 460, 3500);
-    const int64_t small = cycles(128, 64, ds.sm_count, 390, 2500);
+    const int64_t pair = cycles(256, 256, ds.sm_count / 2, 565, MODE == NS_APPLY ? 7500 : 6000);
+    const int64_t single = cycles(128, 128, ds.sm_count, 455, MODE == NS_APPLY ? 4000 : 3000), small = cycles(128, 64, ds.sm_count, 390, 2500);
     if (pair <= single && pair <= small) return launch_product_of<NsCfg<true, 256>, MODE>(a, b, p, batch, ds, s);
     if (single <= small) return launch_product_of<NsCfg<false, 128>, MODE>(a, b, p, batch, ds, s);
     return launch_product_of<NsCfg<false, 64>, MODE>(a, b, p, batch, ds, s);

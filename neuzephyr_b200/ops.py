@@ -278,43 +278,45 @@ def linear_backward(x, w, y, dy, dx=None, dw=None, dbias=None, relu=False, overw
 
 # ---- token models ------------------------------------------------------------------------------------------
 # These work on the device their tensors live on, whichever is current, and take their scratch from torch's
-# allocator call by call: calls on several streams, or captured into several graphs, share no buffer.
+# allocator call by call: calls on several streams, or captured into several graphs, share no buffer. Small calls
+# are bound by the host (a launch is 5 us of it), so the checks go by plain integers.
 
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob entropy lse top_logprob top_index")
 
+_F32 = torch.float32
 _DTYPES = {torch.float32: C.F32, torch.float16: C.F16, torch.bfloat16: C.BF16}
 _INDEX_TYPES = {torch.int32: C.I32, torch.int64: C.I64}
 
 
 def _launch(device, fn, *args):
-    """Calls an entry point on the current stream of `device`; the stream is the call's last argument."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    """Calls an entry point on the current stream of device number `device`; the stream is the call's last argument."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     if rc != C.OK:
         C.check(rc)
 
 
-def _scratch(fn, d, device):
+def _scratch(fn, d, like):
     n = ctypes.c_size_t(0)
     C.check(fn(ctypes.byref(d), ctypes.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=device)
+    return torch.empty(n.value, dtype=torch.uint8, device=like.device)
 
 
 def _dtype(t, what):
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError("%s: expected float32, float16 or bfloat16, got %s" % (what, t.dtype)) from None
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError("%s: expected float32, float16 or bfloat16, got %s" % (what, t.dtype))
+    return code
 
 
 def _index_type(t, what):
-    try:
-        return _INDEX_TYPES[t.dtype]
-    except KeyError:
-        raise ValueError("%s: expected int32 or int64, got %s" % (what, t.dtype)) from None
+    code = _INDEX_TYPES.get(t.dtype)
+    if code is None:
+        raise ValueError("%s: expected int32 or int64, got %s" % (what, t.dtype))
+    return code
 
 
 def _row_stride(t, what):
@@ -322,26 +324,32 @@ def _row_stride(t, what):
     if t.dim() != 2:
         raise ValueError("%s: expected two dimensions, got %d" % (what, t.dim()))
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
         raise ValueError("%s: the elements of a row have to be contiguous" % what)
-    if rows > 1 and t.stride(0) < cols:
-        raise ValueError("%s: rows overlap" % what)
-    return t.stride(0) if rows > 1 else max(cols, 1)
+    if rows > 1:
+        if ld < cols:
+            raise ValueError("%s: rows overlap" % what)
+        return ld
+    return cols or 1
 
 
-def _same_device(device, *ts):
-    for t in ts:
-        if t is not None and t.device != device:
-            raise ValueError("tensors are on different devices")
-    if device.type != "cuda":
+def _same_device(first, *ts):
+    """Number of the CUDA device that all tensors (or None) live on."""
+    device = first.get_device()
+    if device < 0:
         raise ValueError("expected CUDA tensors")
+    for t in ts:
+        if t is not None and t.get_device() != device:
+            raise ValueError("tensors are on different devices")
+    return device
 
 
-def _vector(t, n, what, dtype=torch.float32):
+def _vector(t, n, what, dtype=_F32):
     """Checks an optional contiguous vector of n elements; returns its address (None when absent)."""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
         raise ValueError("%s: expected a contiguous %s tensor of %d elements" % (what, dtype, n))
     return t.data_ptr()
 
@@ -350,15 +358,18 @@ def embedding(table, index, scale=1.0, out=None, out_dtype=None):
     """scale * table[index]: rows of table {vocab, dim} by token number (int32 or int64, any shape); the result has
     the shape of index with dim appended. out_dtype: the table's type, or a 16-bit type for a float32 table. An index
     outside the table gives a row of zeros."""
-    device = table.device
-    _same_device(device, index, out)
+    device = _same_device(table, index, out)
+    ld_table = _row_stride(table, "table")
     if not index.is_contiguous():
         index = index.contiguous()
-    n, (vocab, dim) = index.numel(), table.shape
+    vocab, dim = table.shape
+    shape = index.shape + (dim,)
     if out is None:
-        out = torch.empty(index.shape + (dim,), dtype=out_dtype or table.dtype, device=device)
+        out = table.new_empty(shape) if out_dtype is None else table.new_empty(shape, dtype=out_dtype)
         ld_out = dim
     else:
+        if out.shape != shape:
+            raise ValueError("out: expected the shape %s" % (tuple(shape),))
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError("out is not of out_dtype")
         if out.dim() == 2:
@@ -367,9 +378,7 @@ def embedding(table, index, scale=1.0, out=None, out_dtype=None):
             ld_out = dim
         else:
             raise ValueError("out: expected contiguous rows")
-        if out.shape != index.shape + (dim,):
-            raise ValueError("out: expected the shape %s" % (tuple(index.shape) + (dim,),))
-    d = C.EmbeddingDesc(n, vocab, dim, _row_stride(table, "table"), ld_out, -1, scale, _dtype(out, "out"), _dtype(table, "table"),
+    d = C.EmbeddingDesc(index.numel(), vocab, dim, ld_table, ld_out, -1, scale, _dtype(out, "out"), _dtype(table, "table"),
                         _index_type(index, "index"))
     _launch(device, C.lib().nzb_embedding_forward, ctypes.addressof(d), table.data_ptr(), index.data_ptr(), out.data_ptr())
     return out
@@ -379,10 +388,10 @@ def embedding_backward(dy, index, dtable, scale=1.0, padding_index=None, overwri
     """dtable[v] += scale * the sum of the rows of dy whose index is v, in the order of the rows; overwrite=True
     writes dtable instead, with zeros for tokens that do not occur. dtable is float32 {vocab, dim}; tokens equal to
     padding_index, or outside the table, contribute nothing."""
-    device = dtable.device
-    _same_device(device, dy, index)
-    if dtable.dtype != torch.float32:
+    device = _same_device(dtable, dy, index)
+    if dtable.dtype is not _F32:
         raise ValueError("dtable: expected float32")
+    ld_table = _row_stride(dtable, "dtable")
     n, (vocab, dim) = index.numel(), dtable.shape
     if dy.shape != index.shape + (dim,):
         raise ValueError("dy: expected the shape %s" % (tuple(index.shape) + (dim,),))
@@ -390,11 +399,10 @@ def embedding_backward(dy, index, dtable, scale=1.0, padding_index=None, overwri
         index = index.contiguous()
     if dy.dim() != 2:
         dy = dy.reshape(n, dim)
-    d = C.EmbeddingDesc(n, vocab, dim, _row_stride(dtable, "dtable"), _row_stride(dy, "dy"),
-                        -1 if padding_index is None else padding_index, scale, _dtype(dy, "dy"), C.F32,
-                        _index_type(index, "index"), overwrite)
+    d = C.EmbeddingDesc(n, vocab, dim, ld_table, _row_stride(dy, "dy"), -1 if padding_index is None else padding_index, scale,
+                        _dtype(dy, "dy"), C.F32, _index_type(index, "index"), overwrite)
     L = C.lib()
-    ws = _scratch(L.nzb_embedding_backward_workspace_bytes, d, device)
+    ws = _scratch(L.nzb_embedding_backward_workspace_bytes, d, dtable)
     _launch(device, L.nzb_embedding_backward, ctypes.addressof(d), dy.data_ptr(), index.data_ptr(), dtable.data_ptr(),
             ws.data_ptr(), ws.numel())
     return dtable
@@ -403,17 +411,17 @@ def embedding_backward(dy, index, dtable, scale=1.0, padding_index=None, overwri
 def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None):
     """Layer norm over the last dimension of x {rows, dim}; gamma and beta are float32 {dim}. Returns y, mean and rstd
     (float32 {rows}, what the backward pass reads). out may be x."""
-    device = x.device
-    _same_device(device, gamma, beta, out)
+    device = _same_device(x, gamma, beta, out)
     ld_x = _row_stride(x, "x")
     rows, dim = x.shape
     if out is None:
-        out, ld_y = torch.empty((rows, dim), dtype=x.dtype, device=device), max(dim, 1)
+        out, ld_y = x.new_empty((rows, dim)), dim or 1
     else:
         ld_y = _row_stride(out, "out")
         if out.shape != x.shape or out.dtype != x.dtype:
             raise ValueError("out: expected the shape and type of x")
-    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=device).unbind(0)
+    mean = x.new_empty(rows, dtype=_F32)
+    rstd = torch.empty_like(mean)
     d = C.LayernormDesc(rows, dim, ld_x, ld_y, 0, eps, _dtype(x, "x"))
     _launch(device, C.lib().nzb_layernorm_forward, ctypes.addressof(d), x.data_ptr(), _vector(gamma, dim, "gamma"),
             _vector(beta, dim, "beta"), out.data_ptr(), mean.data_ptr(), rstd.data_ptr())
@@ -424,8 +432,7 @@ def layernorm_backward(dy, x, mean, rstd, gamma=None, dx=None, dgamma=None, dbet
                        overwrite_dparams=False):
     """Adds the gradients of layernorm_forward to the given dx (type of x) and dgamma / dbeta (float32); the overwrite
     flags write instead. mean and rstd are what the forward pass returned. dx may be dy when it is overwritten."""
-    device = x.device
-    _same_device(device, dy, mean, rstd, gamma, dx, dgamma, dbeta)
+    device = _same_device(x, dy, mean, rstd, gamma, dx, dgamma, dbeta)
     ld_x, ld_dy = _row_stride(x, "x"), _row_stride(dy, "dy")
     rows, dim = x.shape
     for t, what in ((dy, "dy"), (dx, "dx")):
@@ -434,7 +441,7 @@ def layernorm_backward(dy, x, mean, rstd, gamma=None, dx=None, dgamma=None, dbet
     d = C.LayernormDesc(rows, dim, ld_x, ld_dy, 0 if dx is None else _row_stride(dx, "dx"), 0.0, _dtype(x, "x"), overwrite_dx,
                         overwrite_dparams)
     L = C.lib()
-    ws = None if dgamma is None and dbeta is None else _scratch(L.nzb_layernorm_backward_workspace_bytes, d, device)
+    ws = None if dgamma is None and dbeta is None else _scratch(L.nzb_layernorm_backward_workspace_bytes, d, x)
     _launch(device, L.nzb_layernorm_backward, ctypes.addressof(d), dy.data_ptr(), x.data_ptr(), _vector(mean, rows, "mean"),
             _vector(rstd, rows, "rstd"), _vector(gamma, dim, "gamma"), None if dx is None else dx.data_ptr(),
             _vector(dgamma, dim, "dgamma"), _vector(dbeta, dim, "dbeta"), None if ws is None else ws.data_ptr(),
@@ -445,29 +452,27 @@ def token_logprobs(logits, targets, scale=1.0, top_k=0):
     """Log probabilities of the targets under softmax(scale * logits) for logits {rows, vocab}, with each row's entropy,
     its log-sum-exp (what the backward pass reads) and the top_k likeliest tokens with their log probabilities (equal
     ones by the lower token; top_k <= 32). A target outside [0, vocab) has log probability 0."""
-    device = logits.device
-    _same_device(device, targets)
+    device = _same_device(logits, targets)
     ld = _row_stride(logits, "logits")
     rows, vocab = logits.shape
-    logprob, entropy, lse = torch.empty((3, rows), dtype=torch.float32, device=device).unbind(0)
-    top_logprob = torch.empty((rows, top_k), dtype=torch.float32, device=device)
-    top_index = torch.empty((rows, top_k), dtype=targets.dtype, device=device)
+    target_ptr = _vector(targets, rows, "targets", targets.dtype)
+    logprob = logits.new_empty(rows, dtype=_F32)
+    entropy, lse = torch.empty_like(logprob), torch.empty_like(logprob)
+    top_logprob, top_index = logprob.new_empty((rows, top_k)), targets.new_empty((rows, top_k))
     d = C.TokenLogprobDesc(rows, vocab, ld, 0, scale, _dtype(logits, "logits"), _index_type(targets, "targets"), top_k)
-    _launch(device, C.lib().nzb_token_logprob_forward, ctypes.addressof(d), logits.data_ptr(),
-            _vector(targets, rows, "targets", targets.dtype), logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
-            top_logprob.data_ptr() if top_k else None, top_index.data_ptr() if top_k else None)
+    _launch(device, C.lib().nzb_token_logprob_forward, ctypes.addressof(d), logits.data_ptr(), target_ptr, logprob.data_ptr(),
+            entropy.data_ptr(), lse.data_ptr(), top_logprob.data_ptr() if top_k else None, top_index.data_ptr() if top_k else None)
     return TokenLogprobs(logprob, entropy, lse, top_logprob, top_index)
 
 
 def token_logprobs_backward(logits, targets, lse, entropy=None, dlogprob=None, dentropy=None, scale=1.0, out=None):
     """Gradient of token_logprobs with respect to the logits, for upstream gradients dlogprob and dentropy (float32
     {rows}, either may be absent); lse and entropy are the forward pass's. out may be logits."""
-    device = logits.device
-    _same_device(device, targets, lse, entropy, dlogprob, dentropy, out)
+    device = _same_device(logits, targets, lse, entropy, dlogprob, dentropy, out)
     ld = _row_stride(logits, "logits")
     rows, vocab = logits.shape
     if out is None:
-        out, ld_out = torch.empty((rows, vocab), dtype=logits.dtype, device=device), max(vocab, 1)
+        out, ld_out = logits.new_empty((rows, vocab)), vocab or 1
     else:
         ld_out = _row_stride(out, "out")
         if out.shape != logits.shape or out.dtype != logits.dtype:
@@ -488,7 +493,7 @@ def _batch_strides(t, what):
     if t.dim() != 3:
         raise ValueError("%s: expected a matrix or a batch of matrices" % what)
     if 0 in t.shape:
-        return max(t.shape[2], 1), 0
+        return t.shape[2] or 1, 0
     ld = _row_stride(t[0], what)
     if t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * ld + t.shape[2]:
         raise ValueError("%s: matrices overlap" % what)
@@ -498,11 +503,10 @@ def _batch_strides(t, what):
 def orthogonalize(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out=None, out_dtype=None):
     """The matrix (or batch of matrices) g with its singular values brought near 1 by Newton-Schulz products, as the
     Muon optimizer applies them to an update. About 1e-3 off the 64-bit result whatever out_dtype (default: g's)."""
-    device = g.device
-    _same_device(device, out)
+    device = _same_device(g, out)
     ld_g, stride_g = _batch_strides(g, "g")
     if out is None:
-        out = torch.empty(g.shape, dtype=out_dtype or g.dtype, device=device)
+        out = g.new_empty(g.shape, dtype=out_dtype)
     elif out.shape != g.shape or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError("out: expected the shape of g and out_dtype")
     ld_out, stride_out = _batch_strides(out, "out")
@@ -510,7 +514,7 @@ def orthogonalize(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out=None, ou
     d = C.OrthogonalizeDesc(batch, g.shape[-2], g.shape[-1], ld_g, stride_g, ld_out, stride_out,
                             (ctypes.c_float * 3)(*coefficients), eps, steps, _dtype(g, "g"), _dtype(out, "out"))
     L = C.lib()
-    ws = _scratch(L.nzb_orthogonalize_workspace_bytes, d, device)
+    ws = _scratch(L.nzb_orthogonalize_workspace_bytes, d, g)
     _launch(device, L.nzb_orthogonalize, ctypes.addressof(d), g.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel())
     return out
 
@@ -520,8 +524,7 @@ def muon_step(w, momentum, grad, lr, scale=None, mu=0.95, weight_decay=0.0, nest
     """One Muon step on contiguous float32 w, momentum and grad ({rows, cols}, or a batch of such):
     momentum = mu * momentum + grad, w = (1 - lr * weight_decay) * w - lr * scale * orthogonalize(u) with u the momentum
     or, with nesterov, grad + mu * momentum. scale: sqrt(max(1, rows / cols)) when not given."""
-    device = w.device
-    _same_device(device, momentum, grad)
+    device = _same_device(w, momentum, grad)
     _check_f32_cuda(w, momentum, grad)
     if momentum.shape != w.shape or grad.shape != w.shape or w.dim() not in (2, 3):
         raise ValueError("expected three matrices, or batches of matrices, of one shape")
@@ -531,7 +534,7 @@ def muon_step(w, momentum, grad, lr, scale=None, mu=0.95, weight_decay=0.0, nest
     d = C.OrthogonalizeDesc(w.shape[0] if w.dim() == 3 else 1, rows, cols, cols, rows * cols, cols, rows * cols,
                             (ctypes.c_float * 3)(*coefficients), eps, steps)
     L = C.lib()
-    ws = _scratch(L.nzb_muon_workspace_bytes, d, device)
+    ws = _scratch(L.nzb_muon_workspace_bytes, d, w)
     _launch(device, L.nzb_muon, ctypes.addressof(d), w.data_ptr(), momentum.data_ptr(), grad.data_ptr(), lr, scale, mu,
             weight_decay, int(nesterov), ws.data_ptr(), ws.numel())
     return w
