@@ -25,11 +25,13 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
 }
 
 constexpr int kNormElems = 16;     // backward: columns per thread
-constexpr int kNormStages = 3;     // backward: rows on their way
+// Backward: rows on their way.
+template <typename T, bool LONG>
+constexpr int kNormBackwardStages = LONG ? (sizeof(T) == 4 ? 1 : 2) : 3;
 // Forward: 32 elements a thread need 80 registers, 16 and fewer 64.
 template <typename T, int ELEMS>
 constexpr int norm_max_threads() { return ELEMS == 32 ? 768 : 1024; }
-constexpr int kNormBackwardMaxThreads = 512;  // backward: 32 sums per thread beside the row
+constexpr int kNormBackwardMaxThreads = 512;  // backward: 32 sums and the row's 32 factors per thread
 constexpr int kNormSmem = 225 * 1024;          // dynamic shared memory of a CTA
 constexpr int kNormSms = 148;      // the workspace holds one pair of sums per CTA of a grid over this many SMs
 
@@ -266,121 +268,171 @@ __device__ __forceinline__ float warp_sum_two(float a, float b, int lane) {
     return v;
 }
 
-// The same walk as the forward kernel's with a row per CTA, x and dy on their way together.
-template <typename T, bool EXACT>
-__global__ void __launch_bounds__(kNormBackwardMaxThreads)
+// The same walk as the forward kernel's, x and dy on their way together. Every group keeps its sums of the parameters'
+// gradients; at the end the CTA adds its groups', in order. LONG: rows of more than 8192 elements, by up to 1024 threads
+// with half the registers: h and g are made twice instead of kept.
+template <typename T, bool EXACT, bool LONG>
+__global__ void __launch_bounds__(LONG ? 1024 : kNormBackwardMaxThreads)
 layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
                           const float* __restrict__ gamma, T* dx, float* __restrict__ partial, int64_t rows, int dim,
-                          int64_t ld_x, int64_t ld_dy, int64_t ld_dx, int period, int add_dx) {
-    constexpr int VEC = Elem<T>::VEC, VPT = kNormElems / VEC, Q = kNormElems / 4;
+                          int64_t ld_x, int64_t ld_dy, int64_t ld_dx, int period, int add_dx, int nt, int groups) {
+    constexpr int VEC = Elem<T>::VEC, VPT = kNormElems / VEC, Q = kNormElems / 4, STAGES = kNormBackwardStages<T, LONG>;
     extern __shared__ uint4 smem_norm[];
-    __shared__ float buf[2][2][16];
-    const int t = threadIdx.x, NT = blockDim.x, lane = t & 31, warps = NT >> 5;
-    uint4* ring = smem_norm + t;  // [stage][x, dy][VPT][NT]
-    float4* params = reinterpret_cast<float4*>(smem_norm + kNormStages * 2 * VPT * NT) + t;  // [Q][NT]
-    const int lead = EXACT ? 0 : row_lead(x + (blockIdx.x % period) * ld_x);
+    __shared__ float buf[2][2][32];  // [turn][sum][warp of the CTA]
+    const int group = threadIdx.x / nt, t = threadIdx.x - group * nt, lane = threadIdx.x & 31;
+    const int warps = nt >> 5, warp0 = group * warps, warp = threadIdx.x >> 5;
+    float4* params = reinterpret_cast<float4*>(smem_norm) + t;                             // [Q][nt], all groups'
+    uint4* ring = smem_norm + Q * nt + group * (STAGES * 2 * VPT * nt) + t;                // per group [stage][x, dy][VPT][nt]
+    const int residue = blockIdx.x % period;
+    const int lead = EXACT ? 0 : row_lead(x + residue * ld_x);
     const int64_t span_x = (rows - 1) * ld_x + dim, span_dy = (rows - 1) * ld_dy + dim;
-    const RowShare<T, VPT> share(t, NT, lead, dim);
+    const int64_t step = static_cast<int64_t>(gridDim.x / period) * groups * period;
+    const int64_t first_row = residue + static_cast<int64_t>(period) * (static_cast<int64_t>(blockIdx.x / period) * groups + group);
+    const RowShare<T, VPT> share(t, nt, lead, dim);
     if (!EXACT) {
         // blocks beyond the row are read as zeros: a dy of zero adds nothing
 #pragma unroll
-        for (int k = 0; k < kNormStages * 2 * VPT; k++)
-            if (!share.has(k % VPT)) ring[k * NT] = make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < STAGES * 2 * VPT; k++)
+            if (!share.has(k % VPT)) ring[k * nt] = make_uint4(0, 0, 0, 0);
     }
     const auto fetch = [&](int64_t r, int stage) {
         if (r < rows) {
             const bool border = !EXACT && (r == 0 || r == rows - 1);
-            share.fetch(ring + stage * 2 * VPT * NT, NT, x, r * ld_x, span_x, border);
-            share.fetch(ring + (stage * 2 + 1) * VPT * NT, NT, dy, r * ld_dy, span_dy, border);
+            share.fetch(ring + stage * 2 * VPT * nt, nt, x, r * ld_x, span_x, border);
+            share.fetch(ring + (stage * 2 + 1) * VPT * nt, nt, dy, r * ld_dy, span_dy, border);
         }
         copies_commit();
     };
 #pragma unroll
-    for (int s = 0; s < kNormStages; s++) fetch(blockIdx.x + static_cast<int64_t>(s) * gridDim.x, s);
+    for (int s = 0; s < STAGES; s++) fetch(first_row + s * step, s);
     float2 dg[VPT][VEC / 2], db[VPT][VEC / 2];
 #pragma unroll
-    for (int q = 0; q < Q; q++) {
+    for (int k = 0; k < VPT; k++)
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) dg[k][i] = db[k][i] = make_float2(0.f, 0.f);
+    for (int q = group; q < Q; q += groups) {
         float g[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int e = q * 4 + i, c = (t + e / VEC * NT) * VEC - lead + e % VEC;
+            const int e = q * 4 + i, c = (t + e / VEC * nt) * VEC - lead + e % VEC;
             g[i] = c >= 0 && c < dim ? (gamma ? gamma[c] : 1.f) : 0.f;
-            dg[e / VEC][e % VEC / 2] = db[e / VEC][e % VEC / 2] = make_float2(0.f, 0.f);
         }
-        params[q * NT] = make_float4(g[0], g[1], g[2], g[3]);
+        params[q * nt] = make_float4(g[0], g[1], g[2], g[3]);
     }
+    __syncthreads();
     const float inv = 1.f / dim;
     int turn = 0, stage = 0;
-    float next_mean = blockIdx.x < rows ? mean[blockIdx.x] : 0.f, next_rstd = blockIdx.x < rows ? rstd[blockIdx.x] : 0.f;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
+    float next_mean = first_row < rows ? mean[first_row] : 0.f, next_rstd = first_row < rows ? rstd[first_row] : 0.f;
+    for (int64_t r = first_row; r < rows; r += step, turn ^= 1) {
         const float2 rs = make_float2(next_rstd, next_rstd), minus = make_float2(-next_mean, -next_mean);
-        if (r + gridDim.x < rows) {
-            next_mean = mean[r + gridDim.x];
-            next_rstd = rstd[r + gridDim.x];
+        if (r + step < rows) {
+            next_mean = mean[r + step];
+            next_rstd = rstd[r + step];
         }
-        copies_wait<kNormStages - 1>();
+        copies_wait<STAGES - 1>();
+        uint4* xs = ring + stage * 2 * VPT * nt;
+        uint4* ds = xs + VPT * nt;
         if (!EXACT) {
             // outside the row: an x of the row, whose h is finite where the row's are, and a dy of zero, which adds nothing
-            share.patch(ring + stage * 2 * VPT * NT, NT, dim, false);
-            share.patch(ring + (stage * 2 + 1) * VPT * NT, NT, dim, true);
+            share.patch(xs, nt, dim, false);
+            share.patch(ds, nt, dim, true);
         }
-        float2 h[VPT][VEC / 2], g[VPT][VEC / 2];
+        // h = (x - mean) rstd and g = dy gamma of columns 2 i, 2 i + 1 of block k
+        const auto make = [&](const float (&fx)[VEC], const float (&fd)[VEC], const float4& ga, int i, float2& h, float2& g) {
+            h = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
+            g = mul2(make_float2(fd[2 * i], fd[2 * i + 1]), i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
+        };
+        constexpr int KEEP = LONG ? 1 : VPT;
+        float2 h[KEEP][VEC / 2], g[KEEP][VEC / 2];
         float2 sg = make_float2(0.f, 0.f), sgh = sg;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             float fx[VEC], fd[VEC];
-            Elem<T>::unpack(ring[((stage * 2) * VPT + k) * NT], fx);
-            Elem<T>::unpack(ring[((stage * 2 + 1) * VPT + k) * NT], fd);
+            Elem<T>::unpack(xs[k * nt], fx);
+            Elem<T>::unpack(ds[k * nt], fd);
 #pragma unroll
             for (int i = 0; i < VEC / 2; i++) {
-                const float4 ga = params[(k * (VEC / 4) + i / 2) * NT];
-                const float2 d = make_float2(fd[2 * i], fd[2 * i + 1]);
-                h[k][i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
-                g[k][i] = mul2(d, i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
-                sg = add2(sg, g[k][i]);
-                sgh = fma2(g[k][i], h[k][i], sgh);
-                dg[k][i] = fma2(d, h[k][i], dg[k][i]);
-                db[k][i] = add2(db[k][i], d);
+                float2 &hh = h[LONG ? 0 : k][i], &gg = g[LONG ? 0 : k][i];
+                make(fx, fd, params[(k * (VEC / 4) + i / 2) * nt], i, hh, gg);
+                sg = add2(sg, gg);
+                sgh = fma2(gg, hh, sgh);
+                dg[k][i] = fma2(make_float2(fd[2 * i], fd[2 * i + 1]), hh, dg[k][i]);
+                db[k][i] = add2(db[k][i], make_float2(fd[2 * i], fd[2 * i + 1]));
             }
         }
-        fetch(r + static_cast<int64_t>(kNormStages) * gridDim.x, stage);
-        stage = stage + 1 == kNormStages ? 0 : stage + 1;
-        if (!dx) continue;
-        float s = warp_sum_two(sg.x + sg.y, sgh.x + sgh.y, lane);
-        if (warps > 1) {
-            if ((lane & 15) == 0) buf[turn][lane >> 4][t >> 5] = s;
-            __syncthreads();
-            s = (lane & 15) < warps ? buf[turn][lane >> 4][lane & 15] : 0.f;
+        if (!LONG) fetch(r + STAGES * step, stage);
+        if (dx) {
+            float s = warp_sum_two(sg.x + sg.y, sgh.x + sgh.y, lane);
+            if (warps > 1) {
+                if ((lane & 15) == 0) buf[turn][lane >> 4][warp] = s;
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(nt) : "memory");
+                // sixteen lanes to a sum, up to two warps to a lane
+                const int w = lane & 15;
+                s = (w < warps ? buf[turn][lane >> 4][warp0 + w] : 0.f) + (w + 16 < warps ? buf[turn][lane >> 4][warp0 + w + 16] : 0.f);
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        }
-        // dx = rstd (g - mean g - h mean(g h))
-        s *= -rs.x * inv;
-        const float other = __shfl_xor_sync(0xffffffffu, s, 16);
-        const float m0 = lane & 16 ? other : s, m1 = lane & 16 ? s : other;
-        const float2 m0s = make_float2(m0, m0), m1s = make_float2(m1, m1);
-        T* dxr = dx + r * ld_dx;
-#pragma unroll
-        for (int k = 0; k < VPT; k++) {
-            if (!EXACT && !share.has(k)) continue;
-            float o[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC / 2; i++) {
-                const float2 d = fma2(g[k][i], rs, fma2(h[k][i], m1s, m0s));
-                o[2 * i] = d.x;
-                o[2 * i + 1] = d.y;
+                for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
             }
-            if (add_dx) {
-                float old[VEC];
-                Elem<T>::unpack(load_block(dxr, share.first(k), dim), old);
+            // dx = rstd (g - mean g - h mean(g h))
+            s *= -rs.x * inv;
+            const float other = __shfl_xor_sync(0xffffffffu, s, 16);
+            const float m0 = lane & 16 ? other : s, m1 = lane & 16 ? s : other;
+            const float2 m0s = make_float2(m0, m0), m1s = make_float2(m1, m1);
+            T* dxr = dx + r * ld_dx;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) o[i] += old[i];
+            for (int k = 0; k < VPT; k++) {
+                if (!EXACT && !share.has(k)) continue;
+                float o[VEC], fx[VEC], fd[VEC];
+                if (LONG) {
+                    Elem<T>::unpack(xs[k * nt], fx);
+                    Elem<T>::unpack(ds[k * nt], fd);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC / 2; i++) {
+                    float2 &hh = h[LONG ? 0 : k][i], &gg = g[LONG ? 0 : k][i];
+                    if (LONG) make(fx, fd, params[(k * (VEC / 4) + i / 2) * nt], i, hh, gg);
+                    const float2 d = fma2(gg, rs, fma2(hh, m1s, m0s));
+                    o[2 * i] = d.x;
+                    o[2 * i + 1] = d.y;
+                }
+                if (add_dx) {
+                    float old[VEC];
+                    Elem<T>::unpack(load_block(dxr, share.first(k), dim), old);
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) o[i] += old[i];
+                }
+                share.store(dxr, k, dim, o);
             }
-            share.store(dxr, k, dim, o);
         }
+        if (LONG) fetch(r + STAGES * step, stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     copies_wait<0>();
     if (!partial) return;
+    if (groups > 1) {
+        // every group's sums where its rows were, then group 0 adds them
+        __syncthreads();
+        float2* mine = reinterpret_cast<float2*>(ring - t) + t;  // [2 kNormElems / 2][nt]
+        static_assert(STAGES * 2 * VPT * 16 >= 2 * kNormElems * 4, "the sums fit in the ring");
+#pragma unroll
+        for (int k = 0; k < VPT; k++)
+#pragma unroll
+            for (int i = 0; i < VEC / 2; i++) {
+                mine[(k * (VEC / 2) + i) * nt] = dg[k][i];
+                mine[(kNormElems / 2 + k * (VEC / 2) + i) * nt] = db[k][i];
+            }
+        __syncthreads();
+        if (group) return;
+        for (int o = 1; o < groups; o++) {
+            const float2* theirs = mine + o * (STAGES * 2 * VPT * nt) * 2;
+#pragma unroll
+            for (int k = 0; k < VPT; k++)
+#pragma unroll
+                for (int i = 0; i < VEC / 2; i++) {
+                    dg[k][i] = add2(dg[k][i], theirs[(k * (VEC / 2) + i) * nt]);
+                    db[k][i] = add2(db[k][i], theirs[(kNormElems / 2 + k * (VEC / 2) + i) * nt]);
+                }
+        }
+    }
     float* pg = partial + static_cast<int64_t>(blockIdx.x) * 2 * dim;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
@@ -481,14 +533,36 @@ static int norm_threads(int64_t dim, int lead, int most, int elems) {
     const int64_t nt = round_up((dim + lead + elems - 1) / elems, 32);
     return nt <= most ? (int)nt : 0;
 }
-// CTAs of the backward kernel, at most; sized for rows that start anywhere, whatever the tensors' addresses. Its 100
-// registers a thread leave room for 640 threads on an SM.
+// CTAs of the backward kernels, at most: one for each SM, and one per residue at least.
 static int64_t norm_parts(const nzb_layernorm_desc* d) {
-    const int nt = norm_threads(d->dim, 0, kNormBackwardMaxThreads, kNormElems);
-    if (nt == 0) return d->rows < 64 ? d->rows : 64;
-    int64_t ctas = (int64_t)kNormSms * (640 / nt);
-    if (ctas > d->rows) ctas = d->rows;
-    return ctas < 8 ? 8 : ctas;  // at least one per residue
+    const int64_t ctas = d->rows < kNormSms ? d->rows : kNormSms;
+    return ctas < 8 ? 8 : ctas;
+}
+
+template <typename T, bool LONG>
+static int launch_norm_backward(const nzb_layernorm_desc* d, const void* dy, const void* x, const float* mean, const float* rstd,
+                                const float* gamma, void* dx, float* partial, int period, bool exact, int nt, int64_t* parts, cudaStream_t s) {
+    constexpr int ring = kNormBackwardStages<T, LONG> * 2 * (int)(kNormElems / Elem<T>::VEC) * 16, params = kNormElems * 4;
+    constexpr int most = LONG ? 1024 : kNormBackwardMaxThreads;
+    // as many groups as threads, named barriers, shared memory and rows allow (eight rows a group, to be worth its sums)
+    int64_t groups = most / nt;
+    const int64_t fit = (kNormSmem / nt - params) / ring, spread = (d->rows + 8 * kNormSms - 1) / (8 * kNormSms);
+    if (groups > 15) groups = 15;
+    if (groups > fit) groups = fit;
+    if (groups > spread) groups = spread;
+    int64_t ctas = (d->rows + groups - 1) / groups;
+    if (ctas > *parts) ctas = *parts;
+    ctas = ctas / period * period;
+    if (ctas == 0) ctas = period;
+    *parts = ctas;
+    const auto kernel = exact ? layernorm_backward_kernel<T, true, LONG> : layernorm_backward_kernel<T, false, LONG>;
+    static std::atomic<uint64_t> smem_set[2];
+    int rc = ensure_dynamic_smem(smem_set[exact], reinterpret_cast<const void*>(kernel), kNormSmem);
+    if (rc != NZB_OK) return rc;
+    kernel<<<(unsigned)ctas, (unsigned)(groups * nt), (size_t)(nt * (params + groups * ring)), s>>>(
+        static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, gamma, static_cast<T*>(dx), partial, d->rows, (int)d->dim,
+        d->ld_x, d->ld_y, d->ld_dx, period, !d->overwrite_dx, nt, (int)groups);
+    return NZB_OK;
 }
 
 }  // namespace nzb
@@ -597,18 +671,14 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
                           (!dx || (offset(x) == offset(dx) && d->ld_x * size % 16 == d->ld_dx * size % 16));
     const int period = d->ld_x * size % 16 == 0 ? 1 : (int)(16 / size);
     const int lead = period == 1 && aligned_to(x, 16) ? 0 : (int)(16 / size) - 1;
-    const int nt = together ? norm_threads(d->dim, lead, kNormBackwardMaxThreads, kNormElems) : 0;
+    const int nt = together ? norm_threads(d->dim, lead, 1024, kNormElems) : 0;
     if (nt) {
-        parts = parts / period * period;  // whole rounds of the residues: norm_parts gives eight at least
+        const bool exact = period == 1 && lead == 0 && d->dim == (int64_t)nt * kNormElems;
         NZB_DISPATCH_DTYPE(d->dtype, T, {
-            constexpr int per_thread = kNormStages * 2 * (int)(kNormElems / Elem<T>::VEC) * 16 + kNormElems * 4;
-            const bool exact = period == 1 && lead == 0 && d->dim == (int64_t)nt * kNormElems;
-            const auto kernel = exact ? layernorm_backward_kernel<T, true> : layernorm_backward_kernel<T, false>;
-            static std::atomic<uint64_t> smem_set[2];
-            rc = ensure_dynamic_smem(smem_set[exact], reinterpret_cast<const void*>(kernel), kNormBackwardMaxThreads * per_thread);
-            if (rc != NZB_OK) return rc;
-            kernel<<<(unsigned)parts, nt, nt * per_thread, s>>>(static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, gamma, static_cast<T*>(dx), partial, d->rows, (int)d->dim, d->ld_x, d->ld_y, d->ld_dx, period, !d->overwrite_dx);
+            rc = nt <= kNormBackwardMaxThreads ? launch_norm_backward<T, false>(d, dy, x, mean, rstd, gamma, dx, partial, period, exact, nt, &parts, s)
+                                               : launch_norm_backward<T, true>(d, dy, x, mean, rstd, gamma, dx, partial, period, exact, nt, &parts, s);
         });
+        if (rc != NZB_OK) return rc;
     } else {
         NZB_DISPATCH_DTYPE(d->dtype, T, {
             const T* xp = static_cast<const T*>(x);

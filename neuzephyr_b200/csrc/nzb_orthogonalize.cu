@@ -735,7 +735,7 @@ static int launch_best(const NsOperand& a, const NsOperand& b, NsParams& p, int6
         const int64_t rounds = (tiles + workers - 1) / workers;
         return rounds * p.k_blocks * block + (rounds - 1) * (MODE == NS_APPLY ? epilogue / 2 : 0) + epilogue;
     };
-    const int64_t pair = cycles(256, 256, ds.sm_count / 2, 565, MODE == NS_APPLY ? 7500 : 6000);
+    const int64_t pair = cycles(256, 256, ds.sm_count / 2, 565, MODE == NS_APPLY ? 10000 : 6000);
     const int64_t single = cycles(128, 128, ds.sm_count, 455, MODE == NS_APPLY ? 4000 : 3000), small = cycles(128, 64, ds.sm_count, 390, 2500);
     if (pair <= single && pair <= small) return launch_product_of<NsCfg<true, 256>, MODE>(a, b, p, batch, ds, s);
     if (single <= small) return launch_product_of<NsCfg<false, 128>, MODE>(a, b, p, batch, ds, s);
