@@ -8,10 +8,14 @@
 // and leave once per CTA; a second kernel adds the CTAs' sums in order (same bits every time).
 // Rows that do not start on 16 bytes: the columns a thread owns shift with the row's address, with a period of
 // at most 16 / element size rows, so a CTA takes rows of one residue only and its threads keep their columns.
-#include "nzb_internal.h"
+#include <cooperative_groups.h>
+
 #include "nzb_elem.cuh"
+#include "nzb_internal.h"
 
 namespace nzb {
+
+namespace cg = cooperative_groups;
 
 // Sum over the CTA, the same bits in every thread. buf: a float per warp, not written again before the next barrier.
 __device__ __forceinline__ float block_sum(float v, float* buf) {
@@ -26,8 +30,8 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
 
 constexpr int kNormElems = 16;     // backward: columns per thread
 // Backward: rows on their way.
-template <typename T, bool LONG>
-constexpr int kNormBackwardStages = LONG ? (sizeof(T) == 4 ? 1 : 2) : 3;
+constexpr int kNormStages = 3;
+constexpr int kNormMaxCluster = 4;
 // Forward: 32 elements a thread need 80 registers, 16 and fewer 64.
 template <typename T, int ELEMS>
 constexpr int norm_max_threads() { return ELEMS == 32 ? 768 : 1024; }
@@ -269,25 +273,37 @@ __device__ __forceinline__ float warp_sum_two(float a, float b, int lane) {
 }
 
 // The same walk as the forward kernel's, x and dy on their way together. Every group keeps its sums of the parameters'
-// gradients; at the end the CTA adds its groups', in order. LONG: rows of more than 8192 elements, by up to 1024 threads
-// with half the registers: h and g are made twice instead of kept.
-template <typename T, bool EXACT, bool LONG>
-__global__ void __launch_bounds__(LONG ? 1024 : kNormBackwardMaxThreads)
+// gradients; at the end the CTA adds its groups', in order. CLUSTER: rows of more than 8192 elements, in as many
+// parts of `share_cols` columns as the cluster has CTAs; the parts' two sums meet in everybody's shared memory, with the
+// cluster's barrier in place of the CTA's.
+template <typename T, bool EXACT, bool CLUSTER>
+__global__ void __launch_bounds__(kNormBackwardMaxThreads)
 layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
-                          const float* __restrict__ gamma, T* dx, float* __restrict__ partial, int64_t rows, int dim,
-                          int64_t ld_x, int64_t ld_dy, int64_t ld_dx, int period, int add_dx, int nt, int groups) {
-    constexpr int VEC = Elem<T>::VEC, VPT = kNormElems / VEC, Q = kNormElems / 4, STAGES = kNormBackwardStages<T, LONG>;
+                          const float* __restrict__ gamma, T* dx, float* __restrict__ partial, int64_t rows, int row_dim,
+                          int64_t ld_x, int64_t ld_dy, int64_t ld_dx, int period, int add_dx, int nt, int groups, int cluster,
+                          int share_cols) {
+    constexpr int VEC = Elem<T>::VEC, VPT = kNormElems / VEC, Q = kNormElems / 4, STAGES = kNormStages;
     extern __shared__ uint4 smem_norm[];
-    __shared__ float buf[2][2][32];  // [turn][sum][warp of the CTA]
+    __shared__ float buf[2][2][kNormMaxCluster * 16];  // [turn][sum][warp of the CTA, of the cluster]
     const int group = threadIdx.x / nt, t = threadIdx.x - group * nt, lane = threadIdx.x & 31;
     const int warps = nt >> 5, warp0 = group * warps, warp = threadIdx.x >> 5;
     float4* params = reinterpret_cast<float4*>(smem_norm) + t;                             // [Q][nt], all groups'
     uint4* ring = smem_norm + Q * nt + group * (STAGES * 2 * VPT * nt) + t;                // per group [stage][x, dy][VPT][nt]
-    const int residue = blockIdx.x % period;
+    // this CTA's columns, as a matrix of its own
+    const int part = CLUSTER ? blockIdx.x % cluster : 0, c0 = part * share_cols;
+    const int64_t walker = CLUSTER ? blockIdx.x / cluster : blockIdx.x, walkers = CLUSTER ? gridDim.x / cluster : gridDim.x;
+    const int dim = CLUSTER ? min(share_cols, row_dim - c0) : row_dim;
+    if (CLUSTER) {
+        x += c0;
+        dy += c0;
+        if (dx) dx += c0;
+        if (gamma) gamma += c0;
+    }
+    const int residue = static_cast<int>(walker % period);
     const int lead = EXACT ? 0 : row_lead(x + residue * ld_x);
     const int64_t span_x = (rows - 1) * ld_x + dim, span_dy = (rows - 1) * ld_dy + dim;
-    const int64_t step = static_cast<int64_t>(gridDim.x / period) * groups * period;
-    const int64_t first_row = residue + static_cast<int64_t>(period) * (static_cast<int64_t>(blockIdx.x / period) * groups + group);
+    const int64_t step = walkers / period * groups * period;
+    const int64_t first_row = residue + period * (walker / period * groups + group);
     const RowShare<T, VPT> share(t, nt, lead, dim);
     if (!EXACT) {
         // blocks beyond the row are read as zeros: a dy of zero adds nothing
@@ -320,7 +336,8 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
         params[q * nt] = make_float4(g[0], g[1], g[2], g[3]);
     }
     __syncthreads();
-    const float inv = 1.f / dim;
+    if (CLUSTER) cg::this_cluster().sync();  // everybody runs before anybody writes into another's shared memory
+    const float inv = 1.f / row_dim;
     int turn = 0, stage = 0;
     float next_mean = first_row < rows ? mean[first_row] : 0.f, next_rstd = first_row < rows ? rstd[first_row] : 0.f;
     for (int64_t r = first_row; r < rows; r += step, turn ^= 1) {
@@ -337,13 +354,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             share.patch(xs, nt, dim, false);
             share.patch(ds, nt, dim, true);
         }
-        // h = (x - mean) rstd and g = dy gamma of columns 2 i, 2 i + 1 of block k
-        const auto make = [&](const float (&fx)[VEC], const float (&fd)[VEC], const float4& ga, int i, float2& h, float2& g) {
-            h = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
-            g = mul2(make_float2(fd[2 * i], fd[2 * i + 1]), i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
-        };
-        constexpr int KEEP = LONG ? 1 : VPT;
-        float2 h[KEEP][VEC / 2], g[KEEP][VEC / 2];
+        float2 h[VPT][VEC / 2], g[VPT][VEC / 2];
         float2 sg = make_float2(0.f, 0.f), sgh = sg;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
@@ -352,23 +363,33 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             Elem<T>::unpack(ds[k * nt], fd);
 #pragma unroll
             for (int i = 0; i < VEC / 2; i++) {
-                float2 &hh = h[LONG ? 0 : k][i], &gg = g[LONG ? 0 : k][i];
-                make(fx, fd, params[(k * (VEC / 4) + i / 2) * nt], i, hh, gg);
-                sg = add2(sg, gg);
-                sgh = fma2(gg, hh, sgh);
-                dg[k][i] = fma2(make_float2(fd[2 * i], fd[2 * i + 1]), hh, dg[k][i]);
-                db[k][i] = add2(db[k][i], make_float2(fd[2 * i], fd[2 * i + 1]));
+                const float4 ga = params[(k * (VEC / 4) + i / 2) * nt];
+                const float2 d = make_float2(fd[2 * i], fd[2 * i + 1]);
+                h[k][i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
+                g[k][i] = mul2(d, i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
+                sg = add2(sg, g[k][i]);
+                sgh = fma2(g[k][i], h[k][i], sgh);
+                dg[k][i] = fma2(d, h[k][i], dg[k][i]);
+                db[k][i] = add2(db[k][i], d);
             }
         }
-        if (!LONG) fetch(r + STAGES * step, stage);
+        fetch(r + STAGES * step, stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
         if (dx) {
             float s = warp_sum_two(sg.x + sg.y, sgh.x + sgh.y, lane);
-            if (warps > 1) {
+            if (CLUSTER) {
+                cg::cluster_group all = cg::this_cluster();
+                if ((lane & 15) == 0)
+                    for (int o = 0; o < cluster; o++) *all.map_shared_rank(&buf[turn][lane >> 4][part * warps + warp], o) = s;
+                all.sync();  // the other turn's sums are not written again before everybody has passed
+                s = 0.f;
+                for (int w = lane & 15; w < cluster * warps; w += 16) s += buf[turn][lane >> 4][w];
+            } else if (warps > 1) {
                 if ((lane & 15) == 0) buf[turn][lane >> 4][warp] = s;
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(nt) : "memory");
-                // sixteen lanes to a sum, up to two warps to a lane
-                const int w = lane & 15;
-                s = (w < warps ? buf[turn][lane >> 4][warp0 + w] : 0.f) + (w + 16 < warps ? buf[turn][lane >> 4][warp0 + w + 16] : 0.f);
+                s = (lane & 15) < warps ? buf[turn][lane >> 4][warp0 + (lane & 15)] : 0.f;
+            }
+            if (CLUSTER || warps > 1) {
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
             }
@@ -381,16 +402,10 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
 #pragma unroll
             for (int k = 0; k < VPT; k++) {
                 if (!EXACT && !share.has(k)) continue;
-                float o[VEC], fx[VEC], fd[VEC];
-                if (LONG) {
-                    Elem<T>::unpack(xs[k * nt], fx);
-                    Elem<T>::unpack(ds[k * nt], fd);
-                }
+                float o[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC / 2; i++) {
-                    float2 &hh = h[LONG ? 0 : k][i], &gg = g[LONG ? 0 : k][i];
-                    if (LONG) make(fx, fd, params[(k * (VEC / 4) + i / 2) * nt], i, hh, gg);
-                    const float2 d = fma2(gg, rs, fma2(hh, m1s, m0s));
+                    const float2 d = fma2(g[k][i], rs, fma2(h[k][i], m1s, m0s));
                     o[2 * i] = d.x;
                     o[2 * i + 1] = d.y;
                 }
@@ -403,10 +418,9 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
                 share.store(dxr, k, dim, o);
             }
         }
-        if (LONG) fetch(r + STAGES * step, stage);
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     copies_wait<0>();
+    if (CLUSTER) cg::this_cluster().sync();  // nobody leaves while another CTA may still write its sums here
     if (!partial) return;
     if (groups > 1) {
         // every group's sums where its rows were, then group 0 adds them
@@ -433,7 +447,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
                 }
         }
     }
-    float* pg = partial + static_cast<int64_t>(blockIdx.x) * 2 * dim;
+    float* pg = partial + walker * 2 * row_dim + c0;
 #pragma unroll
     for (int k = 0; k < VPT; k++) {
 #pragma unroll
@@ -441,7 +455,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             const int c = share.first(k) + i;
             if (c >= 0 && c < dim) {
                 pg[c] = i & 1 ? dg[k][i / 2].y : dg[k][i / 2].x;
-                pg[dim + c] = i & 1 ? db[k][i / 2].y : db[k][i / 2].x;
+                pg[row_dim + c] = i & 1 ? db[k][i / 2].y : db[k][i / 2].x;
             }
         }
     }
@@ -539,29 +553,40 @@ static int64_t norm_parts(const nzb_layernorm_desc* d) {
     return ctas < 8 ? 8 : ctas;
 }
 
-template <typename T, bool LONG>
+template <typename T, bool CLUSTER>
 static int launch_norm_backward(const nzb_layernorm_desc* d, const void* dy, const void* x, const float* mean, const float* rstd,
-                                const float* gamma, void* dx, float* partial, int period, bool exact, int nt, int64_t* parts, cudaStream_t s) {
-    constexpr int ring = kNormBackwardStages<T, LONG> * 2 * (int)(kNormElems / Elem<T>::VEC) * 16, params = kNormElems * 4;
-    constexpr int most = LONG ? 1024 : kNormBackwardMaxThreads;
+                                const float* gamma, void* dx, float* partial, int period, bool exact, int nt, int cluster,
+                                int64_t share_cols, int64_t* parts, cudaStream_t s) {
+    constexpr int ring = kNormStages * 2 * (int)(kNormElems / Elem<T>::VEC) * 16, params = kNormElems * 4;
     // as many groups as threads, named barriers, shared memory and rows allow (eight rows a group, to be worth its sums)
-    int64_t groups = most / nt;
+    int64_t groups = CLUSTER ? 1 : kNormBackwardMaxThreads / nt;
     const int64_t fit = (kNormSmem / nt - params) / ring, spread = (d->rows + 8 * kNormSms - 1) / (8 * kNormSms);
     if (groups > 15) groups = 15;
     if (groups > fit) groups = fit;
     if (groups > spread) groups = spread;
-    int64_t ctas = (d->rows + groups - 1) / groups;
-    if (ctas > *parts) ctas = *parts;
-    ctas = ctas / period * period;
-    if (ctas == 0) ctas = period;
-    *parts = ctas;
-    const auto kernel = exact ? layernorm_backward_kernel<T, true, LONG> : layernorm_backward_kernel<T, false, LONG>;
+    int64_t walkers = (d->rows + groups - 1) / groups;
+    if (walkers > *parts / cluster) walkers = *parts / cluster;
+    walkers = walkers / period * period;
+    if (walkers == 0) walkers = period;
+    *parts = walkers;
+    const auto kernel = exact ? layernorm_backward_kernel<T, true, CLUSTER> : layernorm_backward_kernel<T, false, CLUSTER>;
     static std::atomic<uint64_t> smem_set[2];
     int rc = ensure_dynamic_smem(smem_set[exact], reinterpret_cast<const void*>(kernel), kNormSmem);
     if (rc != NZB_OK) return rc;
-    kernel<<<(unsigned)ctas, (unsigned)(groups * nt), (size_t)(nt * (params + groups * ring)), s>>>(
-        static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, gamma, static_cast<T*>(dx), partial, d->rows, (int)d->dim,
-        d->ld_x, d->ld_y, d->ld_dx, period, !d->overwrite_dx, nt, (int)groups);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(walkers * cluster));
+    cfg.blockDim = dim3((unsigned)(groups * nt));
+    cfg.dynamicSmemBytes = (size_t)(nt * (params + groups * ring));
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CLUSTER ? 1 : 0;
+    NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(dy), static_cast<const T*>(x), mean, rstd, gamma,
+                                    static_cast<T*>(dx), partial, d->rows, (int)d->dim, d->ld_x, d->ld_y, d->ld_dx, period,
+                                    (int)!d->overwrite_dx, nt, (int)groups, cluster, (int)share_cols));
     return NZB_OK;
 }
 
@@ -671,12 +696,18 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
                           (!dx || (offset(x) == offset(dx) && d->ld_x * size % 16 == d->ld_dx * size % 16));
     const int period = d->ld_x * size % 16 == 0 ? 1 : (int)(16 / size);
     const int lead = period == 1 && aligned_to(x, 16) ? 0 : (int)(16 / size) - 1;
-    const int nt = together ? norm_threads(d->dim, lead, 1024, kNormElems) : 0;
+    // CTAs to a row, and the columns of each: whole blocks of 16 bytes
+    int cluster = 1, nt = 0;
+    int64_t share_cols = d->dim;
+    for (; together && cluster <= kNormMaxCluster; cluster *= 2) {
+        share_cols = cluster == 1 ? d->dim : round_up((d->dim + cluster - 1) / cluster, 16 / size);
+        if ((nt = norm_threads(share_cols, lead, kNormBackwardMaxThreads, kNormElems)) != 0) break;
+    }
     if (nt) {
-        const bool exact = period == 1 && lead == 0 && d->dim == (int64_t)nt * kNormElems;
+        const bool exact = period == 1 && lead == 0 && share_cols == (int64_t)nt * kNormElems && share_cols * cluster == d->dim;
         NZB_DISPATCH_DTYPE(d->dtype, T, {
-            rc = nt <= kNormBackwardMaxThreads ? launch_norm_backward<T, false>(d, dy, x, mean, rstd, gamma, dx, partial, period, exact, nt, &parts, s)
-                                               : launch_norm_backward<T, true>(d, dy, x, mean, rstd, gamma, dx, partial, period, exact, nt, &parts, s);
+            rc = cluster == 1 ? launch_norm_backward<T, false>(d, dy, x, mean, rstd, gamma, dx, partial, period, exact, nt, 1, share_cols, &parts, s)
+                              : launch_norm_backward<T, true>(d, dy, x, mean, rstd, gamma, dx, partial, period, exact, nt, cluster, share_cols, &parts, s);
         });
         if (rc != NZB_OK) return rc;
     } else {
