@@ -40,19 +40,22 @@ __device__ __forceinline__ uint4 load_logits(const T* row, int first, int n) {
     for (int i = 0; i < VEC; i++) b.e[i] = first + i >= 0 && first + i < n ? row[first + i] : Elem<T>::from(-INFINITY);
     return b.u;
 }
-// Largest element of a block, NaN left out.
+// Largest element of a block, NaN left out (-inf if there is nothing else).
 __device__ __forceinline__ float block_max(const uint4& u, float) {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    const float m = fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    return m == m ? m : -INFINITY;
 }
 __device__ __forceinline__ float block_max(const uint4& u, __half) {
     const __half2* h = reinterpret_cast<const __half2*>(&u);
     const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const float f = fmaxf(__low2float(m), __high2float(m));
+    return f == f ? f : -INFINITY;
 }
 __device__ __forceinline__ float block_max(const uint4& u, __nv_bfloat16) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const float f = fmaxf(__low2float(m), __high2float(m));
+    return f == f ? f : -INFINITY;
 }
 // The elements of a block as floats no less than kEmpty, NaN kept. bf16 has the range, so two are raised at once.
 __device__ __forceinline__ void unpack_raised(const uint4& u, float (&f)[4], float) {
@@ -88,7 +91,7 @@ __device__ __forceinline__ RowSums join(const RowSums& a, const RowSums& b, floa
     return j;
 }
 
-constexpr int kLogprobThreads = 256;
+constexpr int kLogprobThreads = 256;  // per CTA; 64 for short rows
 constexpr int kLogprobFly = 4;    // blocks in flight per thread
 constexpr int kLogprobCluster = 8;  // CTAs that share a row, at most; lanes of a join too
 constexpr int kTopMax = 32;
@@ -103,20 +106,22 @@ __device__ __forceinline__ float rank_value(T x) {
     return f == f ? f : -INFINITY;
 }
 
+template <int NT>
 struct TopSmem {
-    float lane_max[kLogprobThreads];
+    float lane_max[NT];
     float value[kTopBuffer];
     int column[kTopBuffer];
-    int chosen[kLogprobThreads];
+    int chosen[NT];
     int count, n_chosen, overflow;
     float bound;
-    float best_v[kLogprobThreads / 32];
-    int best_i[kLogprobThreads / 32];
+    float best_v[NT / 32];
+    int best_i[NT / 32];
 };
 
 // Orders the first `count` candidates (at most kTopBuffer) and leaves the top_k best in front.
-__device__ __forceinline__ void rank_candidates(TopSmem& s, int count, int top_k) {
-    constexpr int NT = kLogprobThreads, PER = kTopBuffer / NT;
+template <int NT>
+__device__ __forceinline__ void rank_candidates(TopSmem<NT>& s, int count, int top_k) {
+    constexpr int PER = kTopBuffer / NT;
     const int t = threadIdx.x;
     float v[PER];
     int col[PER], at[PER];
@@ -162,11 +167,12 @@ __device__ __forceinline__ Stretch make_stretch(int vocab, int lead, int vec, in
     return st;
 }
 
-// The top_k-th largest of a CTA's 256 values, by one warp: rounds of the largest one left.
+// The top_k-th largest of a CTA's NT values, by one warp: rounds of the largest one left.
+template <int NT>
 __device__ __forceinline__ float kth_largest(const float* value, int top_k, int lane) {
-    uint32_t key[kLogprobThreads / 32], mine = 0;
+    uint32_t key[NT / 32], mine = 0;
 #pragma unroll
-    for (int j = 0; j < kLogprobThreads / 32; j++) {
+    for (int j = 0; j < NT / 32; j++) {
         const uint32_t u = __float_as_uint(value[lane + 32 * j]);
         key[j] = u & 0x80000000u ? ~u : u | 0x80000000u;  // unsigned numbers in the floats' order
         mine = max(mine, key[j]);
@@ -179,7 +185,7 @@ __device__ __forceinline__ float kth_largest(const float* value, int top_k, int 
             bool taken = false;
             mine = 0;
 #pragma unroll
-            for (int j = 0; j < kLogprobThreads / 32; j++) {
+            for (int j = 0; j < NT / 32; j++) {
                 if (!taken && key[j] == best) {
                     key[j] = 0;
                     taken = true;
@@ -195,26 +201,26 @@ __device__ __forceinline__ float kth_largest(const float* value, int top_k, int 
 // filled up with -inf in columns behind the row. lane_max[t] holds the largest of thread t's logits: the top_k-th
 // largest of these is a lower bound of the top_k-th largest logit, so only the blocks of threads whose maximum
 // reaches the bound are looked at again.
-template <typename T>
-__device__ void top_of_row(TopSmem& s, const T* row, int n, const Stretch& st, int top_k) {
-    constexpr int VEC = Elem<T>::VEC, NT = kLogprobThreads;
+template <typename T, int NT>
+__device__ void top_of_row(TopSmem<NT>& s, const T* row, int n, const Stretch& st, int top_k) {
+    constexpr int VEC = Elem<T>::VEC;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int lead = st.lead;
     if (t == 0) s.count = s.n_chosen = 0;
     __syncthreads();
     const float mine = s.lane_max[t];
     if (warp == 0) {
-        const float bound = kth_largest(s.lane_max, top_k, lane);
+        const float bound = kth_largest<NT>(s.lane_max, top_k, lane);
         if (lane == 0) s.bound = bound;
     }
     __syncthreads();
     const float bound = s.bound;
     if (mine >= bound) s.chosen[atomicAdd(&s.n_chosen, 1)] = t;
     __syncthreads();
-    const auto look = [&](int b) {
-        const int first = b * VEC - lead;
+    const auto look = [&](const uint4& u, int first) {
+        if (!(block_max(u, T()) >= bound)) return;  // most blocks of a chosen thread hold nothing of interest
         union { uint4 u; T e[VEC]; } x;
-        x.u = load_logits(row, first, n);
+        x.u = u;
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             const int col = first + i;
@@ -230,9 +236,9 @@ __device__ void top_of_row(TopSmem& s, const T* row, int n, const Stretch& st, i
     };
     for (int c = warp; c < s.n_chosen; c += NT / 32) {
         const int who = s.chosen[c];
-        for (int b = st.w0 + who + lane * NT; b < st.w1; b += 32 * NT) look(b);
-        if (lane == 0 && who == 0 && st.head >= 0) look(st.head);
-        if (lane == 1 && who == 1 && st.tail >= 0) look(st.tail);
+        for (int b = st.w0 + who + lane * NT; b < st.w1; b += 32 * NT) look(*reinterpret_cast<const uint4*>(row + (b * VEC - lead)), b * VEC - lead);
+        const int cut = who == 0 ? st.head : who == 1 ? st.tail : -1;
+        if (lane == 0 && cut >= 0) look(load_logits(row, cut * VEC - lead, n), cut * VEC - lead);
     }
     __syncthreads();
     const int c0 = st.head >= 0 ? 0 : st.w0 * VEC - lead, c1 = st.tail >= 0 || st.w1 <= st.w0 ? n : st.w1 * VEC - lead;
@@ -297,15 +303,15 @@ __device__ void top_of_row(TopSmem& s, const T* row, int n, const Stretch& st, i
 
 // A row per CTA, or per cluster of CTAs when there are few rows: each takes a stretch of the row, and the first one
 // joins what the others left in their shared memory.
-template <typename T, typename Index, bool CLUSTER>
-__global__ void __launch_bounds__(kLogprobThreads)
+template <typename T, typename Index, int NT, bool CLUSTER>
+__global__ void __launch_bounds__(NT)
 token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ targets, float* __restrict__ logprob,
                      float* __restrict__ entropy, float* __restrict__ lse_out, float* __restrict__ top_logprob,
                      Index* __restrict__ top_index, int vocab, int64_t ld, float scale, int top_k, int parts) {
-    constexpr int VEC = Elem<T>::VEC, NT = kLogprobThreads, FLY = kLogprobFly;
-    __shared__ RowSums warp_sums[NT / 32];
+    constexpr int VEC = Elem<T>::VEC, FLY = kLogprobFly, WARPS = NT / 32;
+    __shared__ RowSums warp_sums[WARPS];
     __shared__ RowSums cta_sums;
-    __shared__ TopSmem top;
+    __shared__ TopSmem<NT> top;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int part = CLUSTER ? blockIdx.x % parts : 0;
     const int64_t r = CLUSTER ? blockIdx.x / parts : blockIdx.x;
@@ -343,7 +349,7 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
             }
         }
     };
-    // whole blocks without any check, FLY of them in flight; what is left, one by one
+    // whole blocks without any check, FLY of them in flight; the last round's missing ones as masked logits
     const uint4* at = reinterpret_cast<const uint4*>(row + st.w0 * VEC - lead) + t;
     int left = (st.w1 - st.w0 - t + NT - 1) / NT;  // of this thread
     for (; left >= FLY; left -= FLY, at += FLY * NT) {
@@ -352,8 +358,13 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
         for (int f = 0; f < FLY; f++) u[f] = __ldcs(at + f * NT);
         take(u);
     }
-    for (; left > 0; left--, at += NT) {
-        const uint4 u[1] = {__ldcs(at)};
+    if (left > 0) {
+        union { T e[VEC]; uint4 u; } none;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) none.e[i] = Elem<T>::from(-INFINITY);
+        uint4 u[FLY - 1];
+#pragma unroll
+        for (int f = 0; f < FLY - 1; f++) u[f] = f < left ? __ldcs(at + f * NT) : none.u;
         take(u);
     }
     const int cut = t == 0 ? st.head : t == 1 ? st.tail : -1;
@@ -388,7 +399,8 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
         return a;
     };
     if (t < 8) {
-        a = join_eight(warp_sums[t]);
+        const RowSums none = {kEmpty, 0.f, 0.f};
+        a = join_eight(t < WARPS ? warp_sums[t] : none);
         if (t == 0) cta_sums = a;
     }
     if (top_k) top_of_row(top, row, vocab, st, top_k);
@@ -497,13 +509,15 @@ template <typename T, typename Index>
 static int launch_logprob(const nzb_token_logprob_desc* d, const void* logits, const void* targets, float* logprob, float* entropy,
                           float* lse, float* top_logprob, void* top_index, int top_k, int sm_count, cudaStream_t s) {
     const int64_t blocks = (d->vocab + Elem<T>::VEC - 1) / Elem<T>::VEC;
-    // few rows: more CTAs share one, as long as each thread keeps a round of blocks
+    // few rows: more CTAs share one, as long as each thread keeps a round of blocks; many short ones: smaller CTAs, whose
+    // joins and selections are shorter (5000 x 3000 bf16 with four alternatives: 48 us by 256 threads)
     int parts = 1;
     while (parts < kLogprobCluster && d->rows * parts < 2 * sm_count && blocks >= (int64_t)parts * 2 * kLogprobThreads * kLogprobFly) parts *= 2;
-    cudaLaunchConfig_t cfg = {};
+    const bool small = parts == 1 && blocks < kLogprobThreads * kLogprobFly;
     if (d->rows * parts > INT32_MAX) return fail(NZB_ERR_UNSUPPORTED, "too many rows");
+    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(d->rows * parts));
-    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.blockDim = dim3(small ? 64 : kLogprobThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -511,7 +525,9 @@ static int launch_logprob(const nzb_token_logprob_desc* d, const void* logits, c
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    const auto kernel = parts > 1 ? token_logprob_kernel<T, Index, true> : token_logprob_kernel<T, Index, false>;
+    const auto kernel = parts > 1 ? token_logprob_kernel<T, Index, kLogprobThreads, true>
+                        : small   ? token_logprob_kernel<T, Index, 64, false>
+                                  : token_logprob_kernel<T, Index, kLogprobThreads, false>;
     NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), static_cast<const Index*>(targets), logprob, entropy,
                                     lse, top_logprob, static_cast<Index*>(top_index), (int)d->vocab, d->ld_logits, d->scale, top_k, parts));
     return NZB_OK;
