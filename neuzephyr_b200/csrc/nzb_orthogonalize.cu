@@ -38,6 +38,9 @@ struct NsParams {
     int32_t by_column;         // NS_APPLY of a tall matrix: the diagonal belongs to the columns
     int32_t out_kind, out_vec; // NS_APPLY
     int64_t tiles, tiles_per_matrix;
+    int32_t splits;            // NS_GRAM: CTAs that share a tile, each with a stretch of the contraction (sums in `partial`)
+    float* partial;            // [split][matrix][rows and columns of the short side in blocks of 32 x 32]
+    int64_t stride_part, batch;
     float c0, c1, c2;
     __half* out16;             // 2^12 A, B or the next 2^12 X
     int64_t ld16, stride16;
@@ -73,6 +76,18 @@ struct NsCfg {
     static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB shared memory of an sm_100 CTA");
 };
 
+// The tile of a work item and the k blocks [k0, k1) it covers.
+template <int MODE>
+__device__ __forceinline__ int64_t ns_tile(const NsParams& p, int64_t item, int32_t& k0, int32_t& k1) {
+    k0 = 0;
+    k1 = p.k_blocks;
+    if (MODE != NS_GRAM || p.splits == 1) return item;
+    const int32_t split = static_cast<int32_t>(item % p.splits);
+    k0 = static_cast<int32_t>(static_cast<int64_t>(p.k_blocks) * split / p.splits);
+    k1 = static_cast<int32_t>(static_cast<int64_t>(p.k_blocks) * (split + 1) / p.splits);
+    return item / p.splits;
+}
+
 // Symmetric outputs: tile numbers run over the lower triangle, row of tiles by row of tiles.
 template <int MODE>
 __device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32_t& mt, int32_t& nt, int32_t& b) {
@@ -96,18 +111,55 @@ __device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32
 // row and four lanes per row both go without bank conflicts.
 __device__ __forceinline__ uint4* ns_piece(float* stage, int r, int j) { return reinterpret_cast<uint4*>(stage) + r * 4 + (j ^ (r >> 1 & 3)); }
 
-// Drains 32 rows x half the columns of a finished A or B tile: every lane holds one row, 32 columns at a time. Writes the
-// fp16 entries and, off the diagonal tiles, their mirror image. `ready` waits for the accumulator; what else a group of
-// columns needs is loaded before that, and for the next group before this one is written. Rows go to and from memory
-// four lanes to 64 bytes, by way of shared memory (a lane per row touches 32 lines an instruction: 19000 cycles for a
-// 256 x 256 tile of B).
+// Writes 32 x 32 entries, a row per lane in h, at (row0, col0) of an A or B and, with `mirror`, their mirror image. Rows
+// go to memory four lanes to 64 bytes, by way of shared memory (a lane per row touches 32 lines an instruction: 19000
+// cycles for a 256 x 256 tile of B).
+__device__ __forceinline__ void ns_store_block(const NsParams& p, __half* out, float* stage, int lane, int32_t row0, int32_t col0,
+                                               const __half2 (&h)[16], bool mirror) {
+    const int pr = lane >> 2, pj = lane & 3;  // this lane's row (of eight) and piece
+    // Rows r0 .. r0 + 31 (below `rows`) of the entries in shared memory, to columns c0 .. of the matrix.
+    const auto put = [&](int32_t r0, int32_t rows, int32_t c0) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
+            if (r0 + 8 * i + pr < rows && c0 + 8 * pj < p.ld16) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r0 + 8 * i + pr) * p.ld16 + c0 + 8 * pj) = u;
+        }
+        __syncwarp();
+    };
+    const uint4* own = reinterpret_cast<const uint4*>(h);
+#pragma unroll
+    for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = own[j];
+    put(row0, p.M, col0);
+    if (!mirror) return;
+    // entry (row, col) to (col, row). Two lanes trade halves so that each holds a pair of rows: the even lane of column 2j,
+    // the odd one of column 2j + 1; a column's 32 rows become a row of 64 bytes.
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const __half give = lane & 1 ? __low2half(h[j]) : __high2half(h[j]);
+        const __half got = __ushort_as_half(__shfl_xor_sync(0xffffffffu, __half_as_ushort(give), 1));
+        const __half2 two = lane & 1 ? __halves2half2(got, __high2half(h[j])) : __halves2half2(__low2half(h[j]), got);
+        reinterpret_cast<__half2*>(ns_piece(stage, 2 * j + (lane & 1), lane >> 3))[lane >> 1 & 3] = two;
+    }
+    put(col0, p.N, row0);
+}
+
+// X32 (2^12 X) in the order the epilogue holds it: blocks of 32 x 32, in each the rows' first four columns, then the rows' next
+// four, so that a lane per row reads and writes 512 contiguous bytes an instruction. Offset of row r's columns c .. c + 3.
+__host__ __device__ __forceinline__ int64_t ns_state_at(int64_t r, int64_t c, int64_t ldx) {
+    return ((r >> 5) * (ldx >> 5) + (c >> 5)) * 1024 + (c >> 2 & 7) * 128 + (r & 31) * 4;
+}
+
+// Drains 32 rows x a warp's columns of a finished A or B tile: every lane holds one row, 32 columns at a time. `ready` waits for
+// the accumulator; what else a group of columns needs is loaded before that, and for the next group before this one is
+// written.
 template <class Cfg, int MODE, class Ready>
 __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b, int32_t row0,
-                                                   int32_t col_first, bool mirror, Ready ready) {
+                                                   int32_t col_first, bool mirror, int32_t split, int64_t batch, Ready ready) {
     using namespace ptx;
     __half* out = p.out16 + b * p.stride16;
     const int32_t row = row0 + lane;
-    const int pr = lane >> 2, pj = lane & 3;  // this lane's row (of eight) and piece
+    const int pr = lane >> 2, pj = lane & 3;
     const __half* gram = p.gram + b * p.stride16;
     uint4 g[4];
     const auto fetch = [&](int32_t col0) {
@@ -116,16 +168,6 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
             const int32_t r = row0 + 8 * i + pr;
             g[i] = r < p.M && col0 < p.N ? *reinterpret_cast<const uint4*>(gram + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj) : make_uint4(0, 0, 0, 0);
         }
-    };
-    // Rows r0 .. r0 + 31 (below `rows`) of the 32 x 32 entries in shared memory, to columns c0 .. of the matrix.
-    const auto put = [&](int32_t r0, int32_t rows, int32_t c0, int32_t cols) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
-            if (r0 + 8 * i + pr < rows && c0 + 8 * pj < cols) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r0 + 8 * i + pr) * p.ld16 + c0 + 8 * pj) = u;
-        }
-        __syncwarp();
     };
     const float k1 = p.c1 * kNsUnscale, k2 = p.c2 * kNsUnscale * kNsUnscale;
     if (MODE == NS_POLY) fetch(col_first);
@@ -138,6 +180,16 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
         tmem_ld_32x32(tmem + c0, v);
         tmem_ld_wait();
         __half2 h[16];
+        if (MODE == NS_GRAM && p.splits > 1) {
+            // a part of the sum, as the accumulator has it
+            if (row0 < p.M) {
+                float4* to = reinterpret_cast<float4*>(p.partial + (split * batch + b) * p.stride_part + ns_state_at(row, col0, p.ld16));
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    to[j * 32] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+            }
+            continue;
+        }
         if (MODE == NS_GRAM) {
 #pragma unroll
             for (int j = 0; j < 16; j++)
@@ -161,30 +213,9 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
                 h[j] = __floats2half2_rn(row == c ? 0.f : x, row == c + 1 ? 0.f : y);
             }
         }
-        const uint4* own = reinterpret_cast<const uint4*>(h);
-#pragma unroll
-        for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = own[j];
-        put(row0, p.M, col0, p.ld16);
-        if (mirror) {
-            // entry (row, col) to (col, row). Two lanes trade halves so that each holds a pair of rows: the even lane of
-            // column 2j, the odd one of column 2j + 1; a column's 32 rows become a row of 64 bytes.
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const __half give = lane & 1 ? __low2half(h[j]) : __high2half(h[j]);
-                const __half got = __ushort_as_half(__shfl_xor_sync(0xffffffffu, __half_as_ushort(give), 1));
-                const __half2 two = lane & 1 ? __halves2half2(got, __high2half(h[j])) : __halves2half2(__low2half(h[j]), got);
-                reinterpret_cast<__half2*>(ns_piece(stage, 2 * j + (lane & 1), lane >> 3))[lane >> 1 & 3] = two;
-            }
-            put(col0, p.N, row0, p.ld16);
-        }
+        ns_store_block(p, out, stage, lane, row0, col0, h, mirror);
     }
     return true;
-}
-
-// X32 (2^12 X) in the order the epilogue holds it: blocks of 32 x 32, in each the rows' first four columns, then the rows' next
-// four, so that a lane per row reads and writes 512 contiguous bytes an instruction. Offset of row r's columns c .. c + 3.
-__host__ __device__ __forceinline__ int64_t ns_state_at(int64_t r, int64_t c, int64_t ldx) {
-    return ((r >> 5) * (ldx >> 5) + (c >> 5)) * 1024 + (c >> 2 & 7) * 128 + (r & 31) * 4;
 }
 
 // Drains 32 rows x a warp's columns of a finished B X tile and completes the step, x = diag * x + product, or writes the
@@ -375,11 +406,11 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     if (warp == 0) {
         uint32_t it = 0;
         bool ok = true;
-        for (int64_t tile = first_tile; tile < p.tiles && ok; tile += step) {
-            int32_t mt, nt, b;
-            ns_decode<MODE>(p, tile, mt, nt, b);
+        for (int64_t item = first_tile; item < p.tiles * p.splits && ok; item += step) {
+            int32_t mt, nt, b, k0, k1;
+            ns_decode<MODE>(p, ns_tile<MODE>(p, item, k0, k1), mt, nt, b);
             const int32_t row_a = mt * Cfg::BM + (int32_t)rank * 128, row_b = nt * Cfg::BN + (int32_t)rank * Cfg::B_ROWS;
-            for (int32_t kb = 0; kb < p.k_blocks; kb++, it++) {
+            for (int32_t kb = k0; kb < k1; kb++, it++) {
                 const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
                 if (!mbar_wait_warp(&empty[s], ph ^ 1, abort_flag)) {
                     ok = false;
@@ -418,12 +449,14 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             const uint32_t ka = desc_kstep(p.a_mn), kb_step = desc_kstep(p.b_mn);
             uint32_t it = 0, tcount = 0;
             bool ok = true;
-            for (int64_t tile = first_tile; tile < p.tiles && ok; tile += step, tcount++) {
+            for (int64_t item = first_tile; item < p.tiles * p.splits && ok; item += step, tcount++) {
+                int32_t k0, k1;
+                ns_tile<MODE>(p, item, k0, k1);
                 const uint32_t acc = tcount & 1, aph = (tcount >> 1) & 1;
                 if (!mbar_wait_warp(&tempty[acc], aph ^ 1, abort_flag)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * Cfg::BN;
-                for (int32_t kb = 0; kb < p.k_blocks; kb++, it++) {
+                for (int32_t kb = k0; kb < k1; kb++, it++) {
                     const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
                     if (!mbar_wait_warp(&full[s], ph, abort_flag)) {
                         ok = false;
@@ -436,13 +469,13 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     const int32_t ksteps = kb == p.k_blocks - 1 ? p.last_ksteps : 4;
                     if (elect_one()) {
                         if constexpr (PAIR) {
-                            mma_f16_ss_pair(d_tmem, da, db, idesc, kb > 0 ? 1u : 0u);
+                            mma_f16_ss_pair(d_tmem, da, db, idesc, kb > k0 ? 1u : 0u);
                             if (ksteps > 1) mma_f16_ss_pair(d_tmem, da + ka, db + kb_step, idesc, 1u);
                             if (ksteps > 2) mma_f16_ss_pair(d_tmem, da + 2 * ka, db + 2 * kb_step, idesc, 1u);
                             if (ksteps > 3) mma_f16_ss_pair(d_tmem, da + 3 * ka, db + 3 * kb_step, idesc, 1u);
                             mma_commit_pair(&empty[s]);
                         } else {
-                            mma_f16_ss(d_tmem, da, db, idesc, kb > 0 ? 1u : 0u);
+                            mma_f16_ss(d_tmem, da, db, idesc, kb > k0 ? 1u : 0u);
                             if (ksteps > 1) mma_f16_ss(d_tmem, da + ka, db + kb_step, idesc, 1u);
                             if (ksteps > 2) mma_f16_ss(d_tmem, da + 2 * ka, db + 2 * kb_step, idesc, 1u);
                             if (ksteps > 3) mma_f16_ss(d_tmem, da + 3 * ka, db + 3 * kb_step, idesc, 1u);
@@ -462,9 +495,9 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         const int q = warp & 3;
         float* stage = epi + (warp - 2) * 512;
         uint32_t tcount = 0;
-        for (int64_t tile = first_tile; tile < p.tiles; tile += step, tcount++) {
-            int32_t mt, nt, b;
-            ns_decode<MODE>(p, tile, mt, nt, b);
+        for (int64_t item = first_tile; item < p.tiles * p.splits; item += step, tcount++) {
+            int32_t mt, nt, b, k0, k1;
+            ns_decode<MODE>(p, ns_tile<MODE>(p, item, k0, k1), mt, nt, b);
             const uint32_t acc = tcount & 1, aph = (tcount >> 1) & 1;
             const auto ready = [&] {
                 if (!mbar_wait_warp(&tfull[acc], aph, abort_flag)) return false;
@@ -476,7 +509,7 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             const uint32_t tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * Cfg::BN + col_part;
             bool ok;
             if constexpr (MODE == NS_APPLY) ok = ns_drain_apply<Cfg>(p, tmem, stage, lane, b, row0, col_first, ready);
-            else ok = ns_drain_symmetric<Cfg, MODE>(p, tmem, stage, lane, b, row0, col_first, p.symmetric && mt != nt, ready);
+            else ok = ns_drain_symmetric<Cfg, MODE>(p, tmem, stage, lane, b, row0, col_first, p.symmetric && mt != nt, static_cast<int32_t>(item % p.splits), p.batch, ready);
             if (!ok) break;
             tc_fence_before();
             __syncwarp();
@@ -501,6 +534,43 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         if constexpr (PAIR) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
         else tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
     }
+}
+
+// Adds the parts of a split A and writes it: a warp per block of 32 x 32 on or below the diagonal, and its mirror image.
+__global__ void __launch_bounds__(128)
+ns_gram_sum_kernel(const NsParams p) {
+    __shared__ float stage[4][512];
+    kernel_wait_previous();
+    kernel_allow_next();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int32_t side = (p.M + 31) / 32, per_matrix = side * (side + 1) / 2;
+    const int64_t block = static_cast<int64_t>(blockIdx.x) * 4 + warp, b = block / per_matrix;
+    if (b >= p.batch) return;
+    const int32_t rem = static_cast<int32_t>(block - b * per_matrix);
+    int32_t m = static_cast<int32_t>((sqrtf(8.f * rem + 1.f) - 1.f) * 0.5f);
+    while (m * (m + 1) / 2 > rem) m--;
+    while ((m + 1) * (m + 2) / 2 <= rem) m++;
+    const int32_t row0 = m * 32, col0 = (rem - m * (m + 1) / 2) * 32;
+    const float4* from = reinterpret_cast<const float4*>(p.partial + b * p.stride_part + ns_state_at(row0 + lane, col0, p.ld16));
+    float4 sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum[j] = from[j * 32];
+#pragma unroll 2
+    for (int s = 1; s < p.splits; s++) {
+        const float4* part = from + s * (p.batch * p.stride_part / 4);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float4 v = part[j * 32];
+            sum[j].x += v.x; sum[j].y += v.y; sum[j].z += v.z; sum[j].w += v.w;
+        }
+    }
+    __half2 h[16];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        h[2 * j] = __floats2half2_rn(sum[j].x * kNsUnscale, sum[j].y * kNsUnscale);
+        h[2 * j + 1] = __floats2half2_rn(sum[j].z * kNsUnscale, sum[j].w * kNsUnscale);
+    }
+    ns_store_block(p, p.out16 + b * p.stride16, stage[warp], lane, row0, col0, h, row0 != col0);
 }
 
 // ---- Frobenius norm and first state ---------------------------------------------------------------------------
@@ -641,11 +711,52 @@ ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __rest
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
+// Three tile sizes. A k block of 64 takes a pair of CTAs 565 cycles on its 256 x 256 tile, a CTA 455 on 128 x 128 (bound
+// by shared memory, which holds both operands) and 390 on 128 x 64. Between two tiles of a CTA the epilogue of the
+// first slows the second down (by about half its own length when it is X's, which moves ten bytes an entry); the last
+// epilogue stands alone. Large products are fastest by pairs, products of few tiles by the size that gives every SM one, the
+// smallest by the tile with the shortest way (8192 x 4096: 2.4 ms by pairs, 3.4 by 128 x 128; 256 x 512: 71 us by 128 x 64,
+// 125 by 128 x 128). A = X X^T of a long X has few tiles and a long contraction: then several CTAs share a tile, at the price of
+// another kernel that adds their parts (about 6000 cycles).
+constexpr int kNsSms = 148;  // the workspace does not depend on the device
+enum { NS_PAIR = 0, NS_SINGLE = 1, NS_SMALL = 2 };
+struct NsChoice {
+    int tile, splits;
+};
+static NsChoice ns_choose(int mode, int64_t M, int64_t N, int64_t K, int64_t batch) {
+    struct { int64_t bm, bn, workers, block, epilogue; } const tile[3] = {
+        {256, 256, kNsSms / 2, 565, mode == NS_APPLY ? 10000 : 6000},
+        {128, 128, kNsSms, 455, mode == NS_APPLY ? 4000 : 3000},
+        {128, 64, kNsSms, 390, 2500}};
+    NsChoice best{0, 1};
+    int64_t least = INT64_MAX;
+    for (int t = 0; t < 3; t++) {
+        const int64_t m = (M + tile[t].bm - 1) / tile[t].bm, n = (N + tile[t].bn - 1) / tile[t].bn, blocks = (K + 63) / 64;
+        const int64_t tiles = batch * (mode != NS_APPLY && tile[t].bm == tile[t].bn ? m * (m + 1) / 2 : m * n);
+        const int64_t rounds = (tiles + tile[t].workers - 1) / tile[t].workers;
+        const int64_t whole = rounds * blocks * tile[t].block + (rounds - 1) * (mode == NS_APPLY ? tile[t].epilogue / 2 : 0) + tile[t].epilogue;
+        if (whole < least) {
+            least = whole;
+            best = NsChoice{t, 1};
+        }
+        int64_t splits = tile[t].workers / tiles;
+        if (splits > blocks / 4) splits = blocks / 4;
+        if (mode != NS_GRAM || splits < 2) continue;
+        const int64_t shared = (blocks + splits - 1) / splits * tile[t].block + tile[t].epilogue + 6000;
+        if (shared < least) {
+            least = shared;
+            best = NsChoice{t, (int)splits};
+        }
+    }
+    return best;
+}
+
 struct NsPlan {
     bool tall;
     int64_t S, L, ldx, lda, stridex;  // stridex: floats of a matrix's X32, whole blocks of 32 rows
-    size_t x32, x16, gram, diag, norm;
-    size_t total() const { return x32 + 2 * x16 + 2 * gram + diag + norm; }
+    int splits;      // of the contraction of A
+    size_t x32, x16, gram, diag, norm, part;
+    size_t total() const { return x32 + 2 * x16 + 2 * gram + diag + part + norm; }
 };
 
 static int plan_ns(const nzb_orthogonalize_desc* d, NsPlan* pl) {
@@ -666,6 +777,8 @@ static int plan_ns(const nzb_orthogonalize_desc* d, NsPlan* pl) {
     pl->gram = (size_t)round_up(d->batch * pl->S * pl->lda * 2, 256);
     pl->diag = (size_t)round_up(d->batch * pl->S * 4, 256);
     pl->norm = (size_t)(d->batch * kNormParts * 8);
+    pl->splits = d->batch > 0 && pl->S > 0 ? ns_choose(NS_GRAM, pl->S, pl->S, pl->L, d->batch).splits : 1;
+    pl->part = pl->splits > 1 ? (size_t)(pl->splits * d->batch * round_up(pl->S, 32) * pl->lda * 4) : 0;
     return NZB_OK;
 }
 
@@ -682,8 +795,9 @@ static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, NsPara
     p.symmetric = MODE != NS_APPLY && Cfg::BM == Cfg::BN;
     p.tiles_per_matrix = p.symmetric ? (int64_t)p.tiles_m * (p.tiles_m + 1) / 2 : (int64_t)p.tiles_m * p.tiles_n;
     p.tiles = p.tiles_per_matrix * batch;
+    if (p.splits < 1) p.splits = 1;
     int64_t workers = Cfg::PAIR ? ds.sm_count / 2 : ds.sm_count;
-    if (p.tiles < workers) workers = p.tiles;
+    if (p.tiles * p.splits < workers) workers = p.tiles * p.splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(Cfg::PAIR ? 2 * workers : workers));
     cfg.blockDim = dim3(Cfg::THREADS);
@@ -720,25 +834,15 @@ static int launch_product_of(const NsOperand& a, const NsOperand& b, NsParams& p
     p.b_mn = b.mn;
     return rc == NZB_OK ? launch_product<Cfg, MODE>(tmA, tmB, p, batch, ds, s) : rc;
 }
-
-// Three tile sizes. A k block of 64 takes a pair of CTAs 565 cycles on its 256 x 256 tile, a CTA 455 on 128 x 128 (bound
-// by shared memory, which holds both operands) and 390 on 128 x 64. Between two tiles of a CTA the epilogue of the
-// first slows the second down (by about half its own length when it is X's, which moves ten bytes an entry); the last
-// epilogue stands alone. Large products are fastest by pairs, products of few tiles by the size that gives every SM one, the
-// smallest by the tile with the shortest way (8192 x 4096: 2.4 ms by pairs, 3.4 by 128 x 128; 256 x 512: 71 us by 128 x 64,
-// 125 by 128 x 128).
 template <int MODE>
-static int launch_best(const NsOperand& a, const NsOperand& b, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
-    const auto cycles = [&](int64_t bm, int64_t bn, int64_t workers, int64_t block, int64_t epilogue) {
-        const int64_t m = (p.M + bm - 1) / bm, n = (p.N + bn - 1) / bn;
-        const int64_t tiles = batch * (MODE != NS_APPLY && bm == bn ? m * (m + 1) / 2 : m * n);
-        const int64_t rounds = (tiles + workers - 1) / workers;
-        return rounds * p.k_blocks * block + (rounds - 1) * (MODE == NS_APPLY ? epilogue / 2 : 0) + epilogue;
-    };
-    const int64_t pair = cycles(256, 256, ds.sm_count / 2, 565, MODE == NS_APPLY ? 10000 : 6000);
-    const int64_t single = cycles(128, 128, ds.sm_count, 455, MODE == NS_APPLY ? 4000 : 3000), small = cycles(128, 64, ds.sm_count, 390, 2500);
-    if (pair <= single && pair <= small) return launch_product_of<NsCfg<true, 256>, MODE>(a, b, p, batch, ds, s);
-    if (single <= small) return launch_product_of<NsCfg<false, 128>, MODE>(a, b, p, batch, ds, s);
+static int launch_best(const NsOperand& a, const NsOperand& b, NsParams& p, int64_t K, int64_t batch, const DeviceState& ds, cudaStream_t s) {
+    p.k_blocks = (int32_t)((K + 63) / 64);
+    p.last_ksteps = (int32_t)((K - (int64_t)(p.k_blocks - 1) * 64 + 15) / 16);
+    const NsChoice c = ns_choose(MODE, p.M, p.N, K, batch);
+    p.splits = c.splits;
+    p.batch = batch;
+    if (c.tile == NS_PAIR) return launch_product_of<NsCfg<true, 256>, MODE>(a, b, p, batch, ds, s);
+    if (c.tile == NS_SINGLE) return launch_product_of<NsCfg<false, 128>, MODE>(a, b, p, batch, ds, s);
     return launch_product_of<NsCfg<false, 64>, MODE>(a, b, p, batch, ds, s);
 }
 
@@ -758,10 +862,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
     float* diag = reinterpret_cast<float*>(ws + pl.x32 + 2 * pl.x16 + 2 * pl.gram);
     const NsOperand gram{A16, false, pl.S, pl.S, pl.lda}, poly{B16, false, pl.S, pl.S, pl.lda};
     int rc;
-    const auto contraction = [](NsParams& p, int64_t k) {
-        p.k_blocks = (int32_t)((k + 63) / 64);
-        p.last_ksteps = (int32_t)((k - (int64_t)(p.k_blocks - 1) * 64 + 15) / 16);
-    };
+    float* partial = reinterpret_cast<float*>(ws + pl.x32 + 2 * pl.x16 + 2 * pl.gram + pl.diag);
     for (int step = 0; step < d->steps; step++) {
         const int cur = step & 1;
         NsParams p{};
@@ -771,18 +872,31 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         p.status = ds.status_dev;
         // A = X X^T, or X^T X of a tall matrix
         p.M = p.N = (int32_t)pl.S;
-        contraction(p, pl.L);
         p.out16 = A16;
         p.ld16 = pl.lda;
         p.stride16 = pl.S * pl.lda;
+        p.partial = partial;
+        p.stride_part = round_up(pl.S, 32) * pl.lda;
         const NsOperand x_k{X16[cur], false, d->rows, d->cols, pl.ldx}, x_mn{X16[cur], true, d->rows, d->cols, pl.ldx};
-        rc = launch_best<NS_GRAM>(pl.tall ? x_mn : x_k, pl.tall ? x_mn : x_k, p, d->batch, ds, s);
+        rc = launch_best<NS_GRAM>(pl.tall ? x_mn : x_k, pl.tall ? x_mn : x_k, p, pl.L, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
+        if (p.splits > 1) {
+            const int64_t side = (pl.S + 31) / 32, warps = d->batch * side * (side + 1) / 2;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)((warps + 3) / 4));
+            cfg.blockDim = dim3(128);
+            cfg.stream = s;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, ns_gram_sum_kernel, p));
+        }
         // B = c1 A + c2 A A; A is symmetric, so both operands are read along its rows
-        contraction(p, pl.S);
         p.out16 = B16;
         p.gram = A16;
-        rc = launch_best<NS_POLY>(gram, gram, p, d->batch, ds, s);
+        rc = launch_best<NS_POLY>(gram, gram, p, pl.S, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
         // X = c0 X + B X, or c0 X + X B
         p.M = (int32_t)d->rows;
@@ -803,7 +917,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
             p.w_keep = target.w_keep;
             p.w_step = target.w_step;
         }
-        rc = launch_best<NS_APPLY>(pl.tall ? x_k : poly, pl.tall ? poly : x_mn, p, d->batch, ds, s);
+        rc = launch_best<NS_APPLY>(pl.tall ? x_k : poly, pl.tall ? poly : x_mn, p, pl.S, d->batch, ds, s);
         if (rc != NZB_OK) return rc;
     }
     return NZB_OK;
