@@ -132,7 +132,27 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Calls f with a null pointer of the element type that `dtype` names.
+// Programmatic launch: a kernel may start while the one before it on the stream ends, and waits here until that one has
+// ended and its writes are visible.
+__device__ __forceinline__ void kernel_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void kernel_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Launches such a kernel.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_programmatic(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+// Runs the statement with T as the element type that `dtype` names.
 #define NZB_DISPATCH_DTYPE(dtype, T, ...)                                             \
     do {                                                                              \
         if ((dtype) == NZB_F32) { using T = float; __VA_ARGS__; }                     \

@@ -22,6 +22,9 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortItems = kSortTile / kSortThreads;
 constexpr int kSortMaxBins = 512;
 constexpr int kChunk = 32;                                  // sorted tokens per warp of the sums
+// Up to so many tokens the rows of the others are cleared beside the sums: the sort is short, and two launches are saved
+// (1000 tokens into 30000 x 512: 45 us with them).
+constexpr int kFewTokens = 2048;
 constexpr int kEmbeddingFly = 4;                            // blocks in flight per thread, forward
 
 // What the sort leaves for the sums, per tile.
@@ -57,17 +60,19 @@ template <typename Index>
 __global__ void __launch_bounds__(256)
 embedding_mark_kernel(const Index* __restrict__ index, int64_t tokens, int64_t vocab, int64_t padding, uint32_t* __restrict__ present) {
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    kernel_allow_next();
     if (t >= tokens) return;
     const uint32_t v = sort_key(index[t], vocab, padding);
     if (v != vocab) atomicOr(present + (v >> 5), 1u << (v & 31));
 }
 
-// Clears the rows whose bit is not set: a warp per row.
-__device__ __forceinline__ void clear_rows(const uint32_t* present, float* dtable, int64_t vocab, int64_t dim, int64_t ld_table,
+// Clears the rows that `present` does not name: a warp per row.
+template <class Present>
+__device__ __forceinline__ void clear_rows(Present present, float* dtable, int64_t vocab, int64_t dim, int64_t ld_table,
                                            int64_t warp, int64_t warps, int lane) {
     const uint4 zero = make_uint4(0, 0, 0, 0);
     for (int64_t v = warp; v < vocab; v += warps) {
-        if (present[v >> 5] >> (v & 31) & 1) continue;
+        if (present(v)) continue;
         float* row = dtable + v * ld_table;
         const int lead = row_lead(row);
         for (int64_t c = lane * 4 - lead; c < dim; c += 128) store_block(row, c, dim, zero);
@@ -82,21 +87,25 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
     extern __shared__ uint4 smem_sort[];
     SortSmem& s = *reinterpret_cast<SortSmem*>(smem_sort);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    kernel_allow_next();
     if (blockIdx.x >= tiles) {
-        clear_rows(present, dtable, vocab, dim, ld_table, static_cast<int64_t>(blockIdx.x - tiles) * 32 + warp,
-                   static_cast<int64_t>(gridDim.x - tiles) * 32, lane);
+        kernel_wait_previous();
+        clear_rows([&](int64_t v) { return present[v >> 5] >> (v & 31) & 1; }, dtable, vocab, dim, ld_table,
+                   static_cast<int64_t>(blockIdx.x - tiles) * 32 + warp, static_cast<int64_t>(gridDim.x - tiles) * 32, lane);
         return;
     }
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kSortTile;
     const int count = static_cast<int>(min(static_cast<int64_t>(kSortTile), tokens - t0));
     SortTile& out = out_tiles[blockIdx.x];
     const uint32_t none = static_cast<uint32_t>(vocab);  // sorts behind every token
+    const int rounds = max(1, (count + kSortThreads - 1) / kSortThreads);  // items of a thread: few tokens are soon sorted
 
     uint32_t k[kSortItems];
     uint16_t p[kSortItems];
 #pragma unroll
     for (int i = 0; i < kSortItems; i++) {
-        const int at = warp * (kSortTile / 32) + i * 32 + lane;
+        if (i >= rounds) break;
+        const int at = warp * (rounds * 32) + i * 32 + lane;
         k[i] = at < count ? sort_key(index[t0 + at], vocab, padding) : none;
         p[i] = static_cast<uint16_t>(at);
     }
@@ -110,6 +119,7 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
         uint32_t rank[kSortItems];
 #pragma unroll
         for (int i = 0; i < kSortItems; i++) {
+            if (i >= rounds) break;
             const uint32_t d = (k[i] >> shift) & mask;
             // lanes with the same digit: a ballot per bit (a match instruction takes a turn per different value,
             // which made the pass over the low bits 15 us instead of 4)
@@ -148,6 +158,7 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kSortItems; i++) {
+            if (i >= rounds) break;
             const uint32_t d = (k[i] >> shift) & mask;
             const uint32_t to = s.bin_base[d] + s.hist[warp][d] + rank[i];
             s.key[to] = k[i];
@@ -157,17 +168,19 @@ embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t v
         if (pass + 1 < passes) {
 #pragma unroll
             for (int i = 0; i < kSortItems; i++) {
-                const int at = warp * (kSortTile / 32) + i * 32 + lane;
+                if (i >= rounds) break;
+                const int at = warp * (rounds * 32) + i * 32 + lane;
                 k[i] = s.key[at];
                 p[i] = s.pos[at];
             }
             __syncthreads();
         }
     }
-    for (int i = tid; i < kSortTile; i += kSortThreads) {
+    const int sorted = rounds * kSortThreads;
+    for (int i = tid; i < sorted; i += kSortThreads) {
         out.key[i] = s.key[i];
         out.order[i] = s.pos[i];
-        if (s.key[i] == none ? i == 0 || s.key[i - 1] != none : i == kSortTile - 1) out.count = s.key[i] == none ? i : kSortTile;
+        if (s.key[i] == none ? i == 0 || s.key[i - 1] != none : i == sorted - 1) out.count = s.key[i] == none ? i : sorted;
     }
 }
 
@@ -195,9 +208,28 @@ __device__ __forceinline__ void put_columns(float* row, int64_t c, int64_t dim, 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
 embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile, float* __restrict__ dtable,
-                     float* __restrict__ partial, int64_t dim, int64_t ld_table, int64_t ld_y, float scale, int add, int vec_out) {
+                     float* __restrict__ partial, int64_t vocab, int64_t dim, int64_t ld_table, int64_t ld_y, float scale, int add,
+                     int vec_out, unsigned sum_ctas) {
     constexpr int VEC = Elem<T>::VEC, FLY = 8;  // FLY: rows of dy in flight
     const int lane = threadIdx.x & 31;
+    kernel_wait_previous();
+    kernel_allow_next();
+    if (blockIdx.x >= sum_ctas) {
+        // few tokens: the rows of the others are cleared here, found by halving among the sorted ones
+        const int count = tile->count;
+        const auto present = [&](int64_t v) {
+            int lo = 0, hi = count;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (tile->key[mid] < v) lo = mid + 1;
+                else hi = mid;
+            }
+            return lo < count && tile->key[lo] == v;
+        };
+        clear_rows(present, dtable, vocab, dim, ld_table, static_cast<int64_t>(blockIdx.x - sum_ctas) * 8 + (threadIdx.x >> 5),
+                   static_cast<int64_t>(gridDim.x - sum_ctas) * 8, lane);
+        return;
+    }
     const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     const int64_t blocks = (dim + 32 * VEC - 1) / (32 * VEC);  // column blocks of a row
     const int64_t chunk = item / blocks, c0 = (item - chunk * blocks) * 32 * VEC;
@@ -271,6 +303,8 @@ embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile
 __global__ void __launch_bounds__(256)
 embedding_join_kernel(const SortTile* __restrict__ tile, const float* __restrict__ partial, float* __restrict__ dtable,
                       int64_t dim, int64_t ld_table, float scale, int add) {
+    kernel_wait_previous();
+    kernel_allow_next();
     const int lane = threadIdx.x & 31;
     const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     const int64_t blocks = (dim + 127) / 128;
@@ -427,16 +461,19 @@ static int launch_sort(const nzb_embedding_desc* d, const void* index, const Emb
     while (d->vocab >> bits) bits++;  // vocab itself stands for "no token"
     const int passes = (bits + 8) / 9, digit = (bits + passes - 1) / passes;
     const Index* ip = static_cast<const Index*>(index);
-    unsigned grid = (unsigned)pl.tiles;
-    if (d->overwrite) {
+    const auto sort = embedding_sort_kernel<Index>;
+    if (d->overwrite && d->tokens > kFewTokens) {
         const int64_t first = d->tokens < kSortTile ? d->tokens : kSortTile;
         NZB_CUDA_TRY(cudaMemsetAsync(present, 0, pl.present_bytes, s));
-        if (first) embedding_mark_kernel<Index><<<(unsigned)((first + 255) / 256), 256, 0, s>>>(ip, first, d->vocab, d->padding_index, present);
-        // the sorting CTAs fill an SM each; the others share the rows to clear
-        grid += (unsigned)(sm_count - (pl.tiles < sm_count / 2 ? pl.tiles : 0));
+        embedding_mark_kernel<Index><<<(unsigned)((first + 255) / 256), 256, 0, s>>>(ip, first, d->vocab, d->padding_index, present);
+        // the sorting CTAs, which need not wait for the marks, fill an SM each; the others share the rows to clear
+        const unsigned grid = (unsigned)(pl.tiles + sm_count - (pl.tiles < sm_count / 2 ? pl.tiles : 0));
+        NZB_CUDA_TRY(launch_programmatic(sort, grid, kSortThreads, sizeof(SortSmem), s, ip, d->tokens, d->vocab, d->padding_index, digit,
+                                         passes, (int)pl.tiles, tiles, present, dtable, d->dim, d->ld_table));
+    } else {
+        sort<<<(unsigned)pl.tiles, kSortThreads, sizeof(SortSmem), s>>>(ip, d->tokens, d->vocab, d->padding_index, digit, passes,
+                                                                       (int)pl.tiles, tiles, present, dtable, d->dim, d->ld_table);
     }
-    embedding_sort_kernel<Index><<<grid, kSortThreads, sizeof(SortSmem), s>>>(ip, d->tokens, d->vocab, d->padding_index, digit, passes,
-                                                                            (int)pl.tiles, tiles, present, dtable, d->dim, d->ld_table);
     NZB_CUDA_TRY(cudaGetLastError());
     return NZB_OK;
 }
@@ -506,19 +543,22 @@ int nzb_embedding_backward(const nzb_embedding_desc* d, const void* dy, const vo
         const int add = t > 0 || !d->overwrite;
         const int64_t n = d->tokens - t * kSortTile < kSortTile ? d->tokens - t * kSortTile : kSortTile;
         const int64_t chunks = (n + kChunk - 1) / kChunk;
-        if (chunks == 0) break;
+        const bool clear = d->overwrite && d->tokens <= kFewTokens;
         NZB_DISPATCH_DTYPE(d->dtype, T, {
             const T* from = static_cast<const T*>(dy) + t * kSortTile * d->ld_y;
             const int64_t warps = chunks * ((d->dim + 32 * Elem<T>::VEC - 1) / (32 * Elem<T>::VEC));
-            const unsigned grid = (unsigned)((warps + 7) / 8);
-            if (aligned_to(dy, 16) && d->ld_y * (int64_t)sizeof(T) % 16 == 0)
-                embedding_sum_kernel<T, true><<<grid, 256, 0, s>>>(from, tiles + t, dtable, partial, d->dim, d->ld_table, d->ld_y, d->scale, add, vec_out);
-            else
-                embedding_sum_kernel<T, false><<<grid, 256, 0, s>>>(from, tiles + t, dtable, partial, d->dim, d->ld_table, d->ld_y, d->scale, add, vec_out);
+            const unsigned sum_ctas = (unsigned)((warps + 7) / 8);
+            int64_t clear_ctas = clear ? (d->vocab + 7) / 8 : 0;
+            if (clear_ctas > (int64_t)ds->sm_count * 8) clear_ctas = (int64_t)ds->sm_count * 8;
+            const bool rows_aligned = aligned_to(dy, 16) && d->ld_y * (int64_t)sizeof(T) % 16 == 0;
+            const auto kernel = rows_aligned ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
+            if (sum_ctas + clear_ctas)
+                NZB_CUDA_TRY(launch_programmatic(kernel, sum_ctas + (unsigned)clear_ctas, 256, 0, s, from, tiles + t, dtable, partial, d->vocab, d->dim,
+                                                 d->ld_table, d->ld_y, d->scale, add, vec_out, sum_ctas));
         });
         if (chunks > 1)
-            embedding_join_kernel<<<(unsigned)((chunks * ((d->dim + 127) / 128) + 7) / 8), 256, 0, s>>>(tiles + t, partial, dtable, d->dim, d->ld_table, d->scale, add);
-        NZB_CUDA_TRY(cudaGetLastError());
+            NZB_CUDA_TRY(launch_programmatic(embedding_join_kernel, (unsigned)((chunks * ((d->dim + 127) / 128) + 7) / 8), 256, 0, s, tiles + t, partial,
+                                             dtable, d->dim, d->ld_table, d->scale, add));
     }
     return NZB_OK;
 }

@@ -340,11 +340,6 @@ __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem,
     return true;
 }
 
-// Programmatic launch: a kernel may start while the one before it on the stream ends, and waits here until that one has
-// ended and its writes are visible.
-__device__ __forceinline__ void kernel_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void kernel_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // One product of all matrices. CTA layout (persistent over the tiles): warp 0 TMA producer, warp 1 tensor-memory
 // allocator and MMA issuer, the others epilogue; two accumulators, so that a tile's epilogue runs
 // under the next tile's products. PAIR: two CTAs share a 256 x 256 tile (each loads its 128 rows of both operands).
@@ -882,16 +877,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         if (rc != NZB_OK) return rc;
         if (p.splits > 1) {
             const int64_t side = (pl.S + 31) / 32, warps = d->batch * side * (side + 1) / 2;
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3((unsigned)((warps + 3) / 4));
-            cfg.blockDim = dim3(128);
-            cfg.stream = s;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            attr[0].val.programmaticStreamSerializationAllowed = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            NZB_CUDA_TRY(cudaLaunchKernelEx(&cfg, ns_gram_sum_kernel, p));
+            NZB_CUDA_TRY(launch_programmatic(ns_gram_sum_kernel, (unsigned)((warps + 3) / 4), 128, 0, s, p));
         }
         // B = c1 A + c2 A A; A is symmetric, so both operands are read along its rows
         p.out16 = B16;

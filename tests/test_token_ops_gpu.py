@@ -98,7 +98,8 @@ def _embedding_grad(dy, idx, vocab, scale, padding):
 
 
 @pytest.mark.parametrize("tokens,vocab,dim", [(1, 1, 1), (1, 300, 64), (64, 3, 40), (65, 3, 40), (200, 2, 257), (1000, 70000, 24),
-                                              (16384, 500, 16), (16385, 500, 16), (40000, 33, 12), (5000, 1 << 20, 8)])
+                                              (2048, 300, 16), (2049, 300, 16), (3000, 5000, 200), (16384, 500, 16), (16385, 500, 16),
+                                              (40000, 33, 12), (5000, 1 << 20, 8)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_embedding_backward(tokens, vocab, dim, dtype):
     g = torch.Generator("cuda").manual_seed(5)
@@ -509,6 +510,16 @@ def test_orthogonalize(rows, cols, dtype):
             assert got.dtype == out_dtype and torch.isfinite(got).all()
             assert _rel(got, want) <= ORTHO_TOL + half_step(out_dtype)
         assert torch.equal(got, nz.orthogonalize(g, out_dtype=got.dtype))
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 130, 5000), (1, 5000, 130), (1, 31, 9001), (1, 700, 4100), (2, 4001, 300), (1, 64, 1030)])
+def test_orthogonalize_long_sides(batch, rows, cols):
+    """A long contraction of few tiles is shared among CTAs."""
+    g = torch.stack([_gradient_like(rows, cols, 47 + i) for i in range(batch)])
+    got = nz.orthogonalize(g)
+    for i in range(batch):
+        assert _rel(got[i], _ortho_ref(g[i])) <= ORTHO_TOL
+    assert torch.equal(got, nz.orthogonalize(g))
 
 
 @pytest.mark.parametrize("rows,cols", [(64, 96), (96, 64), (300, 500), (500, 300)])
