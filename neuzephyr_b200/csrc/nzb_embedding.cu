@@ -22,9 +22,10 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortItems = kSortTile / kSortThreads;
 constexpr int kSortMaxBins = 512;
 constexpr int kChunk = 32;                                  // sorted tokens per warp of the sums
-// Up to so many tokens the rows of the others are cleared beside the sums: the sort is short, and two launches are saved
-// (1000 tokens into 30000 x 512: 45 us with them).
-constexpr int kFewTokens = 2048;
+// The rows of the other tokens are cleared beside the sums, not beside the sort, when the sort is short or the table
+// small: two launches less (1000 tokens into 30000 x 512: 25 us instead of 45).
+constexpr int64_t kFewTokens = 2048, kSmallTable = 8 << 20;  // elements
+inline bool clear_beside_sums(const nzb_embedding_desc* d) { return d->tokens <= kFewTokens || d->vocab * d->dim <= kSmallTable; }
 constexpr int kEmbeddingFly = 4;                            // blocks in flight per thread, forward
 
 // What the sort leaves for the sums, per tile.
@@ -206,7 +207,7 @@ __device__ __forceinline__ void put_columns(float* row, int64_t c, int64_t dim, 
 }
 
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, ALIGNED ? 4 : 2)
 embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile, float* __restrict__ dtable,
                      float* __restrict__ partial, int64_t vocab, int64_t dim, int64_t ld_table, int64_t ld_y, float scale, int add,
                      int vec_out, unsigned sum_ctas) {
@@ -462,7 +463,7 @@ static int launch_sort(const nzb_embedding_desc* d, const void* index, const Emb
     const int passes = (bits + 8) / 9, digit = (bits + passes - 1) / passes;
     const Index* ip = static_cast<const Index*>(index);
     const auto sort = embedding_sort_kernel<Index>;
-    if (d->overwrite && d->tokens > kFewTokens) {
+    if (d->overwrite && !clear_beside_sums(d)) {
         const int64_t first = d->tokens < kSortTile ? d->tokens : kSortTile;
         NZB_CUDA_TRY(cudaMemsetAsync(present, 0, pl.present_bytes, s));
         embedding_mark_kernel<Index><<<(unsigned)((first + 255) / 256), 256, 0, s>>>(ip, first, d->vocab, d->padding_index, present);
@@ -543,7 +544,7 @@ int nzb_embedding_backward(const nzb_embedding_desc* d, const void* dy, const vo
         const int add = t > 0 || !d->overwrite;
         const int64_t n = d->tokens - t * kSortTile < kSortTile ? d->tokens - t * kSortTile : kSortTile;
         const int64_t chunks = (n + kChunk - 1) / kChunk;
-        const bool clear = d->overwrite && d->tokens <= kFewTokens;
+        const bool clear = t == 0 && d->overwrite && clear_beside_sums(d);
         NZB_DISPATCH_DTYPE(d->dtype, T, {
             const T* from = static_cast<const T*>(dy) + t * kSortTile * d->ld_y;
             const int64_t warps = chunks * ((d->dim + 32 * Elem<T>::VEC - 1) / (32 * Elem<T>::VEC));
