@@ -573,7 +573,7 @@ NZB_API int nzb_token_logprob_backward(const nzb_token_logprob_desc* desc, const
  * X is held in fp32; the tensor cores read fp16 copies of X, A and B (scaled by 2^12, fp32 sums), the diagonal
  * of B is kept in fp32. Relative error of the result against 64 bits: about 1e-3 (2-norm), whatever out_dtype.
  * Coefficients have to keep the singular values of X below 2.8, as (3.4445, -4.775, 2.0315) do. A matrix of
- * zeros gives zeros.
+ * zeros gives zeros. out may be g.
  */
 typedef struct nzb_orthogonalize_desc {
     int64_t batch, rows, cols;

@@ -162,6 +162,7 @@ inline cudaError_t launch_programmatic(void (*kernel)(Params...), unsigned grid,
 
 inline bool known_dtype(int32_t t) { return t == 0 || t == 1 || t == 2; }
 inline int64_t dtype_size(int32_t t) { return t == 0 ? 4 : 2; }
+inline int64_t index_size(int32_t t) { return t == 0 ? 4 : 8; }
 inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 }  // namespace nzb

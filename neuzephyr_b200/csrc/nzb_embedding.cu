@@ -80,10 +80,12 @@ __device__ __forceinline__ void clear_rows(Present present, float* dtable, int64
     }
 }
 
+// What an earlier kernel of a programmatic launch writes (present, the tiles, the parts) is not `restrict`: such a pointer's
+// loads count as independent of everything else and could move before the wait.
 template <typename Index>
 __global__ void __launch_bounds__(kSortThreads, 1)
 embedding_sort_kernel(const Index* __restrict__ index, int64_t tokens, int64_t vocab, int64_t padding, int digit_bits,
-                      int passes, int tiles, SortTile* __restrict__ out_tiles, const uint32_t* __restrict__ present,
+                      int passes, int tiles, SortTile* __restrict__ out_tiles, const uint32_t* present,
                       float* __restrict__ dtable, int64_t dim, int64_t ld_table) {
     extern __shared__ uint4 smem_sort[];
     SortSmem& s = *reinterpret_cast<SortSmem*>(smem_sort);
@@ -208,7 +210,7 @@ __device__ __forceinline__ void put_columns(float* row, int64_t c, int64_t dim, 
 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2)
-embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile, float* __restrict__ dtable,
+embedding_sum_kernel(const T* __restrict__ dy, const SortTile* tile, float* __restrict__ dtable,
                      float* __restrict__ partial, int64_t vocab, int64_t dim, int64_t ld_table, int64_t ld_y, float scale, int add,
                      int vec_out, unsigned sum_ctas) {
     constexpr int VEC = Elem<T>::VEC, FLY = 8;  // FLY: rows of dy in flight
@@ -302,7 +304,7 @@ embedding_sum_kernel(const T* __restrict__ dy, const SortTile* __restrict__ tile
 
 // Runs over more than one chunk: the warp of the chunk such a run starts in adds its parts, 32 columns x 4.
 __global__ void __launch_bounds__(256)
-embedding_join_kernel(const SortTile* __restrict__ tile, const float* __restrict__ partial, float* __restrict__ dtable,
+embedding_join_kernel(const SortTile* tile, const float* partial, float* __restrict__ dtable,
                       int64_t dim, int64_t ld_table, float scale, int add) {
     kernel_wait_previous();
     kernel_allow_next();
@@ -490,7 +492,7 @@ int nzb_embedding_forward(const nzb_embedding_desc* d, const void* table, const 
     if (rc != NZB_OK) return rc;
     if (d->tokens == 0 || d->dim == 0) return NZB_OK;
     if ((!table && d->vocab > 0) || !index || !y) return fail(NZB_ERR_BAD_ARG, "table, index and y must be non-null");
-    if (!aligned_to(table, dtype_size(d->table_dtype)) || !aligned_to(y, dtype_size(d->dtype)))
+    if (!aligned_to(table, dtype_size(d->table_dtype)) || !aligned_to(y, dtype_size(d->dtype)) || !aligned_to(index, index_size(d->index_type)))
         return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     DeviceState* ds;
     rc = get_device_state(&ds);
@@ -522,7 +524,7 @@ int nzb_embedding_backward(const nzb_embedding_desc* d, const void* dy, const vo
     if (rc != NZB_OK) return rc;
     if (d->vocab == 0 || d->dim == 0 || (d->tokens == 0 && !d->overwrite)) return NZB_OK;
     if (!dtable || (d->tokens > 0 && (!dy || !index))) return fail(NZB_ERR_BAD_ARG, "dy, index and dtable must be non-null");
-    if (!aligned_to(dy, dtype_size(d->dtype)) || !aligned_to(dtable, 4))
+    if (!aligned_to(dy, dtype_size(d->dtype)) || !aligned_to(dtable, 4) || !aligned_to(index, index_size(d->index_type)))
         return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     const EmbeddingPlan pl = plan_embedding(d);
     if (!workspace || workspace_bytes < pl.total())

@@ -558,7 +558,7 @@ int nzb_token_logprob_forward(const nzb_token_logprob_desc* d, const void* logit
     if (d->rows == 0) return NZB_OK;
     if (d->vocab == 0) return fail(NZB_ERR_UNSUPPORTED, "vocab = 0 is not supported");
     if (!logits || (logprob && !targets)) return fail(NZB_ERR_BAD_ARG, "logits and targets must be non-null");
-    if (!aligned_to(logits, dtype_size(d->dtype))) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
+    if (!aligned_to(logits, dtype_size(d->dtype)) || !aligned_to(targets, index_size(d->index_type)) || !aligned_to(top_index, index_size(d->index_type))) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     DeviceState* ds;
     rc = get_device_state(&ds);
     if (rc != NZB_OK) return rc;
@@ -580,7 +580,7 @@ int nzb_token_logprob_backward(const nzb_token_logprob_desc* d, const void* logi
     if (!logits || !targets || !lse || !dlogits || (dentropy && !entropy))
         return fail(NZB_ERR_BAD_ARG, "logits, targets, lse, dlogits (and entropy beside dentropy) must be non-null");
     const int64_t size = dtype_size(d->dtype);
-    if (!aligned_to(logits, size) || !aligned_to(dlogits, size)) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
+    if (!aligned_to(logits, size) || !aligned_to(dlogits, size) || !aligned_to(targets, index_size(d->index_type))) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     DeviceState* ds;
     rc = get_device_state(&ds);
     if (rc != NZB_OK) return rc;

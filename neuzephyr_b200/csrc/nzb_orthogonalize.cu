@@ -676,7 +676,12 @@ ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __rest
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < 8; w++) sum += buf[w];
-    const float div = static_cast<float>(sqrt(sum) + eps);
+    // x / (norm + eps) as x 2^-e / d, so that a norm beyond fp32's range divides too; a zero divisor leaves zeros
+    int e = 0;
+    const double norm = sqrt(sum) + eps;
+    if (norm > 0.0 && norm <= 1.7e308) frexp(norm, &e);
+    e = max(-100, min(100, e));
+    const float div = norm == 0.0 ? 1.f : static_cast<float>(ldexp(norm, -e)), pre = exp2f(static_cast<float>(-e));
 #pragma unroll 2
     for (NsGroups<false> it(rows, cols); it.more(); it.next()) {
         int64_t r, c;
@@ -693,7 +698,7 @@ ns_start_kernel(const T* __restrict__ g, float* __restrict__ X32, __half* __rest
         }
         uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = v[i] / div * kNsScale;
+        for (int i = 0; i < 8; i++) v[i] = v[i] * pre / div * kNsScale;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const __half2 two = __floats2half2_rn(v[2 * i], v[2 * i + 1]);

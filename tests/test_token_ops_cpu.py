@@ -40,6 +40,7 @@ def test_embedding_pointers_and_workspace():
     assert L.nzb_embedding_forward(ctypes.byref(d), FAKE, None, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_embedding_forward(ctypes.byref(d), FAKE, FAKE, FAKE + 1, None) == C.ERR_BAD_ARG
     assert L.nzb_embedding_forward(ctypes.byref(d), FAKE + 2, FAKE, FAKE, None) == C.ERR_BAD_ARG
+    assert L.nzb_embedding_forward(ctypes.byref(d), FAKE, FAKE + 4, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_embedding_backward_workspace_bytes(ctypes.byref(d), None) == C.ERR_BAD_ARG
     assert L.nzb_embedding_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(n)) == C.OK and n.value > 0
     small = n.value
@@ -113,6 +114,7 @@ def test_token_logprob_pointers():
     assert L.nzb_token_logprob_forward(ctypes.byref(d), None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_token_logprob_forward(ctypes.byref(d), FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_token_logprob_forward(ctypes.byref(d), FAKE + 2, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
+    assert L.nzb_token_logprob_forward(ctypes.byref(d), FAKE, FAKE + 4, FAKE, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_token_logprob_backward(ctypes.byref(d), FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_token_logprob_backward(ctypes.byref(d), FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
     assert L.nzb_token_logprob_backward(ctypes.byref(_logprob(ld_dlogits=299)), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
