@@ -56,6 +56,8 @@ protected:
     Node* Bias(Node* input);
     Node* Reshape(Node* input, const data::Tensor::shape_type& shape);
     Node* Linear(Node* input, size_t outSize);
+    // layer norm over each sample, gamma 1 and beta 0 at the start
+    Node* LayerNorm(Node* input, float eps = 1e-5f);
     Node* ReLU(Node* input);
     Node* Softmax(Node* input);
     Node* TargetExpand(Node* input, const data::Tensor::shape_type& shape);

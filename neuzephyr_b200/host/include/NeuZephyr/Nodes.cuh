@@ -2,7 +2,7 @@
 // io::InputNode; calc::{Add, MatMul, ReLU, Reshape, Expand, Img2Col, Col2Img, AveragePooling,
 // Softmax}Node; loss::BinaryCrossEntropyNode; plus two fused nodes without a counterpart in the
 // reference, calc::Conv2dNode and calc::LinearNode, that collapse the compositions Model::Conv2d
-// and Model::Linear build. Gradient write semantics (overwrite vs accumulate) follow the
+// and Model::Linear build, and calc::LayerNormNode, which has none either. Gradient write semantics (overwrite vs accumulate) follow the
 // reference node by node.
 #pragma once
 #include <memory>
@@ -188,6 +188,21 @@ public:
 
 private:
     bool relu_;
+};
+
+// Layer norm over all elements of a sample (no counterpart in the reference): y = (x - mean) / sqrt(var + eps) * gamma +
+// beta for each of the N samples of C*H*W elements. inputs: {x, gamma, beta}, the last two of C*H*W values;
+// output of x's shape.
+class LayerNormNode : public Node {
+public:
+    LayerNormNode(Node* x, Node* gamma, Node* beta, float eps = 1e-5f);
+    void forward() override;
+    void backward() override;
+    std::vector<size_t> attributes() const override;  // eps, by its bits
+
+private:
+    float eps_;
+    std::unique_ptr<Tensor> mean_, rstd_;  // one number a sample, for the backward pass
 };
 }  // namespace calc
 

@@ -1,5 +1,5 @@
 // Optimizers used by the training step (mirrors include/NeuZephyr/Optimizer.cuh,
-// src/Optimizer.cu:79-102): SGD and Adam. Adam keeps the reference's quirk of one time step per
+// src/Optimizer.cu:79-102): SGD and Adam, and Muon beside them. Adam keeps the reference's quirk of one time step per
 // step(Node*) call (the counter is shared by all parameters), eps 1e-6.
 #pragma once
 #include <memory>
@@ -80,6 +80,32 @@ private:
     bool batching_ = false;
     std::vector<std::pair<nodes::Node*, int>> batch_;  // (node, time step) collected between begin / endBatch
     std::unordered_map<nodes::Node*, std::unique_ptr<data::Tensor>> m_, v_;
+};
+
+// Muon (no counterpart in the reference): momentum, then the update with its singular values brought near 1 by five
+// Newton-Schulz products (nzb_muon); w = (1 - lr * weight_decay) * w - lr * sqrt(max(1, H / W)) * update. It takes parameters
+// whose H and W are above 1, as N*C matrices; the others (biases, norms) go to `others`, which the caller owns and which
+// keeps its own learning rate, counter and state.
+class Muon : public Optimizer {
+public:
+    Muon(float learning_rate, float momentum, Optimizer* others = nullptr, float weight_decay = 0.f, bool nesterov = true);
+    void step(nodes::Node* input) override;
+    void skip(int n) override { if (others_) others_->skip(n); }
+    void beginBatch() override { if (others_) others_->beginBatch(); }
+    void endBatch() override { if (others_) others_->endBatch(); }
+    const char* name() const override { return "Muon"; }
+    long counter() const override { return others_ ? others_->counter() : 0; }
+    void setCounter(long it) override { if (others_) others_->setCounter(it); }
+    // {momentum} of a matrix, in host memory; the state of `others` for the rest
+    std::vector<std::vector<float>> exportState(nodes::Node* node) const override;
+    void importState(nodes::Node* node, const std::vector<std::vector<float>>& state) override;
+
+private:
+    static bool isMatrix(nodes::Node* node);
+    float mu_, weight_decay_;
+    bool nesterov_;
+    Optimizer* others_;
+    std::unordered_map<nodes::Node*, std::unique_ptr<data::Tensor>> momentum_;
 };
 
 }  // namespace nz::opt

@@ -71,7 +71,7 @@ void ComputeGraph::overwriteSingleConsumerGradients(bool on) {
             Node* u = users[n][0];
             const bool first = !u->inputs.empty() && u->inputs[0] == n &&
                                std::count(u->inputs.begin(), u->inputs.end(), n) == 1;
-            mark = first && (u->type == "Conv2d" || u->type == "Linear" || u->type == "AveragePooling");
+            mark = first && (u->type == "Conv2d" || u->type == "Linear" || u->type == "LayerNorm" || u->type == "AveragePooling");
         }
         // an output node shares its input's tensor: never mark that one
         for (Node* o : outputs_)
@@ -284,7 +284,12 @@ void ComputeGraph::load(const std::string& path, opt::Optimizer* optimizer) {
                                      attr(2), attr(3), attr(4) != 0);
         else if (r.type == "Linear")
             n = new calc::LinearNode(in_node(0), in_node(1), r.pre.size() > 2 ? in_node(2) : nullptr, attr(0) != 0);
-        else if (r.type == "BinaryCrossEntropy") n = out = new nodes::loss::BinaryCrossEntropyNode(in_node(0), in_node(1));
+        else if (r.type == "LayerNorm") {
+            const uint32_t bits = (uint32_t)attr(0);
+            float eps;
+            memcpy(&eps, &bits, sizeof(eps));
+            n = new calc::LayerNormNode(in_node(0), in_node(1), in_node(2), eps);
+        } else if (r.type == "BinaryCrossEntropy") n = out = new nodes::loss::BinaryCrossEntropyNode(in_node(0), in_node(1));
         else throw std::runtime_error("node type '" + r.type + "' is not part of this library");
         owned_.emplace_back(n);
         created.push_back(n);
@@ -401,6 +406,66 @@ void Adam::endBatch() {
         sm.recordRead(t.grad(), s);
     }
     batch_.clear();
+}
+
+Muon::Muon(float lr, float mu, Optimizer* others, float weight_decay, bool nesterov)
+    : mu_(mu), weight_decay_(weight_decay), nesterov_(nesterov), others_(others) {
+    learning_rate = lr;
+}
+bool Muon::isMatrix(nodes::Node* node) {
+    const auto s = node->output->shape();
+    return s.H() > 1 && s.W() > 1;
+}
+void Muon::step(nodes::Node* input) {
+    const auto slice = slices_.find(input);
+    if (!isMatrix(input)) {
+        if (!others_) throw std::invalid_argument("Muon updates matrices only: give it another optimizer for the other parameters");
+        if (slice != slices_.end()) others_->setSlice(input, slice->second.first, slice->second.second);
+        else others_->setSlice(input, 0, 0);
+        others_->step(input);
+        return;
+    }
+    if (slice != slices_.end()) throw std::runtime_error("Muon needs whole matrices: it cannot take a sharded optimizer's slice");
+    data::Tensor& t = *input->output;
+    auto& m = momentum_[input];
+    if (!m) {
+        m = std::make_unique<data::Tensor>(t.shape());
+        m->clear();
+    }
+    const auto s = t.shape();
+    nzb_orthogonalize_desc d{};
+    d.batch = (int64_t)(s.N() * s.C());
+    d.rows = (int64_t)s.H();
+    d.cols = (int64_t)s.W();
+    d.coef[0] = 3.4445f; d.coef[1] = -4.7750f; d.coef[2] = 2.0315f;
+    d.eps = 1e-7f;
+    d.steps = 5;
+    const float scale = s.H() > s.W() ? std::sqrt((float)s.H() / (float)s.W()) : 1.f;
+    size_t bytes = 0;
+    NZB_CHECK(nzb_muon_workspace_bytes(&d, &bytes));
+    SM::Instance().run({t.data(), m->data()}, {t.grad()}, [&](cudaStream_t st) {
+        void* ws = SM::Instance().scratch(bytes, st);
+        const int rc = nzb_muon(&d, t.data(), m->data(), t.grad(), learning_rate, scale, mu_, weight_decay_, nesterov_, ws, bytes, st);
+        SM::Instance().releaseScratch(ws, st);
+        NZB_CHECK(rc);
+    });
+}
+std::vector<std::vector<float>> Muon::exportState(nodes::Node* node) const {
+    if (!isMatrix(node)) return others_ ? others_->exportState(node) : std::vector<std::vector<float>>{};
+    auto m = momentum_.find(node);
+    if (m == momentum_.end() || !m->second) return {};
+    return {m->second->hostData()};
+}
+void Muon::importState(nodes::Node* node, const std::vector<std::vector<float>>& state) {
+    if (!isMatrix(node)) {
+        if (others_) others_->importState(node, state);
+        return;
+    }
+    if (state.size() != 1 || state[0].size() != node->output->size())
+        throw std::runtime_error("Muon state of a node does not match its size");
+    auto& m = momentum_[node];
+    m = std::make_unique<data::Tensor>(node->output->shape());
+    m->dataInject(const_cast<float*>(state[0].data()));
 }
 
 std::vector<std::vector<float>> Adam::exportState(nodes::Node* node) const {
@@ -556,6 +621,18 @@ Model::Node* Model::Linear(Node* input, size_t outSize) {
     w->output->randomize();
     own(w, true);
     return Bias(Mul(w, shaped));
+}
+Model::Node* Model::LayerNorm(Node* input, float eps) {
+    computeGraph.addNode(input);
+    const auto s = input->output->shape();
+    const Dimension row(1, 1, 1, s[1] * s[2] * s[3]);
+    auto* gamma = new io::InputNode(row, true);
+    gamma->output->fill(1.f);
+    own(gamma, true);
+    auto* beta = new io::InputNode(row, true);
+    beta->output->fill(0.f);
+    own(beta, true);
+    return own(new calc::LayerNormNode(input, gamma, beta, eps));
 }
 Model::Node* Model::ReLU(Node* input) {
     computeGraph.addNode(input);

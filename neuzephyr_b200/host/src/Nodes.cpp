@@ -4,6 +4,8 @@
 #include <NeuZephyr/Nodes.cuh>
 #include <NeuZephyr/TensorOperations.cuh>
 
+#include <cstring>
+
 #include <nzb.h>
 
 namespace nz::nodes {
@@ -441,6 +443,59 @@ void LinearNode::backward() {
         void* ws = SM::Instance().scratch(bytes, s);
         const int rc = nzb_linear_backward(&d, x.data(), w.data(), output->data(), output->grad(), dx, dw, db, ws,
                                            bytes, s);
+        SM::Instance().releaseScratch(ws, s);
+        NZB_CHECK(rc);
+    });
+}
+
+LayerNormNode::LayerNormNode(Node* x, Node* gamma, Node* beta, float eps) : eps_(eps) {
+    if (!x || !gamma || !beta) throw std::invalid_argument("LayerNormNode: x, gamma and beta must be given");
+    const auto sx = x->output->shape();
+    const size_t dim = sx.C() * sx.H() * sx.W();
+    if (gamma->output->size() != dim || beta->output->size() != dim)
+        throw std::invalid_argument("LayerNormNode: gamma and beta must hold one value per element of a sample");
+    if (!(eps >= 0.f)) throw std::invalid_argument("LayerNormNode: eps must not be negative");
+    inputs = {x, gamma, beta};
+    output = std::make_shared<Tensor>(sx, true);
+    mean_ = std::make_unique<Tensor>(Dimension(sx.N(), 1, 1, 1));
+    rstd_ = std::make_unique<Tensor>(Dimension(sx.N(), 1, 1, 1));
+    type = "LayerNorm";
+}
+std::vector<size_t> LayerNormNode::attributes() const {
+    uint32_t bits;
+    memcpy(&bits, &eps_, sizeof(bits));
+    return {bits};
+}
+static nzb_layernorm_desc layernorm_desc(const Tensor& x, float eps) {
+    nzb_layernorm_desc d{};
+    d.rows = x.shape().N();
+    d.dim = d.ld_x = d.ld_y = d.ld_dx = (int64_t)(x.shape().C() * x.shape().H() * x.shape().W());
+    d.eps = eps;
+    d.dtype = NZB_F32;
+    return d;
+}
+void LayerNormNode::forward() {
+    const Tensor& x = *inputs[0]->output;
+    const Tensor &g = *inputs[1]->output, &b = *inputs[2]->output;
+    const nzb_layernorm_desc d = layernorm_desc(x, eps_);
+    SM::Instance().run({output->data(), mean_->data(), rstd_->data()}, {x.data(), g.data(), b.data()}, [&](cudaStream_t s) {
+        NZB_CHECK(nzb_layernorm_forward(&d, x.data(), g.data(), b.data(), output->data(), mean_->data(), rstd_->data(), s));
+    });
+}
+void LayerNormNode::backward() {
+    const Tensor& x = *inputs[0]->output;
+    const Tensor &g = *inputs[1]->output, &b = *inputs[2]->output;
+    nzb_layernorm_desc d = layernorm_desc(x, eps_);
+    d.overwrite_dx = x.gradOverwritten() ? 1 : 0;
+    float* dx = x.requiresGrad() ? x.grad() : nullptr;
+    float* dg = g.requiresGrad() ? g.grad() : nullptr;
+    float* db = b.requiresGrad() ? b.grad() : nullptr;
+    size_t bytes = 0;
+    NZB_CHECK(nzb_layernorm_backward_workspace_bytes(&d, &bytes));
+    SM::Instance().run({dx, dg, db}, {x.data(), g.data(), mean_->data(), rstd_->data(), output->grad()}, [&](cudaStream_t s) {
+        void* ws = SM::Instance().scratch(bytes, s);
+        const int rc = nzb_layernorm_backward(&d, output->grad(), x.data(), mean_->data(), rstd_->data(), g.data(), dx, dg, db,
+                                              ws, bytes, s);
         SM::Instance().releaseScratch(ws, s);
         NZB_CHECK(rc);
     });
