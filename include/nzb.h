@@ -515,11 +515,11 @@ NZB_API int nzb_embedding_backward(const nzb_embedding_desc* desc, const void* d
 /*
  * Layer norm over the last dimension: mean and variance of each row (the variance from the centred row),
  * rstd = 1 / sqrt(var + eps), y = (x - mean) * rstd * gamma + beta. gamma and beta (fp32, {dim}) may be null
- * (1 and 0), mean and rstd (fp32, {rows}) may be null when nothing reads them. y may be x.
+ * (1 and 0), mean and rstd (fp32, {rows}) may be null when nothing reads them. y may be x (with its ld).
  * Backward, with h = (x - mean) * rstd and g = dy * gamma:
  *   dx (+)= rstd * (g - mean(g) - h * mean(g * h))     = with overwrite_dx, += without
  *   dgamma (+)= sum over rows of dy * h, dbeta (+)= sum over rows of dy      = with overwrite_dparams
- * Null outputs are skipped. dx may be dy. dtype is the type of x, y, dy and dx.
+ * Null outputs are skipped. dx may be dy or x (with its ld). dtype is the type of x, y, dy and dx.
  */
 typedef struct nzb_layernorm_desc {
     int64_t rows, dim;
@@ -538,7 +538,7 @@ NZB_API int nzb_layernorm_backward(const nzb_layernorm_desc* desc, const void* d
                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * Log probabilities of given tokens: with z = scale * logits (scale > 0, the inverse temperature) and
+ * Log probabilities of given tokens: with z = scale * logits (scale, the inverse temperature, in [1e-4, 1e6]) and
  * lse = ln sum exp z over each row of `vocab` logits,
  *   logprob[r] = z[target[r]] - lse, entropy[r] = -sum p ln p with p = exp(z - lse),
  *   top_logprob / top_index {rows, top_k}: the top_k largest logits' log probabilities and columns, largest
@@ -546,10 +546,11 @@ NZB_API int nzb_layernorm_backward(const nzb_layernorm_desc* desc, const void* d
  * Any output may be null. Targets and top_index have the type index_type. A target outside [0, vocab) stands
  * for a position without one: its logprob is 0. Logits of -2^27 and less (-inf, -1e9, the lowest fp32 or bf16
  * number) are masked: probability 0 beside any other. A row of masked logits is empty: lse and its log
- * probabilities are -inf, its entropy is 0. A NaN or +inf in a row makes the row's results NaN; a NaN ranks with -inf among the alternatives.
+ * probabilities are -inf, its entropy is 0. A NaN or +inf in a row makes the row's results NaN; a NaN ranks with
+ * -inf among the alternatives. Beyond 1e37 / scale a logit's lse may leave fp32's range, and no gradient is defined.
  * Backward: dlogits = scale * (dlogprob * (1[target] - p) - dentropy * p * (ln p + entropy)), from lse and
  * entropy of the forward pass; dlogprob or dentropy may be null (0), entropy too when dentropy is. Rows that
- * are empty get zeros; positions without a target only the entropy's part. dlogits may be logits.
+ * are empty get zeros; positions without a target only the entropy's part. dlogits may be logits (with its ld).
  */
 typedef struct nzb_token_logprob_desc {
     int64_t rows, vocab;
@@ -594,7 +595,7 @@ NZB_API int nzb_orthogonalize(const nzb_orthogonalize_desc* desc, const void* g,
  * One Muon step on a weight matrix (fp32, like nzb_adam): momentum = mu * momentum + grad, u = momentum or,
  * with nesterov, grad + mu * momentum, w = (1 - lr * weight_decay) * w - lr * scale * orthogonalised(u).
  * desc gives the matrix (batch, rows, cols, coefficients, steps, eps); its strides and types are not used:
- * w, momentum and grad are contiguous.
+ * w, momentum and grad are contiguous, momentum apart from the others.
  */
 NZB_API int nzb_muon_workspace_bytes(const nzb_orthogonalize_desc* desc, size_t* bytes_out);
 NZB_API int nzb_muon(const nzb_orthogonalize_desc* desc, float* w, float* momentum, const float* grad, float lr,

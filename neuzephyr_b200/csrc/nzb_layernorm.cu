@@ -37,6 +37,7 @@ template <typename T, int ELEMS>
 constexpr int norm_max_threads() { return ELEMS == 32 ? 640 : 1024; }
 constexpr int kNormBackwardMaxThreads = 512;  // backward: 32 sums and the row's 32 factors per thread
 constexpr int kNormSmem = 225 * 1024;          // dynamic shared memory of a CTA
+constexpr int kNormLongParts = 64;
 constexpr int kNormSms = 148;      // the workspace holds one pair of sums per CTA of a grid over this many SMs
 
 // A thread's share of a row: the blocks t, t + nt, ... of VPT. The same for every row of a residue.
@@ -94,6 +95,8 @@ struct RowShare {
         else if (has(k)) store_block(row, first(k), dim, Elem<T>::pack(f));
     }
 };
+// Rows at either end of a tensor whose blocks may reach beyond it: more than one when a block holds several rows.
+__device__ __forceinline__ int border_rows(int64_t ld, int vec) { return ld < vec ? vec : 1; }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -120,6 +123,7 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
     const int residue = blockIdx.x % period;
     const int lead = EXACT ? 0 : row_lead(x + residue * ld_x);
     const int64_t span = (rows - 1) * ld_x + dim;
+    const int edge = border_rows(ld_x, VEC);
     const int64_t step = static_cast<int64_t>(gridDim.x / period) * groups * period;
     const int64_t first_row = residue + static_cast<int64_t>(period) * (static_cast<int64_t>(blockIdx.x / period) * groups + group);
     const RowShare<T, VPT> share(t, nt, lead, dim);
@@ -130,7 +134,7 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
             if (!share.has(k % VPT)) ring[k * nt] = make_uint4(0, 0, 0, 0);
     }
     const auto fetch = [&](int64_t r, int stage) {
-        if (r < rows) share.fetch(ring + stage * VPT * nt, nt, x, r * ld_x, span, !EXACT && (r == 0 || r == rows - 1));
+        if (r < rows) share.fetch(ring + stage * VPT * nt, nt, x, r * ld_x, span, !EXACT && (r < edge || r >= rows - edge));
         copies_commit();
     };
 #pragma unroll
@@ -302,6 +306,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
     const int residue = static_cast<int>(walker % period);
     const int lead = EXACT ? 0 : row_lead(x + residue * ld_x);
     const int64_t span_x = (rows - 1) * ld_x + dim, span_dy = (rows - 1) * ld_dy + dim;
+    const int edge = border_rows(min(ld_x, ld_dy), VEC);
     const int64_t step = walkers / period * groups * period;
     const int64_t first_row = residue + period * (walker / period * groups + group);
     const RowShare<T, VPT> share(t, nt, lead, dim);
@@ -313,7 +318,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
     }
     const auto fetch = [&](int64_t r, int stage) {
         if (r < rows) {
-            const bool border = !EXACT && (r == 0 || r == rows - 1);
+            const bool border = !EXACT && (r < edge || r >= rows - edge);
             share.fetch(ring + stage * 2 * VPT * nt, nt, x, r * ld_x, span_x, border);
             share.fetch(ring + (stage * 2 + 1) * VPT * nt, nt, dy, r * ld_dy, span_dy, border);
         }
@@ -547,9 +552,11 @@ static int norm_threads(int64_t dim, int lead, int most, int elems) {
     const int64_t nt = round_up((dim + lead + elems - 1) / elems, 32);
     return nt <= most ? (int)nt : 0;
 }
-// CTAs of the backward kernels, at most: one for each SM, and one per residue at least.
+// CTAs of the backward kernels, at most: one for each SM, and one per residue at least; 64 of the kernel that takes the
+// longest rows, so that its workspace stays small beside them.
 static int64_t norm_parts(const nzb_layernorm_desc* d) {
-    const int64_t ctas = d->rows < kNormSms ? d->rows : kNormSms;
+    const int64_t most = d->dim > (int64_t)kNormMaxCluster * kNormBackwardMaxThreads * kNormElems ? kNormLongParts : kNormSms;
+    const int64_t ctas = d->rows < most ? d->rows : most;
     return ctas < 8 ? 8 : ctas;
 }
 
@@ -602,6 +609,7 @@ int nzb_layernorm_forward(const nzb_layernorm_desc* d, const void* x, const floa
     if (rc != NZB_OK) return rc;
     if (d->rows == 0 || d->dim == 0) return NZB_OK;
     if (!x || !y) return fail(NZB_ERR_BAD_ARG, "x and y must be non-null");
+    if (x == y && d->ld_x != d->ld_y) return fail(NZB_ERR_BAD_ARG, "y in place of x needs its leading dimension");
     const int64_t size = dtype_size(d->dtype);
     if (!aligned_to(x, size) || !aligned_to(y, size)) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     DeviceState* ds;
@@ -669,6 +677,8 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
     const bool params = dgamma || dbeta;
     if (d->dim == 0 || (!dx && !params)) return NZB_OK;
     if (dx && d->ld_dx < d->dim) return fail(NZB_ERR_BAD_ARG, "leading dimension smaller than the row length");
+    if (dx && ((dx == dy && d->ld_dx != d->ld_y) || (dx == x && d->ld_dx != d->ld_x)))
+        return fail(NZB_ERR_BAD_ARG, "dx in place of dy or x needs its leading dimension");
     DeviceState* ds;
     rc = get_device_state(&ds);
     if (rc != NZB_OK) return rc;
@@ -715,7 +725,7 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
             const T* xp = static_cast<const T*>(x);
             const T* dyp = static_cast<const T*>(dy);
             if (params) {
-                if (parts > 64) parts = 64;
+                if (parts > kNormLongParts) parts = kNormLongParts;
                 const dim3 grid((unsigned)((d->dim + 255) / 256), (unsigned)parts);
                 layernorm_dparams_kernel<T><<<grid, 256, 0, s>>>(dyp, xp, mean, rstd, partial, d->rows, (int)d->dim, d->ld_x, d->ld_y);
             }

@@ -433,7 +433,8 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
     const float log_s = log2f(all.s);
     if (t == 0) {
         if (lse_out) lse_out[r] = empty ? -INFINITY : fmaf(all.top, scale, log_s * kLn2);
-        if (entropy) entropy[r] = empty ? 0.f : (log_s - all.w / all.s) * kLn2;
+        // a sum w of NaN beside a finite s: a logit so large (above 2^126) that u left fp32's range. Then every e is 0 or 1
+        if (entropy) entropy[r] = empty ? 0.f : (log_s - (all.w == all.w || all.s != all.s ? all.w / all.s : 0.f)) * kLn2;
         if (logprob) {
             const int64_t tgt = static_cast<int64_t>(targets[r]);
             float lp = 0.f;
@@ -539,7 +540,8 @@ static int check_logprob(const nzb_token_logprob_desc* d) {
     if (d->rows > 65535ll * 32768 || d->vocab > (1 << 28)) return fail(NZB_ERR_UNSUPPORTED, "vocab at most 2^28, rows below 2^31");
     if (!known_dtype(d->dtype)) return fail(NZB_ERR_BAD_ARG, "unknown element type");
     if (d->index_type != NZB_I32 && d->index_type != NZB_I64) return fail(NZB_ERR_BAD_ARG, "unknown index type");
-    if (!(d->scale > 0.f) || d->scale > 1e6f) return fail(NZB_ERR_BAD_ARG, "scale must be in (0, 1e6]");
+    // below 1e-4 a masked logit's 2^27 would leave it a probability
+    if (!(d->scale >= 1e-4f) || d->scale > 1e6f) return fail(NZB_ERR_BAD_ARG, "scale must be in [1e-4, 1e6]");
     if (d->ld_logits < d->vocab) return fail(NZB_ERR_BAD_ARG, "leading dimension smaller than the row length");
     return NZB_OK;
 }
@@ -579,6 +581,7 @@ int nzb_token_logprob_backward(const nzb_token_logprob_desc* d, const void* logi
     if (d->rows == 0 || d->vocab == 0) return NZB_OK;
     if (!logits || !targets || !lse || !dlogits || (dentropy && !entropy))
         return fail(NZB_ERR_BAD_ARG, "logits, targets, lse, dlogits (and entropy beside dentropy) must be non-null");
+    if (logits == dlogits && d->ld_logits != d->ld_dlogits) return fail(NZB_ERR_BAD_ARG, "dlogits in place of logits needs their leading dimension");
     const int64_t size = dtype_size(d->dtype);
     if (!aligned_to(logits, size) || !aligned_to(dlogits, size) || !aligned_to(targets, index_size(d->index_type))) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     DeviceState* ds;

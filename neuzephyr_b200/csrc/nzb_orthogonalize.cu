@@ -949,6 +949,7 @@ int nzb_orthogonalize(const nzb_orthogonalize_desc* d, const void* g, void* out,
     if (!known_dtype(d->dtype) || !known_dtype(d->out_dtype)) return fail(NZB_ERR_BAD_ARG, "unknown element type");
     if (d->ld_g < d->cols || d->ld_out < d->cols) return fail(NZB_ERR_BAD_ARG, "leading dimension smaller than the row length");
     if (d->batch == 0 || d->rows == 0 || d->cols == 0) return NZB_OK;
+    if (d->batch > 1 && d->stride_out < d->cols) return fail(NZB_ERR_BAD_ARG, "output matrices overlap");
     if (!g || !out) return fail(NZB_ERR_BAD_ARG, "g and out must be non-null");
     if (!aligned_to(g, dtype_size(d->dtype)) || !aligned_to(out, dtype_size(d->out_dtype)))
         return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
@@ -987,6 +988,7 @@ int nzb_muon(const nzb_orthogonalize_desc* d, float* w, float* momentum, const f
     if (rc != NZB_OK) return rc;
     if (d->batch == 0 || d->rows == 0 || d->cols == 0) return NZB_OK;
     if (!w || !momentum || !grad) return fail(NZB_ERR_BAD_ARG, "w, momentum and grad must be non-null");
+    if (w == momentum || grad == momentum) return fail(NZB_ERR_BAD_ARG, "momentum needs memory of its own");
     if (!aligned_to(w, 4) || !aligned_to(momentum, 4) || !aligned_to(grad, 4))
         return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
     rc = check_ws(pl, workspace, workspace_bytes);

@@ -98,7 +98,7 @@ def _logprob(**kw):
 @pytest.mark.parametrize("change,code", [
     (dict(rows=-1), C.ERR_BAD_ARG), (dict(vocab=-1), C.ERR_BAD_ARG), (dict(ld_logits=299), C.ERR_BAD_ARG),
     (dict(scale=0.0), C.ERR_BAD_ARG), (dict(scale=-1.0), C.ERR_BAD_ARG), (dict(scale=float("nan")), C.ERR_BAD_ARG),
-    (dict(scale=float("inf")), C.ERR_BAD_ARG), (dict(dtype=3), C.ERR_BAD_ARG), (dict(index_type=-1), C.ERR_BAD_ARG),
+    (dict(scale=float("inf")), C.ERR_BAD_ARG), (dict(scale=9e-5), C.ERR_BAD_ARG), (dict(dtype=3), C.ERR_BAD_ARG), (dict(index_type=-1), C.ERR_BAD_ARG),
     (dict(top_k=33), C.ERR_BAD_ARG), (dict(top_k=-1), C.ERR_BAD_ARG), (dict(vocab=3, top_k=4), C.ERR_BAD_ARG),
     (dict(vocab=0, top_k=0), C.ERR_UNSUPPORTED), (dict(vocab=1 << 29, ld_logits=1 << 29), C.ERR_UNSUPPORTED),
 ])
@@ -184,3 +184,27 @@ def test_wrappers_refuse_host_tensors_and_bad_shapes():
         ops._dtype(t, "x")
     with pytest.raises(ValueError):
         ops._index_type(x, "index")
+
+
+def test_results_in_place_need_the_same_rows():
+    L = C.lib()
+    d = _layernorm(ld_y=104)
+    assert L.nzb_layernorm_forward(ctypes.byref(d), FAKE, None, None, FAKE, None, None, None) == C.ERR_BAD_ARG
+    far = FAKE + (1 << 20)
+    d = _layernorm(ld_dx=104)
+    for dy, x, dx in ((FAKE, far, FAKE), (far, FAKE, FAKE)):
+        assert L.nzb_layernorm_backward(ctypes.byref(d), dy, x, FAKE, FAKE, None, dx, None, None, None, 0, None) == C.ERR_BAD_ARG
+    d = _logprob(ld_dlogits=304)
+    assert L.nzb_token_logprob_backward(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None) == C.ERR_BAD_ARG
+    d = _ortho(batch=2, stride_out=39)
+    assert L.nzb_orthogonalize(ctypes.byref(d), FAKE, FAKE, FAKE, 1 << 30, None) == C.ERR_BAD_ARG
+    for w, m, g in ((FAKE, FAKE, far), (far, FAKE, FAKE)):
+        assert L.nzb_muon(ctypes.byref(_ortho()), w, m, g, 0.1, 1.0, 0.9, 0.0, 0, FAKE, 1 << 30, None) == C.ERR_BAD_ARG
+
+
+def test_long_rows_need_a_small_workspace():
+    L = C.lib()
+    n = ctypes.c_size_t()
+    dim = 1 << 20
+    d = _layernorm(rows=1000, dim=dim, ld_x=dim, ld_y=dim, ld_dx=dim)
+    assert L.nzb_layernorm_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(n)) == C.OK and n.value == 64 * 2 * dim * 4

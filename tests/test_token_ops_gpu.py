@@ -587,6 +587,23 @@ def test_muon_step(shape, nesterov):
     assert err <= step * ORTHO_TOL * torch.linalg.norm(o) + 4 * U * torch.linalg.norm(w)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logprob_of_a_largest_number(dtype):
+    """A token forced by the type's largest number takes all of the probability; two of them share it."""
+    big = torch.finfo(dtype).max
+    x = rnd((4, 3001), 70, dtype)
+    x[0, 7] = big
+    x[1, 7] = x[1, 2900] = big
+    x[2, :] = -math.inf
+    x[2, 2000] = big
+    t = torch.tensor([7, 2900, 2000, 0], device="cuda")
+    f = nz.token_logprobs(x, t, top_k=2)
+    ln2 = math.log(2.0)
+    within(f.logprob[:3], torch.tensor([0.0, -ln2, 0.0], device="cuda"), 2 * U)
+    within(f.entropy[:3], torch.tensor([0.0, ln2, 0.0], device="cuda"), 2 * U)
+    assert f.top_index[:3, 0].tolist() == [7, 7, 2000] and f.top_index[1, 1] == 2900
+
+
 # ---- all of them together ----------------------------------------------------------------------------------
 def _token_model(p, idx, targets):
     """Rows of a table, layer norm, Linear, log probability of the next token: forward and backward by this library."""
