@@ -60,6 +60,8 @@ struct RowShare {
     __device__ __forceinline__ int first(int k) const { return first0 + k * pitch; }
     __device__ __forceinline__ bool has(int k) const { return some >> k & 1; }
     __device__ __forceinline__ float weight(int k) const { return has(k) ? 1.f : 0.f; }
+    // every block of the warp's lies whole within the row
+    __device__ __forceinline__ bool plain() const { return __all_sync(0xffffffffu, whole == (1u << VPT) - 1); }
     __device__ __forceinline__ float count() const { return __popc(some) * static_cast<float>(VEC) - extra; }
     // Gives the elements outside the row, in this thread's places in shared memory, the value of one inside it (so that
     // they deviate from the mean like any other and can be subtracted from the sums without loss), or zero; returns that
@@ -75,24 +77,30 @@ struct RowShare {
                     if (first(k) + i < 0 || first(k) + i >= dim) reinterpret_cast<T*>(ring + k * nt)[i] = value;
         return Elem<T>::to(value);
     }
-    // Starts the copies of the row that begins at element `at` of a tensor of n to this thread's own places in shared
-    // memory, nt blocks apart; the same thread reads them after they have landed, so no barrier is needed. A block at
-    // the row's end brings elements of its neighbours, or of the gap between two rows, along, which patch() replaces;
-    // only blocks that reach beyond the tensor go element by element (waiting for them cost a memory latency per row).
-    __device__ __forceinline__ void fetch(uint4* ring, int nt, const T* base, int64_t at, int64_t n, bool border) const {
-        uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-        const T* from = base + at + first0;
+    // Starts the copies of the row whose block 0 is `from` to this thread's own places in shared memory, nt blocks apart
+    // (copies to places that are not side by side in a warp take half as long again); the same thread reads them after they have landed, so no barrier is needed. A block at the row's end brings elements of its
+    // neighbours, or of the gap between two rows, along, which patch() replaces; only blocks that reach beyond the tensor
+    // (of n elements from `base`) go element by element (waiting for them cost a memory latency per row).
+    __device__ __forceinline__ void fetch(uint4* ring, int nt, const T* from, bool plain, bool border, const T* base, int64_t n) const {
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+        const auto copy = [&](int k) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * nt * 16), "l"(from + k * pitch) : "memory"); };
+        if (plain) {
 #pragma unroll
-        for (int k = 0; k < VPT; k++, to += nt * 16, from += pitch) {
+            for (int k = 0; k < VPT; k++) copy(k);
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; k++) {
             if (!has(k)) continue;
-            if (border && (at + first(k) < 0 || at + first(k) + VEC > n)) ring[k * nt] = load_block(base, at + first(k), n);
-            else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+            const int64_t at = from - base + k * pitch;
+            if (border && (at < 0 || at + VEC > n)) ring[k * nt] = load_block(base, at, n);
+            else copy(k);
         }
     }
-    // Writes block k of a row that starts on the same offset from 16 bytes.
-    __device__ __forceinline__ void store(T* row, int k, int dim, const float (&f)[VEC]) const {
-        if (whole >> k & 1) *reinterpret_cast<uint4*>(row + first(k)) = Elem<T>::pack(f);
-        else if (has(k)) store_block(row, first(k), dim, Elem<T>::pack(f));
+    // Writes block k of a row that starts on the same offset from 16 bytes; block0: where block 0 lies.
+    __device__ __forceinline__ void store(T* block0, int k, bool plain, int dim, const float (&f)[VEC]) const {
+        if (plain || (whole >> k & 1)) *reinterpret_cast<uint4*>(block0 + k * pitch) = Elem<T>::pack(f);
+        else if (has(k)) store_block(block0 - first0, first(k), dim, Elem<T>::pack(f));
     }
 };
 // Rows at either end of a tensor whose blocks may reach beyond it: more than one when a block holds several rows.
@@ -102,9 +110,9 @@ template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // A group of `nt` threads works on a row; the CTA's groups walk the rows of one residue, so that a thread's columns
-// stay the same: gamma and beta lie in shared memory as the threads read them, four at a time without bank conflicts
-// (read from memory unaligned for every row they cost more than the row: 8191 x 5003 fp16 113 us), and all groups
-// share them. STAGES rows per group are on their way while one is worked on. EXACT: rows start on 16 bytes and fill
+// stay the same: gamma and beta lie in shared memory, all groups', thread by thread as they are read (read from memory
+// unaligned for every row they cost more than the row: 8191 x 5003 fp16 113 us). A thread's are an odd number of 16-byte
+// blocks: no bank conflicts, and addresses that differ by constants. STAGES rows per group are on their way while one is worked on. EXACT: rows start on 16 bytes and fill
 // the group's threads, so nothing is masked.
 // Statistics with one barrier: a warp's mean and its squares about that mean, then the warps' pairs joined,
 // M2 = sum_w (M2_w + n_w (mean_w - mean)^2); no difference of large numbers anywhere.
@@ -118,8 +126,8 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
     __shared__ float2 buf[2][32];  // per warp of the CTA: mean and M2
     const int group = threadIdx.x / nt, t = threadIdx.x - group * nt, lane = threadIdx.x & 31;
     const int warps = nt >> 5, warp0 = group * warps, warp = threadIdx.x >> 5;
-    float4* params = reinterpret_cast<float4*>(smem_norm) + t;                          // [2][Q][nt]
-    uint4* ring = smem_norm + 2 * Q * nt + group * (STAGES * VPT * nt) + t;             // per group [STAGES][VPT][nt]
+    float4* params = reinterpret_cast<float4*>(smem_norm) + t * (2 * Q + 1);             // [nt][gamma, beta][Q], one unused
+    uint4* ring = smem_norm + nt * (2 * Q + 1) + group * (STAGES * VPT * nt) + t;   // per group [STAGES][VPT][nt]
     const int residue = blockIdx.x % period;
     const int lead = EXACT ? 0 : row_lead(x + residue * ld_x);
     const int64_t span = (rows - 1) * ld_x + dim;
@@ -133,8 +141,12 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
         for (int k = 0; k < STAGES * VPT; k++)
             if (!share.has(k % VPT)) ring[k * nt] = make_uint4(0, 0, 0, 0);
     }
+    const bool plain = EXACT || share.plain();
+    const T* next = x + first_row * ld_x + share.first0;  // of the row to fetch next
+    const int64_t step_x = step * ld_x, step_y = step * ld_y;
     const auto fetch = [&](int64_t r, int stage) {
-        if (r < rows) share.fetch(ring + stage * VPT * nt, nt, x, r * ld_x, span, !EXACT && (r < edge || r >= rows - edge));
+        if (r < rows) share.fetch(ring + stage * VPT * nt, nt, next, plain, !EXACT && (r < edge || r >= rows - edge), x, span);
+        next += step_x;
         copies_commit();
     };
 #pragma unroll
@@ -148,8 +160,8 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
             g[i] = in ? (gamma ? gamma[c] : 1.f) : 0.f;
             b[i] = in && beta ? beta[c] : 0.f;
         }
-        params[q * nt] = make_float4(g[0], g[1], g[2], g[3]);
-        params[(Q + q) * nt] = make_float4(b[0], b[1], b[2], b[3]);
+        params[q] = make_float4(g[0], g[1], g[2], g[3]);
+        params[Q + q] = make_float4(b[0], b[1], b[2], b[3]);
     }
     __syncthreads();
     // elements of this warp and, lane by lane, of the group's warps
@@ -162,24 +174,26 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
         __syncthreads();
     }
     int turn = 0, stage = 0;
-    for (int64_t r = first_row; r < rows; r += step, turn ^= 1) {
+    T* yr = y + first_row * ld_y + share.first0;
+    for (int64_t r = first_row; r < rows; r += step, turn ^= 1, yr += step_y) {
         copies_wait<STAGES - 1>();
-        const float extra_value = EXACT ? 0.f : share.patch(ring + stage * VPT * nt, nt, dim, false);
+        uint4* row = ring + stage * VPT * nt;
+        const float extra_value = plain ? 0.f : share.patch(row, nt, dim, false);
         float2 v[VPT][VEC / 2];
         float sum = 0.f, sq = 0.f;
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
             float f[VEC];
-            Elem<T>::unpack(ring[(stage * VPT + k) * nt], f);
+            Elem<T>::unpack(row[k * nt], f);
             float2 part = make_float2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < VEC / 2; i++) {
                 v[k][i] = make_float2(f[2 * i], f[2 * i + 1]);
                 part = add2(part, v[k][i]);
             }
-            sum = EXACT ? sum + (part.x + part.y) : fmaf(share.weight(k), part.x + part.y, sum);
+            sum += part.x + part.y;
         }
-        if (!EXACT) sum = fmaf(-share.extra, extra_value, sum);
+        if (!plain) sum = fmaf(-share.extra, extra_value, sum);
         fetch(r + STAGES * step, stage);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         float mean = warp_sum(sum) * inv_warp;
@@ -192,9 +206,9 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
                 const float2 d = add2(v[k][i], minus);
                 part = fma2(d, d, part);
             }
-            sq = EXACT ? sq + (part.x + part.y) : fmaf(share.weight(k), part.x + part.y, sq);
+            sq = plain ? sq + (part.x + part.y) : fmaf(share.weight(k), part.x + part.y, sq);
         }
-        if (!EXACT) {
+        if (!plain) {
             const float d = extra_value - mean;
             sq = fmaf(-share.extra * d, d, sq);
         }
@@ -212,27 +226,26 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
             if (mean_out) mean_out[r] = mean;
             if (rstd_out) rstd_out[r] = rstd;
         }
-        T* yr = y + r * ld_y;
         const float2 rs = make_float2(rstd, rstd), shift = make_float2(-mean, -mean);
 #pragma unroll
         for (int k = 0; k < VPT; k++) {
-            if (!EXACT && !share.has(k)) continue;
+            if (!plain && !share.has(k)) continue;
             float o[VEC];
 #pragma unroll
             for (int q = 0; q < VEC / 4; q++) {
-                const float4 g = params[(k * (VEC / 4) + q) * nt], b = params[(Q + k * (VEC / 4) + q) * nt];
+                const float4 g = params[k * (VEC / 4) + q], b = params[Q + k * (VEC / 4) + q];
                 // (x - mean) rstd, then gamma and beta
                 const float2 lo = fma2(mul2(add2(v[k][2 * q], shift), rs), make_float2(g.x, g.y), make_float2(b.x, b.y));
                 const float2 hi = fma2(mul2(add2(v[k][2 * q + 1], shift), rs), make_float2(g.z, g.w), make_float2(b.z, b.w));
                 o[4 * q] = lo.x; o[4 * q + 1] = lo.y; o[4 * q + 2] = hi.x; o[4 * q + 3] = hi.y;
             }
             if (EXACT || y_together) {
-                share.store(yr, k, dim, o);
+                share.store(yr, k, plain, dim, o);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
                     const int c = share.first(k) + i;
-                    if (c >= 0 && c < dim) yr[c] = Elem<T>::from(o[i]);
+                    if (c >= 0 && c < dim) yr[c - share.first0] = Elem<T>::from(o[i]);
                 }
             }
         }
@@ -291,8 +304,8 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
     __shared__ float buf[2][2][kNormMaxCluster * 16];  // [turn][sum][warp of the CTA, of the cluster]
     const int group = threadIdx.x / nt, t = threadIdx.x - group * nt, lane = threadIdx.x & 31;
     const int warps = nt >> 5, warp0 = group * warps, warp = threadIdx.x >> 5;
-    float4* params = reinterpret_cast<float4*>(smem_norm) + t;                             // [Q][nt], all groups'
-    uint4* ring = smem_norm + Q * nt + group * (STAGES * 2 * VPT * nt) + t;                // per group [stage][x, dy][VPT][nt]
+    float4* params = reinterpret_cast<float4*>(smem_norm) + t * (Q | 1);                   // [nt][Q], all groups'
+    uint4* ring = smem_norm + (Q | 1) * nt + group * (STAGES * 2 * VPT * nt) + t;          // per group [stage][x, dy][VPT][nt]
     // this CTA's columns, as a matrix of its own
     const int part = CLUSTER ? blockIdx.x % cluster : 0, c0 = part * share_cols;
     const int64_t walker = CLUSTER ? blockIdx.x / cluster : blockIdx.x, walkers = CLUSTER ? gridDim.x / cluster : gridDim.x;
@@ -316,12 +329,18 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
         for (int k = 0; k < STAGES * 2 * VPT; k++)
             if (!share.has(k % VPT)) ring[k * nt] = make_uint4(0, 0, 0, 0);
     }
+    const bool plain = EXACT || share.plain();
+    const T* next_x = x + first_row * ld_x + share.first0;  // of the row to fetch next
+    const T* next_dy = dy + first_row * ld_dy + share.first0;
+    const int64_t step_x = step * ld_x, step_dy = step * ld_dy, step_dx = step * ld_dx;
     const auto fetch = [&](int64_t r, int stage) {
         if (r < rows) {
             const bool border = !EXACT && (r < edge || r >= rows - edge);
-            share.fetch(ring + stage * 2 * VPT * nt, nt, x, r * ld_x, span_x, border);
-            share.fetch(ring + (stage * 2 + 1) * VPT * nt, nt, dy, r * ld_dy, span_dy, border);
+            share.fetch(ring + stage * 2 * VPT * nt, nt, next_x, plain, border, x, span_x);
+            share.fetch(ring + (stage * 2 + 1) * VPT * nt, nt, next_dy, plain, border, dy, span_dy);
         }
+        next_x += step_x;
+        next_dy += step_dy;
         copies_commit();
     };
 #pragma unroll
@@ -338,14 +357,15 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             const int e = q * 4 + i, c = (t + e / VEC * nt) * VEC - lead + e % VEC;
             g[i] = c >= 0 && c < dim ? (gamma ? gamma[c] : 1.f) : 0.f;
         }
-        params[q * nt] = make_float4(g[0], g[1], g[2], g[3]);
+        params[q] = make_float4(g[0], g[1], g[2], g[3]);
     }
     __syncthreads();
     if (CLUSTER) cg::this_cluster().sync();  // everybody runs before anybody writes into another's shared memory
     const float inv = 1.f / row_dim;
     int turn = 0, stage = 0;
     float next_mean = first_row < rows ? mean[first_row] : 0.f, next_rstd = first_row < rows ? rstd[first_row] : 0.f;
-    for (int64_t r = first_row; r < rows; r += step, turn ^= 1) {
+    T* dxr = dx + first_row * ld_dx + share.first0;
+    for (int64_t r = first_row; r < rows; r += step, turn ^= 1, dxr += step_dx) {
         const float2 rs = make_float2(next_rstd, next_rstd), minus = make_float2(-next_mean, -next_mean);
         if (r + step < rows) {
             next_mean = mean[r + step];
@@ -354,7 +374,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
         copies_wait<STAGES - 1>();
         uint4* xs = ring + stage * 2 * VPT * nt;
         uint4* ds = xs + VPT * nt;
-        if (!EXACT) {
+        if (!plain) {
             // outside the row: an x of the row, whose h is finite where the row's are, and a dy of zero, which adds nothing
             share.patch(xs, nt, dim, false);
             share.patch(ds, nt, dim, true);
@@ -368,7 +388,7 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             Elem<T>::unpack(ds[k * nt], fd);
 #pragma unroll
             for (int i = 0; i < VEC / 2; i++) {
-                const float4 ga = params[(k * (VEC / 4) + i / 2) * nt];
+                const float4 ga = params[k * (VEC / 4) + i / 2];
                 const float2 d = make_float2(fd[2 * i], fd[2 * i + 1]);
                 h[k][i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
                 g[k][i] = mul2(d, i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
@@ -403,10 +423,9 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             const float other = __shfl_xor_sync(0xffffffffu, s, 16);
             const float m0 = lane & 16 ? other : s, m1 = lane & 16 ? s : other;
             const float2 m0s = make_float2(m0, m0), m1s = make_float2(m1, m1);
-            T* dxr = dx + r * ld_dx;
 #pragma unroll
             for (int k = 0; k < VPT; k++) {
-                if (!EXACT && !share.has(k)) continue;
+                if (!plain && !share.has(k)) continue;
                 float o[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC / 2; i++) {
@@ -416,11 +435,11 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
                 }
                 if (add_dx) {
                     float old[VEC];
-                    Elem<T>::unpack(load_block(dxr, share.first(k), dim), old);
+                    Elem<T>::unpack(load_block(dxr - share.first0, share.first(k), dim), old);
 #pragma unroll
                     for (int i = 0; i < VEC; i++) o[i] += old[i];
                 }
-                share.store(dxr, k, dim, o);
+                share.store(dxr, k, plain, dim, o);
             }
         }
     }
@@ -564,13 +583,14 @@ template <typename T, bool CLUSTER>
 static int launch_norm_backward(const nzb_layernorm_desc* d, const void* dy, const void* x, const float* mean, const float* rstd,
                                 const float* gamma, void* dx, float* partial, int period, bool exact, int nt, int cluster,
                                 int64_t share_cols, int64_t* parts, cudaStream_t s) {
-    constexpr int ring = kNormStages * 2 * (int)(kNormElems / Elem<T>::VEC) * 16, params = kNormElems * 4;
+    constexpr int ring = kNormStages * 2 * (int)(kNormElems / Elem<T>::VEC) * 16, params = ((kNormElems / 4) | 1) * 16;
     // as many groups as threads, named barriers, shared memory and rows allow (eight rows a group, to be worth its sums)
     int64_t groups = CLUSTER ? 1 : kNormBackwardMaxThreads / nt;
     const int64_t fit = (kNormSmem / nt - params) / ring, spread = (d->rows + 8 * kNormSms - 1) / (8 * kNormSms);
-    if (groups > 15) groups = 15;
+    if (groups > 15 && nt > 32) groups = 15;
     if (groups > fit) groups = fit;
     if (groups > spread) groups = spread;
+    if (groups < 1) return fail(NZB_ERR_UNSUPPORTED, "a group's rows exceed shared memory");
     int64_t walkers = (d->rows + groups - 1) / groups;
     if (walkers > *parts / cluster) walkers = *parts / cluster;
     walkers = walkers / period * period;
@@ -629,16 +649,16 @@ int nzb_layernorm_forward(const nzb_layernorm_desc* d, const void* x, const floa
         const bool y_together = reinterpret_cast<uintptr_t>(x) % 16 == reinterpret_cast<uintptr_t>(y) % 16 && d->ld_x * size % 16 == d->ld_y * size % 16;
         const int elems = nt ? VEC : WIDE, most = nt ? 1024 : norm_max_threads<T, WIDE>();
         if (!nt) nt = norm_threads(d->dim, lead, most, elems);
-        const int params = nt * 2 * elems * 4, row = nt * elems / VEC * 16;
+        const int params = nt * (elems / 2 + 1) * 16, row = nt * elems / VEC * 16;
         const int stages = elems == VEC || params + 2 * row > kNormSmem ? 1 : 2;
         const T* xp = static_cast<const T*>(x);
         T* yp = static_cast<T*>(y);
         if (nt && params + stages * row <= kNormSmem) {
             const bool exact = lead == 0 && d->dim == (int64_t)nt * elems && y_together;
-            // as many groups as threads, named barriers, shared memory and rows allow
+            // as many groups as threads, named barriers (of groups of several warps), shared memory and rows allow
             int64_t groups = most / nt;
             const int64_t fit = (kNormSmem - params) / (stages * row), spread = (d->rows + ds->sm_count - 1) / ds->sm_count;
-            if (groups > 15) groups = 15;
+            if (groups > 15 && nt > 32) groups = 15;
             if (groups > fit) groups = fit;
             if (groups > spread) groups = spread;
             int64_t ctas = (d->rows + groups - 1) / groups;
@@ -706,12 +726,13 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
                           (!dx || (offset(x) == offset(dx) && d->ld_x * size % 16 == d->ld_dx * size % 16));
     const int period = d->ld_x * size % 16 == 0 ? 1 : (int)(16 / size);
     const int lead = period == 1 && aligned_to(x, 16) ? 0 : (int)(16 / size) - 1;
-    // CTAs to a row, and the columns of each: whole blocks of 16 bytes
+    // CTAs to a row, and the columns of each: whole blocks of 16 bytes. Shared memory holds the rows of 480 threads in fp32
+    const int most = size == 4 ? kNormBackwardMaxThreads - 32 : kNormBackwardMaxThreads;
     int cluster = 1, nt = 0;
     int64_t share_cols = d->dim;
     for (; together && cluster <= kNormMaxCluster; cluster *= 2) {
         share_cols = cluster == 1 ? d->dim : round_up((d->dim + cluster - 1) / cluster, 16 / size);
-        if ((nt = norm_threads(share_cols, lead, kNormBackwardMaxThreads, kNormElems)) != 0) break;
+        if ((nt = norm_threads(share_cols, lead, most, kNormElems)) != 0) break;
     }
     if (nt) {
         const bool exact = period == 1 && lead == 0 && share_cols == (int64_t)nt * kNormElems && share_cols * cluster == d->dim;
