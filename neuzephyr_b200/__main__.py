@@ -3,10 +3,13 @@
     python -m neuzephyr_b200 info
     python -m neuzephyr_b200 gemm M N K [--staged] [--iters 10] [--warmup 3]
     python -m neuzephyr_b200 conv N C H W Cout K pad [--backward] [--no-bias] [--counters] [--iters 5] [--warmup 2]
+    python -m neuzephyr_b200 tokens TOKENS VOCAB DIM [--dtype bf16] [--iters 5] [--warmup 2]
 
 `gemm` times nzb_gemm (fp32 in / out, uniform[-1,1]); with --staged the GEMM kernel alone on operands
 that are already fp16 (nzb_gemm_f16). `conv` times nzb_conv2d_forward (+ untied bias matrix + ReLU) or,
 with --backward, nzb_conv2d_backward_data, on N(0,1) tensors with Kaiming-normal weights, stride 1.
+`tokens` times the operators of a token model one by one: rows of a table, layer norm, log probabilities of
+the next token with entropy (each forward and backward) on --dtype, and a Muon step on a DIM x DIM weight.
 Times are CUDA-event averages over --iters calls after --warmup calls. Needs a B200.
 
 --counters prints, after the timed calls, the clock64() counters of the channels-last convolution kernel:
@@ -36,6 +39,35 @@ def _time(fn, iters, warmup):
     return e0.elapsed_time(e1) / max(iters, 1)
 
 
+def _tokens(args, gen):
+    n, vocab, dim = args.shape
+    dtype = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[args.dtype]
+    rand = lambda *shape: torch.randn(shape, device="cuda", generator=gen)
+    table, dtable = rand(vocab, dim), torch.empty((vocab, dim), device="cuda")
+    tokens = torch.randint(0, vocab, (n,), device="cuda", generator=gen)
+    gamma, beta = torch.ones(dim, device="cuda"), torch.zeros(dim, device="cuda")
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+    x = nz.embedding(table, tokens, out_dtype=dtype)
+    y, mean, rstd = nz.layernorm_forward(x, gamma, beta)
+    dy, dx = rand(n, dim).to(dtype), torch.empty_like(x)
+    logits = rand(n, vocab).to(dtype)
+    f = nz.token_logprobs(logits, tokens)
+    dlogits, dl, dh = torch.empty_like(logits), torch.full((n,), -1.0 / n, device="cuda"), torch.full((n,), 1e-3 / n, device="cuda")
+    w, momentum, grad = rand(dim, dim), torch.zeros((dim, dim), device="cuda"), rand(dim, dim)
+    run = {
+        "embedding": lambda: nz.embedding(table, tokens, out_dtype=dtype),
+        "embedding_backward": lambda: nz.embedding_backward(dy, tokens, dtable, overwrite=True),
+        "layernorm": lambda: nz.layernorm_forward(x, gamma, beta),
+        "layernorm_backward": lambda: nz.layernorm_backward(dy, x, mean, rstd, gamma, dx, dgamma, dbeta, overwrite_dx=True,
+                                                            overwrite_dparams=True),
+        "token_logprobs": lambda: nz.token_logprobs(logits, tokens),
+        "token_logprobs_backward": lambda: nz.token_logprobs_backward(logits, tokens, f.lse, f.entropy, dl, dh, out=dlogits),
+        "muon_step": lambda: nz.muon_step(w, momentum, grad, lr=1e-3),
+    }
+    ms = {name: _time(fn, args.iters, args.warmup) for name, fn in run.items()}
+    return {"op": "tokens", "tokens": n, "vocab": vocab, "dim": dim, "dtype": args.dtype, "ms": ms, "status": nz.device_status()}
+
+
 def main():
     ap = argparse.ArgumentParser(prog="python -m neuzephyr_b200", description=__doc__,
                                  formatter_class=argparse.RawDescriptionHelpFormatter)
@@ -53,6 +85,11 @@ def main():
     c.add_argument("--counters", action="store_true")
     c.add_argument("--iters", type=int, default=5)
     c.add_argument("--warmup", type=int, default=2)
+    t = sub.add_parser("tokens")
+    t.add_argument("shape", type=int, nargs=3, metavar=("TOKENS", "VOCAB", "DIM"))
+    t.add_argument("--dtype", choices=("f32", "f16", "bf16"), default="bf16")
+    t.add_argument("--iters", type=int, default=5)
+    t.add_argument("--warmup", type=int, default=2)
     args = ap.parse_args()
     if args.cmd == "info":
         print(json.dumps({"abi_version": _capi.lib().nzb_version(), "library": _capi.LIB_PATH,
@@ -72,6 +109,9 @@ def main():
             ms = _time(lambda: nz.gemm(A, B, out=C), args.iters, args.warmup)
         print(json.dumps({"op": "gemm", "M": M, "N": N, "K": K, "staged": args.staged, "ms": ms,
                           "tflops": 2.0 * M * N * K / ms / 1e9, "status": nz.device_status()}), flush=True)
+        return
+    if args.cmd == "tokens":
+        print(json.dumps(_tokens(args, gen)), flush=True)
         return
     N, C, H, W, Co, k, p = args.dims
     x = torch.randn((N, C, H, W), device="cuda", generator=gen)

@@ -2,6 +2,7 @@
 operation, finfo.eps / 2 for the rounding to the stored type, and the length of the longest chain of additions."""
 import ctypes
 import math
+import os
 
 import pytest
 import torch
@@ -726,3 +727,15 @@ def test_far_offsets():
     assert torch.equal(y[-3:], nz.layernorm_forward(view[-3:])[0])
     nz.layernorm_forward(view, out=view)
     assert torch.equal(view[-3:], y[-3:])
+
+
+def test_command_line_runs_every_operator():
+    import json
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-m", "neuzephyr_b200", "tokens", "100", "500", "96", "--dtype", "f16"],
+                       capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr[-2000:]
+    line = json.loads(r.stdout.splitlines()[-1])
+    assert line["status"] == 0 and len(line["ms"]) == 7 and all(ms > 0 for ms in line["ms"].values())
