@@ -138,9 +138,9 @@ __device__ __forceinline__ void kernel_wait_previous() { asm volatile("griddepco
 __device__ __forceinline__ void kernel_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Launches such a kernel.
 template <typename... Params, typename... Args>
-inline cudaError_t launch_programmatic(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, Args... args) {
+inline cudaError_t launch_programmatic(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
