@@ -491,7 +491,7 @@ enum { NZB_I32 = 0, NZB_I64 = 1 };
  *   dtype        of y and dy
  *   table_dtype  of the table: dtype, or NZB_F32
  * Backward: dtable[v] += scale * sum over t with index[t] == v of dy[t], in fp32 and in the order of t
- * (sorted by token in chunks of 32, then the chunks), with overwrite != 0: dtable = ... and rows of tokens that
+ * (sorted by token in chunks of 8 to 32, then the chunks), with overwrite != 0: dtable = ... and rows of tokens that
  * do not occur are set to zero. Without it those rows are neither read nor written. Tokens equal to
  * padding_index, or outside [0, vocab), contribute nothing (padding_index -1: none). ld_table is then the
  * stride of dtable, whose type is fp32 always.

@@ -7,9 +7,10 @@
 //   2. one CTA per tile of 16384 tokens sorts the tile in shared memory (radix, up to 9 bits a pass; the items
 //      wait in registers between passes, so one copy of the keys is enough), while the other SMs clear the
 //      rows of the tokens that do not occur: most of the bytes, and nothing they need from the sort;
-//   3. the sorted tokens are cut into chunks of 32, whatever runs of equal tokens they hold: one warp per chunk and
-//      32 vectors of columns. A run inside a chunk goes straight to the table, what crosses a chunk's border
-//      to the workspace, so a token that makes up a tenth of the text costs no more than any other;
+//   3. the sorted tokens are cut into chunks of 32 (8 or 16 when they are few), whatever runs of equal tokens they
+//      hold: one warp per chunk and 32 vectors of columns. A run inside a chunk goes straight to the table, what
+//      crosses a chunk's border to the workspace, so a token that makes up a tenth of the text costs no more than
+//      any other;
 //   4. the parts of the runs that cross are added in order.
 // Tiles after the first add to the rows the earlier ones wrote, in launch order: the same bits every time.
 #include "nzb_internal.h"
@@ -21,10 +22,12 @@ constexpr int kSortTile = 16384;
 constexpr int kSortThreads = 1024;
 constexpr int kSortItems = kSortTile / kSortThreads;
 constexpr int kSortMaxBins = 512;
-constexpr int kChunk = 32;                                  // sorted tokens per warp of the sums
 // The rows of the other tokens are cleared beside the sums, not beside the sort, when the sort is short or the table
 // small: two launches less (1000 tokens into 30000 x 512: 25 us instead of 45).
 constexpr int64_t kFewTokens = 2048, kSmallTable = 8 << 20;  // elements
+// Sorted tokens per warp of the sums: few tokens leave SMs idle, and shorter chunks are done sooner, until the joins of long
+// runs outweigh that (64 tokens into 14651 x 185: 23.8 us by 32, 16.3 by 16, 15.1 by 8; 1500 into 14652 x 184: 20.5, 17.1, 17.8).
+inline int chunk_of(const nzb_embedding_desc* d) { return d->tokens <= 256 ? 8 : d->tokens <= kFewTokens ? 16 : 32; }
 inline bool clear_beside_sums(const nzb_embedding_desc* d) { return d->tokens <= kFewTokens || d->vocab * d->dim <= kSmallTable; }
 constexpr int kEmbeddingFly = 4;                            // blocks in flight per thread, forward
 
@@ -212,7 +215,7 @@ template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2)
 embedding_sum_kernel(const T* __restrict__ dy, const SortTile* tile, float* __restrict__ dtable,
                      float* __restrict__ partial, int64_t vocab, int64_t dim, int64_t ld_table, int64_t ld_y, float scale, int add,
-                     int vec_out, unsigned sum_ctas) {
+                     int vec_out, unsigned sum_ctas, int chunk_len) {
     constexpr int VEC = Elem<T>::VEC, FLY = 8;  // FLY: rows of dy in flight
     const int lane = threadIdx.x & 31;
     kernel_wait_previous();
@@ -236,9 +239,9 @@ embedding_sum_kernel(const T* __restrict__ dy, const SortTile* tile, float* __re
     const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     const int64_t blocks = (dim + 32 * VEC - 1) / (32 * VEC);  // column blocks of a row
     const int64_t chunk = item / blocks, c0 = (item - chunk * blocks) * 32 * VEC;
-    const int count = tile->count, i0 = static_cast<int>(chunk) * kChunk;
+    const int count = tile->count, i0 = static_cast<int>(chunk) * chunk_len;
     if (i0 >= count) return;
-    const int i1 = min(i0 + kChunk, count);
+    const int i1 = min(i0 + chunk_len, count);
     const uint32_t none = 0xffffffffu;
     const uint32_t my_key = i0 + lane < i1 ? tile->key[i0 + lane] : none;
     const int32_t my_row = i0 + lane < i1 ? tile->order[i0 + lane] : 0;
@@ -305,21 +308,21 @@ embedding_sum_kernel(const T* __restrict__ dy, const SortTile* tile, float* __re
 // Runs over more than one chunk: the warp of the chunk such a run starts in adds its parts, 32 columns x 4.
 __global__ void __launch_bounds__(256)
 embedding_join_kernel(const SortTile* tile, const float* partial, float* __restrict__ dtable,
-                      int64_t dim, int64_t ld_table, float scale, int add) {
+                      int64_t dim, int64_t ld_table, float scale, int add, int chunk_len) {
     kernel_wait_previous();
     kernel_allow_next();
     const int lane = threadIdx.x & 31;
     const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     const int64_t blocks = (dim + 127) / 128;
     const int64_t chunk = item / blocks;
-    const int count = tile->count, i0 = static_cast<int>(chunk) * kChunk, i1 = i0 + kChunk;
+    const int count = tile->count, i0 = static_cast<int>(chunk) * chunk_len, i1 = i0 + chunk_len;
     if (i1 >= count) return;
     const uint32_t key = tile->key[i1 - 1];
     if (tile->key[i1] != key || (i0 > 0 && tile->key[i0 - 1] == key)) return;
     // parts in the chunks behind: one, and one more for every border the run crosses
     int parts = 1;
-    for (int i = i1 + kChunk;; i += 32 * kChunk) {
-        const int at = i + lane * kChunk;
+    for (int i = i1 + chunk_len;; i += 32 * chunk_len) {
+        const int at = i + lane * chunk_len;
         const uint32_t ends = __ballot_sync(0xffffffffu, at >= count || tile->key[at] != key);
         parts += ends ? __ffs(ends) - 1 : 32;
         if (ends) break;
@@ -430,7 +433,7 @@ static EmbeddingPlan plan_embedding(const nzb_embedding_desc* d) {
     pl.tiles_bytes = (size_t)round_up(pl.tiles * (int64_t)sizeof(SortTile), 256);
     pl.present_bytes = (size_t)round_up((d->vocab + 31) / 32 * 4, 256);
     const int64_t most = d->tokens < kSortTile ? d->tokens : kSortTile;
-    pl.partial_bytes = (size_t)round_up((most + kChunk - 1) / kChunk * 2 * d->dim * 4, 256);  // two borders a chunk
+    pl.partial_bytes = (size_t)round_up((most + chunk_of(d) - 1) / chunk_of(d) * 2 * d->dim * 4, 256);  // two borders a chunk
     return pl;
 }
 
@@ -542,10 +545,11 @@ int nzb_embedding_backward(const nzb_embedding_desc* d, const void* dy, const vo
                                   : launch_sort<int32_t>(d, index, pl, tiles, present, dtable, ds->sm_count, s);
     if (rc != NZB_OK) return rc;
     const int vec_out = aligned_to(dtable, 16) && d->ld_table % 4 == 0;
+    const int chunk = chunk_of(d);
     for (int64_t t = 0; t < pl.tiles; t++) {
         const int add = t > 0 || !d->overwrite;
         const int64_t n = d->tokens - t * kSortTile < kSortTile ? d->tokens - t * kSortTile : kSortTile;
-        const int64_t chunks = (n + kChunk - 1) / kChunk;
+        const int64_t chunks = (n + chunk - 1) / chunk;
         const bool clear = t == 0 && d->overwrite && clear_beside_sums(d);
         NZB_DISPATCH_DTYPE(d->dtype, T, {
             const T* from = static_cast<const T*>(dy) + t * kSortTile * d->ld_y;
@@ -557,11 +561,11 @@ int nzb_embedding_backward(const nzb_embedding_desc* d, const void* dy, const vo
             const auto kernel = rows_aligned ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
             if (sum_ctas + clear_ctas)
                 NZB_CUDA_TRY(launch_programmatic(kernel, sum_ctas + (unsigned)clear_ctas, 256, 0, s, from, tiles + t, dtable, partial, d->vocab, d->dim,
-                                                 d->ld_table, d->ld_y, d->scale, add, vec_out, sum_ctas));
+                                                 d->ld_table, d->ld_y, d->scale, add, vec_out, sum_ctas, chunk));
         });
         if (chunks > 1)
             NZB_CUDA_TRY(launch_programmatic(embedding_join_kernel, (unsigned)((chunks * ((d->dim + 127) / 128) + 7) / 8), 256, 0, s, tiles + t, partial,
-                                             dtable, d->dim, d->ld_table, d->scale, add));
+                                             dtable, d->dim, d->ld_table, d->scale, add, chunk));
     }
     return NZB_OK;
 }
