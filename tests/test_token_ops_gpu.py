@@ -739,3 +739,42 @@ def test_command_line_runs_every_operator():
     assert r.returncode == 0, r.stderr[-2000:]
     line = json.loads(r.stdout.splitlines()[-1])
     assert line["status"] == 0 and len(line["ms"]) == 7 and all(ms > 0 for ms in line["ms"].values())
+
+
+def test_captured_behind_copies_and_other_streams():
+    """The first kernel of a call is launched programmatically: in a graph it may follow a copy, a memset or another
+    stream's work instead of a kernel."""
+    src, other = rnd((96, 160), 90), rnd((96, 160), 91)
+    g, cleared = torch.empty_like(src), torch.ones(4096, device="cuda")
+    idx = torch.arange(50, device="cuda")
+    dtable, dy = torch.empty((60, 32), device="cuda"), rnd((50, 32), 92)
+    side = torch.cuda.Stream()
+
+    def run():
+        g.copy_(src)  # a copy right before
+        a = nz.orthogonalize(g)
+        cleared.zero_()  # a memset
+        b = nz.orthogonalize(g)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            g.copy_(other)
+        torch.cuda.current_stream().wait_stream(side)  # two streams join
+        c = nz.orthogonalize(g)
+        cleared.zero_()
+        nz.embedding_backward(dy, idx, dtable, overwrite=True)
+        return a, b, c
+
+    want = [nz.orthogonalize(t) for t in (src, src, other)]
+    assert all(torch.equal(x, y) for x, y in zip(run(), want))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        for x in got:
+            x.zero_()
+        dtable.fill_(-1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert torch.equal(dtable[:50], dy) and not dtable[50:].any()
