@@ -15,11 +15,22 @@ namespace nz::nodes {
 
 using data::Tensor;
 
+// What a parameter is to an optimizer that treats matrices apart (opt::Muon). The layers that know it say so: the Model
+// builders where they make a parameter, the fused nodes of a parameter that nobody has named. Unknown: its shape decides.
+enum class ParameterRole : unsigned {
+    Unknown = 0,
+    OutByIn = 1,   // a weight {.., outputs, inputs}: Linear
+    InByOut = 2,   // a weight {.., inputs, outputs}: Conv2d
+    NoMatrix = 3,  // a bias, a norm's gamma or beta, whatever its shape
+};
+
 class Node {
 public:
     std::vector<Node*> inputs;
     std::shared_ptr<Tensor> output;
     std::string type;
+    ParameterRole role = ParameterRole::Unknown;
+    void nameRole(ParameterRole r) { if (role == ParameterRole::Unknown) role = r; }
     virtual ~Node() = default;
     virtual void forward() = 0;
     virtual void backward() = 0;
@@ -41,6 +52,10 @@ public:
     explicit InputNode(const Tensor& tensor);
     void forward() override {}
     void backward() override {}
+    // the role of a parameter that has one, so that a saved graph keeps it
+    std::vector<size_t> attributes() const override {
+        return role == ParameterRole::Unknown ? std::vector<size_t>{} : std::vector<size_t>{(size_t)role};
+    }
 };
 
 // Base of loss nodes: accumulates a scalar loss on the device (the reference's loss nodes do

@@ -83,9 +83,10 @@ private:
 };
 
 // Muon (no counterpart in the reference): momentum, then the update with its singular values brought near 1 by five
-// Newton-Schulz products (nzb_muon); w = (1 - lr * weight_decay) * w - lr * sqrt(max(1, H / W)) * update. It takes parameters
-// whose H and W are above 1, as N*C matrices; the others (biases, norms) go to `others`, which the caller owns and which
-// keeps its own learning rate, counter and state.
+// Newton-Schulz products (nzb_muon); w = (1 - lr * weight_decay) * w - lr * sqrt(max(1, outputs / inputs)) * update. It takes
+// weights whose H and W are above 1, as N*C matrices: what Linear (outputs by inputs) and Conv2d (inputs by outputs) name
+// as such, and what has no role, read as outputs by inputs. Biases (a convolution's {1, 1, Ho*Wo, Cout} too), norms and
+// vectors go to `others`, which the caller owns and which keeps its own learning rate, counter and state.
 class Muon : public Optimizer {
 public:
     Muon(float learning_rate, float momentum, Optimizer* others = nullptr, float weight_decay = 0.f, bool nesterov = true);

@@ -267,7 +267,14 @@ void ComputeGraph::load(const std::string& path, opt::Optimizer* optimizer) {
         } else throw std::runtime_error("node " + r.name + " has no usable shape");
         Node* n = nullptr;
         io::OutputNode* out = nullptr;
-        if (r.type == "Input") n = new io::InputNode(shape, r.requires_grad);
+        if (r.type == "Input") {
+            n = new io::InputNode(shape, r.requires_grad);
+            if (!r.attr.empty()) {
+                if (r.attr[0] < 0 || r.attr[0] > (long)nodes::ParameterRole::NoMatrix)
+                    throw std::runtime_error("node " + r.name + " has an unknown role");
+                n->role = (nodes::ParameterRole)r.attr[0];
+            }
+        }
         else if (r.type == "Output") n = out = new io::OutputNode(in_node(0));
         else if (r.type == "Add") n = new calc::AddNode(in_node(0), in_node(1));
         else if (r.type == "MatMul") n = new calc::MatMulNode(in_node(0), in_node(1));
@@ -413,6 +420,7 @@ Muon::Muon(float lr, float mu, Optimizer* others, float weight_decay, bool neste
     learning_rate = lr;
 }
 bool Muon::isMatrix(nodes::Node* node) {
+    if (node->role == nodes::ParameterRole::NoMatrix) return false;
     const auto s = node->output->shape();
     return s.H() > 1 && s.W() > 1;
 }
@@ -440,7 +448,9 @@ void Muon::step(nodes::Node* input) {
     d.coef[0] = 3.4445f; d.coef[1] = -4.7750f; d.coef[2] = 2.0315f;
     d.eps = 1e-7f;
     d.steps = 5;
-    const float scale = s.H() > s.W() ? std::sqrt((float)s.H() / (float)s.W()) : 1.f;
+    const bool turned = input->role == nodes::ParameterRole::InByOut;
+    const float out = (float)(turned ? s.W() : s.H()), in = (float)(turned ? s.H() : s.W());
+    const float scale = out > in ? std::sqrt(out / in) : 1.f;
     size_t bytes = 0;
     NZB_CHECK(nzb_muon_workspace_bytes(&d, &bytes));
     SM::Instance().run({t.data(), m->data()}, {t.grad()}, [&](cudaStream_t st) {
@@ -593,6 +603,7 @@ Model::Node* Model::Bias(Node* input) {
     const auto s = input->output->shape();
     auto* param = new io::InputNode(Dimension(1, s[1], s[2], s[3]), true);
     param->output->randomize();
+    param->role = nodes::ParameterRole::NoMatrix;
     own(param, true);
     return Add(input, param);
 }
@@ -619,6 +630,7 @@ Model::Node* Model::Linear(Node* input, size_t outSize) {
     Node* shaped = s[2] != inSize ? Reshape(input, Dimension(s[0], 1, inSize, 1)) : input;
     auto* w = new io::InputNode(Dimension(1, 1, outSize, inSize), true);
     w->output->randomize();
+    w->role = nodes::ParameterRole::OutByIn;
     own(w, true);
     return Bias(Mul(w, shaped));
 }
@@ -668,6 +680,7 @@ Model::Node* Model::Conv2d(Node* input, size_t outChannels, size_t kh, size_t kw
     const size_t ho = (s.H() + 2 * pad - kh) / stride + 1, wo = (s.W() + 2 * pad - kw) / stride + 1;
     auto* w = new io::InputNode(Dimension(perSampleWeights ? s.N() : 1, 1, s.C() * kh * kw, outChannels), true);
     w->output->randomize();
+    w->role = nodes::ParameterRole::InByOut;
     own(w, true);
     if (fused_) {
         // The fused node stands for Img2Col, MatMul, [Add], Col2Img, [ReLU] (src/Model.cu:244-263):

@@ -292,7 +292,11 @@ Conv2dNode::Conv2dNode(Node* x, Node* weight, Node* bias, Tensor::size_type kh, 
             throw std::invalid_argument("Conv2dNode: bias must be {1, 1, Ho*Wo, Cout}");
     }
     inputs = {x, weight};
-    if (bias) inputs.push_back(bias);
+    weight->nameRole(ParameterRole::InByOut);
+    if (bias) {
+        inputs.push_back(bias);
+        bias->nameRole(ParameterRole::NoMatrix);
+    }
     output = std::make_shared<Tensor>(Dimension(sx.N(), sw.W(), ho, wo), true);
     type = "Conv2d";
 }
@@ -409,7 +413,11 @@ LinearNode::LinearNode(Node* x, Node* weight, Node* bias, bool relu) : relu_(rel
         if (sb.size() != sw.H()) throw std::invalid_argument("LinearNode: bias must hold one value per output");
     }
     inputs = {x, weight};
-    if (bias) inputs.push_back(bias);
+    weight->nameRole(ParameterRole::OutByIn);
+    if (bias) {
+        inputs.push_back(bias);
+        bias->nameRole(ParameterRole::NoMatrix);
+    }
     output = std::make_shared<Tensor>(Dimension(sx.N(), 1, sw.H(), 1), true);
     type = "Linear";
 }
@@ -456,6 +464,8 @@ LayerNormNode::LayerNormNode(Node* x, Node* gamma, Node* beta, float eps) : eps_
         throw std::invalid_argument("LayerNormNode: gamma and beta must hold one value per element of a sample");
     if (!(eps >= 0.f)) throw std::invalid_argument("LayerNormNode: eps must not be negative");
     inputs = {x, gamma, beta};
+    gamma->nameRole(ParameterRole::NoMatrix);
+    beta->nameRole(ParameterRole::NoMatrix);
     output = std::make_shared<Tensor>(sx, true);
     mean_ = std::make_unique<Tensor>(Dimension(sx.N(), 1, 1, 1));
     rstd_ = std::make_unique<Tensor>(Dimension(sx.N(), 1, 1, 1));
