@@ -22,12 +22,18 @@ public:
     // between and run them as one launch in endBatch() (Adam does). The default runs each step at once.
     virtual void beginBatch() {}
     virtual void endBatch() {}
+    // A step between the two threw: the steps collected so far (and their counts) are forgotten, and the next one runs at once.
+    virtual void dropBatch() {}
+    // Throws if step(node) would be refused; `sliced`: with a slice of the node. Touches nothing. Model::update and
+    // ComputeGraph::update ask for every node before they exchange a gradient or take a step.
+    virtual void checkStep(nodes::Node* node, bool sliced) const { (void)node; (void)sliced; }
     // Restricts the steps of `node` to elements [offset, offset + count) of its tensor (count == 0: the
     // whole tensor again). A data-parallel run with a sharded optimizer gives every rank its own slice.
     void setSlice(nodes::Node* node, size_t offset, size_t count) {
         if (count) slices_[node] = {offset, count};
         else slices_.erase(node);
     }
+    bool hasSlice(nodes::Node* node) const { return slices_.count(node) != 0; }
 
 protected:
     std::pair<size_t, size_t> sliceOf(nodes::Node* node) const {
@@ -63,6 +69,7 @@ public:
     void skip(int n) override { it_ += n; }
     void beginBatch() override;
     void endBatch() override;  // one nzb_adam_multi launch over every tensor stepped since beginBatch()
+    void dropBatch() override;
     const char* name() const override { return "Adam"; }
     long counter() const override { return it_; }
     void setCounter(long it) override { it_ = (int)it; }
@@ -76,7 +83,7 @@ public:
 
 private:
     float beta1_, beta2_, epsilon_ = 1e-6f;
-    int it_ = 0, it_shared_ = 0;
+    int it_ = 0, it_shared_ = 0, it_before_batch_ = 0;
     bool batching_ = false;
     std::vector<std::pair<nodes::Node*, int>> batch_;  // (node, time step) collected between begin / endBatch
     std::unordered_map<nodes::Node*, std::unique_ptr<data::Tensor>> m_, v_;
@@ -94,6 +101,8 @@ public:
     void skip(int n) override { if (others_) others_->skip(n); }
     void beginBatch() override { if (others_) others_->beginBatch(); }
     void endBatch() override { if (others_) others_->endBatch(); }
+    void dropBatch() override { if (others_) others_->dropBatch(); }
+    void checkStep(nodes::Node* node, bool sliced) const override;
     const char* name() const override { return "Muon"; }
     long counter() const override { return others_ ? others_->counter() : 0; }
     void setCounter(long it) override { if (others_) others_->setCounter(it); }

@@ -94,14 +94,21 @@ void ComputeGraph::zeroGrad() const {
     for (Node* n : nodes_) n->output->zeroGrad();
 }
 void ComputeGraph::update(opt::Optimizer* optimizer, const std::function<void()>& before_step) const {
+    const auto steps = [&](Node* n) { return n->output->requiresGrad() && (step_intermediates_ || n->inputs.empty()); };
+    for (Node* n : nodes_)
+        if (steps(n)) optimizer->checkStep(n, optimizer->hasSlice(n));
     if (before_step) before_step();
     optimizer->beginBatch();
-    for (size_t i = 0; i < nodes_.size(); i++) {
-        Node* n = nodes_[i];
-        if (ticks_before_[i]) optimizer->skip(ticks_before_[i]);
-        if (!n->output->requiresGrad()) continue;
-        if (step_intermediates_ || n->inputs.empty()) optimizer->step(n);
-        else optimizer->skip(1);  // the reference steps this activation (src/ComputeGraph.cu:541-547)
+    try {
+        for (size_t i = 0; i < nodes_.size(); i++) {
+            Node* n = nodes_[i];
+            if (ticks_before_[i]) optimizer->skip(ticks_before_[i]);
+            if (steps(n)) optimizer->step(n);
+            else if (n->output->requiresGrad()) optimizer->skip(1);  // the reference steps this activation (src/ComputeGraph.cu:541-547)
+        }
+    } catch (...) {
+        optimizer->dropBatch();
+        throw;
     }
     if (pending_ticks_) optimizer->skip(pending_ticks_);
     optimizer->endBatch();
@@ -383,6 +390,12 @@ void Adam::step(nodes::Node* input) {
 void Adam::beginBatch() {
     batching_ = true;
     batch_.clear();
+    it_before_batch_ = it_;
+}
+void Adam::dropBatch() {
+    if (batching_) it_ = it_before_batch_;
+    batching_ = false;
+    batch_.clear();
 }
 void Adam::endBatch() {
     batching_ = false;
@@ -424,16 +437,23 @@ bool Muon::isMatrix(nodes::Node* node) {
     const auto s = node->output->shape();
     return s.H() > 1 && s.W() > 1;
 }
+void Muon::checkStep(nodes::Node* node, bool sliced) const {
+    if (isMatrix(node)) {
+        if (sliced) throw std::runtime_error("Muon needs whole matrices: it cannot take a sharded optimizer's slice");
+        return;
+    }
+    if (!others_) throw std::invalid_argument("Muon updates matrices only: give it another optimizer for the other parameters");
+    others_->checkStep(node, sliced);
+}
 void Muon::step(nodes::Node* input) {
     const auto slice = slices_.find(input);
+    checkStep(input, slice != slices_.end());
     if (!isMatrix(input)) {
-        if (!others_) throw std::invalid_argument("Muon updates matrices only: give it another optimizer for the other parameters");
         if (slice != slices_.end()) others_->setSlice(input, slice->second.first, slice->second.second);
         else others_->setSlice(input, 0, 0);
         others_->step(input);
         return;
     }
-    if (slice != slices_.end()) throw std::runtime_error("Muon needs whole matrices: it cannot take a sharded optimizer's slice");
     data::Tensor& t = *input->output;
     auto& m = momentum_[input];
     if (!m) {
@@ -572,6 +592,7 @@ void Model::gatherGradients() {
 }
 void Model::update(opt::Optimizer* optimizer) {
     const bool dp = comm_ && comm_->world() > 1;
+    for (size_t i = 0; i < params_.size(); i++) optimizer->checkStep(params_[i], dp && sharded(i));
     for (size_t i = 0; i < params_.size(); i++) {
         const size_t n = params_[i]->output->size();
         if (dp && sharded(i)) optimizer->setSlice(params_[i], (size_t)comm_->rank() * (n / comm_->world()), n / comm_->world());

@@ -223,9 +223,53 @@ static void test_saved_graph() {
     remove(path);
 }
 
+// A graph's update that is refused leaves everything as it was; one that breaks off does not leave the other optimizer in
+// the middle of a batch, where its next step would wait for an end that never comes.
+static void test_refused_updates() {
+    for (int kind = 0; kind < 3; kind++) {
+        // 0: a slice of a matrix, 1: nobody for the vector, 2: more matrices than the operator takes (found in the step itself)
+        InputNode w({1, kind == 2 ? 70000u : 1u, 2, 3}, true), bias({1, 1, 40, 1}, true), fresh({1, 1, 40, 1}, true);
+        const auto v = normal(40, 50), g = normal(40, 51);
+        for (InputNode* n : {&bias, &fresh}) {
+            n->output->dataInject(v.begin(), v.end());
+            n->output->dataInject(g.begin(), g.end(), true);
+        }
+        w.output->fill(0.5f);
+        w.output->zeroGrad();
+        opt::Adam adam(0.01f, 0.9f, 0.999f), alone(0.01f, 0.9f, 0.999f);
+        opt::Muon muon(0.02f, 0.95f, kind == 1 ? nullptr : &adam);
+        if (kind == 0) muon.setSlice(&w, 0, 3);
+        graph::ComputeGraph graph;
+        graph.addInput(&bias);
+        graph.addInput(&w);
+        bool threw = false, exchanged = false;
+        try {
+            graph.update(&muon, [&] { exchanged = true; });
+        } catch (const std::exception&) {
+            threw = true;
+        }
+        EXPECT_TRUE(threw && exchanged == (kind == 2));
+        EXPECT_TRUE(bias.output->hostData() == v && w.output->hostData() == std::vector<float>(w.output->size(), 0.5f));
+        EXPECT_TRUE(adam.counter() == 0);
+        // the other optimizer's own steps run at once
+        adam.step(&fresh);
+        const auto got = fresh.output->hostData();
+        fresh.output->dataInject(v.begin(), v.end());
+        alone.step(&fresh);
+        EXPECT_TRUE(got != v && got == fresh.output->hostData());
+        // and so does the graph's update once its cause is gone
+        if (kind == 0) {
+            muon.setSlice(&w, 0, 0);
+            graph.update(&muon);
+            EXPECT_TRUE(bias.output->hostData() != v);
+        }
+    }
+}
+
 int main() {
     const struct { const char* name; void (*fn)(); } tests[] = {
         {"convolutions", test_convolutions}, {"nodes_of_ones_own", test_nodes_of_ones_own}, {"saved_graph", test_saved_graph},
+        {"refused_updates", test_refused_updates},
     };
     for (auto& t : tests) {
         g_current = t.name;
