@@ -77,6 +77,17 @@ struct RowShare {
                     if (first(k) + i < 0 || first(k) + i >= dim) reinterpret_cast<T*>(ring + k * nt)[i] = value;
         return Elem<T>::to(value);
     }
+    // Sum of f over the thread's elements of a row in memory.
+    template <class F>
+    __device__ __forceinline__ float sum(const T* row, int dim, F f) const {
+        float s = 0.f;
+#pragma unroll 1
+        for (int e = 0; e < VPT * VEC; e++) {
+            const int c = first(e / VEC) + e % VEC;
+            if (c >= 0 && c < dim) s += f(Elem<T>::to(row[c]));
+        }
+        return s;
+    }
     // Starts the copies of the row whose block 0 is `from` to this thread's own places in shared memory, nt blocks apart
     // (copies to places that are not side by side in a warp take half as long again); the same thread reads them after they have landed, so no barrier is needed. A block at the row's end brings elements of its
     // neighbours, or of the gap between two rows, along, which patch() replaces; only blocks that reach beyond the tensor
@@ -213,6 +224,12 @@ layernorm_kernel(const T* x, const float* __restrict__ gamma, const float* __res
             sq = fmaf(-share.extra * d, d, sq);
         }
         float m2 = warp_sum(sq);
+        if (!plain && !(m2 < INFINITY)) {
+            // what is subtracted or weighted by 0 above may have left fp32's range where the row's own elements do not: their
+            // sums again, without any other (a mask for every row would cost 8191 x 5003 fp16 two microseconds)
+            mean = warp_sum(share.sum(x + r * ld_x, dim, [](float f) { return f; })) * inv_warp;
+            m2 = warp_sum(share.sum(x + r * ld_x, dim, [&](float f) { return (f - mean) * (f - mean); }));
+        }
         if (warps > 1) {
             if (lane == 0) buf[turn][warp] = make_float2(mean, m2);
             asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(nt) : "memory");

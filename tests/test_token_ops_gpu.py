@@ -778,3 +778,24 @@ def test_captured_behind_copies_and_other_streams():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
         assert torch.equal(dtable[:50], dy) and not dtable[50:].any()
+
+
+# ---- rows at the border of fp32's range, whatever their length and alignment ---------------------------------
+@pytest.mark.parametrize("dim", [9, 300, 301, 1000, 1024, 5003, 16000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layernorm_rows_of_large_numbers(dim, dtype):
+    """What a thread holds beside its row (places without an element, neighbours in a cut block) must not reach the sums, not
+    even as the square of a mean beyond 2^64 times zero."""
+    x = torch.zeros(6, dim, device="cuda")
+    x[0] = 2.0 ** 63
+    x[1, 0] = x[2, -1] = 1.5e19  # squares 2.2e38, of which fp32 holds one
+    x[3] = rnd((dim,), 120) * 1e17
+    x[4, 0] = x[5, -1] = 1e38    # the sum fits, the squares do not: 1 / sqrt(inf)
+    x = x.to(dtype)
+    for v in (x, padded(x, 1), padded(x, 8, 1), padded(x, 3, 2)):
+        for gamma, beta in ((None, None), (rnd((dim,), 121) + 1, rnd((dim,), 122))):
+            y, mean, rstd = nz.layernorm_forward(v, gamma, beta)
+            _check_norm(x[:4], gamma, beta, 1e-5, (y[:4], mean[:4], rstd[:4]))
+            within(mean[4:], x[4:].double().mean(1), CHAIN * U * 1e38 / dim)
+            assert torch.equal(rstd[4:], torch.zeros(2, device="cuda"))
+            assert torch.equal(y[4:], torch.zeros_like(y[4:]) if beta is None else beta.to(dtype).expand(2, dim))
