@@ -403,11 +403,13 @@ layernorm_backward_kernel(const T* dy, const T* x, const float* __restrict__ mea
             float fx[VEC], fd[VEC];
             Elem<T>::unpack(xs[k * nt], fx);
             Elem<T>::unpack(ds[k * nt], fd);
+            // a place without elements: x is 0, and so has to be the mean, whose product with rstd may be inf (and its with 0 NaN)
+            const float2 shift = plain || share.has(k) ? minus : make_float2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < VEC / 2; i++) {
                 const float4 ga = params[k * (VEC / 4) + i / 2];
                 const float2 d = make_float2(fd[2 * i], fd[2 * i + 1]);
-                h[k][i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), minus), rs);
+                h[k][i] = mul2(add2(make_float2(fx[2 * i], fx[2 * i + 1]), shift), rs);
                 g[k][i] = mul2(d, i & 1 ? make_float2(ga.z, ga.w) : make_float2(ga.x, ga.y));
                 sg = add2(sg, g[k][i]);
                 sgh = fma2(g[k][i], h[k][i], sgh);

@@ -799,3 +799,25 @@ def test_layernorm_rows_of_large_numbers(dim, dtype):
             within(mean[4:], x[4:].double().mean(1), CHAIN * U * 1e38 / dim)
             assert torch.equal(rstd[4:], torch.zeros(2, device="cuda"))
             assert torch.equal(y[4:], torch.zeros_like(y[4:]) if beta is None else beta.to(dtype).expand(2, dim))
+
+
+@pytest.mark.parametrize("dim", [9, 300, 301, 1000, 1024, 5003, 9001, 16000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layernorm_backward_rows_of_large_numbers(dim, dtype):
+    """A mean whose product with rstd leaves fp32's range, beside places that hold no element of the row."""
+    rows = 5
+    x = torch.full((rows, dim), 2.0 ** 122, device="cuda").to(dtype)
+    mean, rstd = torch.full((rows,), 2.0 ** 122, device="cuda"), torch.full((rows,), 316.25, device="cuda")
+    dy, gamma = rnd((rows, dim), 123, dtype), rnd((dim,), 124) + 1
+    for gm in (gamma, None):
+        g = dy.double() * (1.0 if gm is None else gm.double())
+        want = 316.25 * (g - g.mean(1, keepdim=True))  # h is 0
+        tol = 316.25 * (g.abs() + g.abs().mean(1, keepdim=True)) * 2 * CHAIN * U
+        for extra, offset in ((0, 0), (1, 0), (8, 1)):
+            dx = padded(torch.zeros_like(x), extra, offset)
+            dg, db = torch.full((dim,), math.nan, device="cuda"), torch.full((dim,), math.nan, device="cuda")
+            nz.layernorm_backward(padded(dy, extra, offset), padded(x, extra, offset), mean, rstd, gm, dx, dg, db, overwrite_dx=True,
+                                  overwrite_dparams=True)
+            within(dx, want, tol + half_step(dtype) * (want.abs() + tol))
+            assert torch.equal(dg, torch.zeros_like(dg))
+            within(db, dy.double().sum(0), dy.double().abs().sum(0) * (rows + 32) * U)
