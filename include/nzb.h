@@ -519,7 +519,7 @@ NZB_API int nzb_embedding_backward(const nzb_embedding_desc* desc, const void* d
  * Backward, with h = (x - mean) * rstd and g = dy * gamma:
  *   dx (+)= rstd * (g - mean(g) - h * mean(g * h))     = with overwrite_dx, += without
  *   dgamma (+)= sum over rows of dy * h, dbeta (+)= sum over rows of dy      = with overwrite_dparams
- * Null outputs are skipped. dx may be dy or x (with its ld). dtype is the type of x, y, dy and dx.
+ * Null outputs are skipped. dx may be dy or x (with its ld); dgamma and dbeta must not overlap, nor mean and rstd. dtype is the type of x, y, dy and dx.
  */
 typedef struct nzb_layernorm_desc {
     int64_t rows, dim;

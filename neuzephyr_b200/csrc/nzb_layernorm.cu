@@ -584,6 +584,8 @@ static int check_layernorm(const nzb_layernorm_desc* d) {
     return NZB_OK;
 }
 
+static bool overlap(const float* a, const float* b, int64_t n) { return a && b && a < b + n && b < a + n; }
+
 // Threads that hold a row of `dim` elements in registers, `elems` each; 0: more than `most`. lead: elements the row's
 // first block may share with what is before it.
 static int norm_threads(int64_t dim, int lead, int most, int elems) {
@@ -648,6 +650,7 @@ int nzb_layernorm_forward(const nzb_layernorm_desc* d, const void* x, const floa
     if (rc != NZB_OK) return rc;
     if (d->rows == 0 || d->dim == 0) return NZB_OK;
     if (!x || !y) return fail(NZB_ERR_BAD_ARG, "x and y must be non-null");
+    if (overlap(mean, rstd, d->rows)) return fail(NZB_ERR_BAD_ARG, "mean and rstd overlap");
     if (x == y && d->ld_x != d->ld_y) return fail(NZB_ERR_BAD_ARG, "y in place of x needs its leading dimension");
     const int64_t size = dtype_size(d->dtype);
     if (!aligned_to(x, size) || !aligned_to(y, size)) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");
@@ -718,6 +721,8 @@ int nzb_layernorm_backward(const nzb_layernorm_desc* d, const void* dy, const vo
     if (dx && d->ld_dx < d->dim) return fail(NZB_ERR_BAD_ARG, "leading dimension smaller than the row length");
     if (dx && ((dx == dy && d->ld_dx != d->ld_y) || (dx == x && d->ld_dx != d->ld_x)))
         return fail(NZB_ERR_BAD_ARG, "dx in place of dy or x needs its leading dimension");
+    // both sums would go to one place, from different threads
+    if (overlap(dgamma, dbeta, d->dim)) return fail(NZB_ERR_BAD_ARG, "dgamma and dbeta overlap");
     DeviceState* ds;
     rc = get_device_state(&ds);
     if (rc != NZB_OK) return rc;

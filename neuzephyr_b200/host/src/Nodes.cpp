@@ -458,6 +458,7 @@ void LinearNode::backward() {
 
 LayerNormNode::LayerNormNode(Node* x, Node* gamma, Node* beta, float eps) : eps_(eps) {
     if (!x || !gamma || !beta) throw std::invalid_argument("LayerNormNode: x, gamma and beta must be given");
+    if (gamma == beta) throw std::invalid_argument("LayerNormNode: gamma and beta must be two nodes");
     const auto sx = x->output->shape();
     const size_t dim = sx.C() * sx.H() * sx.W();
     if (gamma->output->size() != dim || beta->output->size() != dim)

@@ -1,4 +1,4 @@
-// Which parameters of a model opt::Muon takes, by which scale, and what a refused step leaves behind. Needs a GPU.
+// Which parameters of a model opt::Muon takes, by which scale, what a refused step leaves behind, and what is refused. Needs a GPU.
 #include <NeuZephyr/Model.cuh>
 
 #include <algorithm>
@@ -266,10 +266,22 @@ static void test_refused_updates() {
     }
 }
 
+// One node cannot be both of a norm's parameters: two sums would be added to one gradient at a time.
+static void test_norm_of_one_parameter() {
+    InputNode x({2, 1, 8, 1}, true), g({1, 1, 8, 1}, true);
+    bool threw = false;
+    try {
+        LayerNormNode norm(&x, &g, &g);
+    } catch (const std::invalid_argument&) {
+        threw = true;
+    }
+    EXPECT_TRUE(threw);
+}
+
 int main() {
     const struct { const char* name; void (*fn)(); } tests[] = {
         {"convolutions", test_convolutions}, {"nodes_of_ones_own", test_nodes_of_ones_own}, {"saved_graph", test_saved_graph},
-        {"refused_updates", test_refused_updates},
+        {"refused_updates", test_refused_updates}, {"norm_of_one_parameter", test_norm_of_one_parameter},
     };
     for (auto& t : tests) {
         g_current = t.name;

@@ -208,3 +208,15 @@ def test_long_rows_need_a_small_workspace():
     dim = 1 << 20
     d = _layernorm(rows=1000, dim=dim, ld_x=dim, ld_y=dim, ld_dx=dim)
     assert L.nzb_layernorm_backward_workspace_bytes(ctypes.byref(d), ctypes.byref(n)) == C.OK and n.value == 64 * 2 * dim * 4
+
+
+def test_layernorm_results_that_overlap():
+    L = C.lib()
+    d = _layernorm(overwrite_dx=1, overwrite_dparams=1)
+    far = FAKE + (1 << 20)
+    for other in (FAKE, FAKE + 4 * 95, FAKE - 4 * 95):  # 96 floats each
+        assert L.nzb_layernorm_backward(ctypes.byref(d), far, far, far, far, None, far, FAKE, other, far, 1 << 30, None) == C.ERR_BAD_ARG
+        assert b"overlap" in L.nzb_last_error_string()
+    for other in (FAKE, FAKE + 4 * 6, FAKE - 4 * 6):  # 7 rows
+        assert L.nzb_layernorm_forward(ctypes.byref(d), far, None, None, far, FAKE, other, None) == C.ERR_BAD_ARG
+        assert b"overlap" in L.nzb_last_error_string()
