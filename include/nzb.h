@@ -515,7 +515,8 @@ NZB_API int nzb_embedding_backward(const nzb_embedding_desc* desc, const void* d
 /*
  * Layer norm over the last dimension: mean and variance of each row (the variance from the centred row),
  * rstd = 1 / sqrt(var + eps), y = (x - mean) * rstd * gamma + beta. gamma and beta (fp32, {dim}) may be null
- * (1 and 0), mean and rstd (fp32, {rows}) may be null when nothing reads them. y may be x (with its ld).
+ * (1 and 0), mean and rstd (fp32, {rows}) may be null when nothing reads them; rows of no elements (dim 0) have NaN. y may be
+ * x (with its ld).
  * Backward, with h = (x - mean) * rstd and g = dy * gamma:
  *   dx (+)= rstd * (g - mean(g) - h * mean(g * h))     = with overwrite_dx, += without
  *   dgamma (+)= sum over rows of dy * h, dbeta (+)= sum over rows of dy      = with overwrite_dparams

@@ -648,9 +648,14 @@ int nzb_layernorm_forward(const nzb_layernorm_desc* d, const void* x, const floa
                           float* mean, float* rstd, void* stream) {
     int rc = check_layernorm(d);
     if (rc != NZB_OK) return rc;
-    if (d->rows == 0 || d->dim == 0) return NZB_OK;
-    if (!x || !y) return fail(NZB_ERR_BAD_ARG, "x and y must be non-null");
+    if (d->rows == 0) return NZB_OK;
     if (overlap(mean, rstd, d->rows)) return fail(NZB_ERR_BAD_ARG, "mean and rstd overlap");
+    if (d->dim == 0) {  // the mean of nothing: every bit set is a NaN
+        if (mean) NZB_CUDA_TRY(cudaMemsetAsync(mean, 0xff, (size_t)d->rows * 4, static_cast<cudaStream_t>(stream)));
+        if (rstd) NZB_CUDA_TRY(cudaMemsetAsync(rstd, 0xff, (size_t)d->rows * 4, static_cast<cudaStream_t>(stream)));
+        return NZB_OK;
+    }
+    if (!x || !y) return fail(NZB_ERR_BAD_ARG, "x and y must be non-null");
     if (x == y && d->ld_x != d->ld_y) return fail(NZB_ERR_BAD_ARG, "y in place of x needs its leading dimension");
     const int64_t size = dtype_size(d->dtype);
     if (!aligned_to(x, size) || !aligned_to(y, size)) return fail(NZB_ERR_BAD_ARG, "pointer is not a multiple of its element's size");

@@ -821,3 +821,11 @@ def test_layernorm_backward_rows_of_large_numbers(dim, dtype):
             within(dx, want, tol + half_step(dtype) * (want.abs() + tol))
             assert torch.equal(dg, torch.zeros_like(dg))
             within(db, dy.double().sum(0), dy.double().abs().sum(0) * (rows + 32) * U)
+
+
+def test_layernorm_of_rows_without_elements():
+    torch.full((64,), 5.0, device="cuda")  # what the allocator hands out next is not NaN by chance
+    y, mean, rstd = nz.layernorm_forward(torch.empty(3, 0, device="cuda"))
+    assert y.shape == (3, 0) and torch.isnan(mean).all() and torch.isnan(rstd).all()
+    dx, none = torch.empty(3, 0, device="cuda"), torch.empty(0, device="cuda")
+    nz.layernorm_backward(y, y, mean, rstd, none, dx, none, none, overwrite_dx=True, overwrite_dparams=True)
