@@ -368,7 +368,8 @@ void Adam::step(nodes::Node* input) {
     data::Tensor& t = *input->output;
     auto& m = m_[input];
     auto& v = v_[input];
-    if (!m) {
+    // moments of another size belong to a node that is gone and whose address this one took
+    if (!m || m->size() != t.size()) {
         m = std::make_unique<data::Tensor>(t.shape());
         v = std::make_unique<data::Tensor>(t.shape());
         m->clear();
@@ -456,7 +457,7 @@ void Muon::step(nodes::Node* input) {
     }
     data::Tensor& t = *input->output;
     auto& m = momentum_[input];
-    if (!m) {
+    if (!m || !(m->shape() == t.shape())) {  // none, or that of a node that is gone and whose address this one took
         m = std::make_unique<data::Tensor>(t.shape());
         m->clear();
     }

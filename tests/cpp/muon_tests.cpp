@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <new>
 #include <random>
 #include <stdexcept>
 #include <string>
@@ -278,10 +279,39 @@ static void test_norm_of_one_parameter() {
     EXPECT_TRUE(threw);
 }
 
+// A parameter at the address of one that is gone, of another size: it has a state of its own.
+static void test_address_taken_again() {
+    alignas(InputNode) unsigned char place[sizeof(InputNode)];
+    opt::Adam adam(0.01f, 0.9f, 0.999f);
+    opt::Muon muon(0.05f, 0.9f, &adam);
+    const size_t sides[][2] = {{4, 6}, {40, 70}, {70, 40}, {300, 1}, {4, 1}};
+    for (const auto& hw : sides) {
+        const size_t h = hw[0], w = hw[1];
+        auto* n = new (place) InputNode({1, 1, h, w}, true);
+        const auto v = normal(h * w, 60), g = normal(h * w, 61);
+        n->output->dataInject(v.begin(), v.end());
+        n->output->dataInject(g.begin(), g.end(), true);
+        muon.step(n);
+        const auto got = n->output->hostData(), state = muon.exportState(n)[0];
+        EXPECT_TRUE(state.size() == h * w);
+        if (w > 1) {
+            EXPECT_TRUE(updated(got, v, g, 1, h, w, 0.05f * std::sqrt(std::max(1.0, (double)h / w))));
+            EXPECT_TRUE(state == g);  // the first step's momentum
+        } else {
+            // Adam's first moment after one step: (1 - 0.9) g
+            double worst = 0;
+            for (size_t i = 0; i < h; i++) worst = std::max(worst, std::fabs(state[i] - (1.0 - 0.9f) * g[i]));
+            EXPECT_TRUE(worst <= 4 * U * 4);
+        }
+        n->~InputNode();
+    }
+}
+
 int main() {
     const struct { const char* name; void (*fn)(); } tests[] = {
         {"convolutions", test_convolutions}, {"nodes_of_ones_own", test_nodes_of_ones_own}, {"saved_graph", test_saved_graph},
         {"refused_updates", test_refused_updates}, {"norm_of_one_parameter", test_norm_of_one_parameter},
+        {"address_taken_again", test_address_taken_again},
     };
     for (auto& t : tests) {
         g_current = t.name;
