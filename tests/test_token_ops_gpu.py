@@ -829,3 +829,16 @@ def test_layernorm_of_rows_without_elements():
     assert y.shape == (3, 0) and torch.isnan(mean).all() and torch.isnan(rstd).all()
     dx, none = torch.empty(3, 0, device="cuda"), torch.empty(0, device="cuda")
     nz.layernorm_backward(y, y, mean, rstd, none, dx, none, none, overwrite_dx=True, overwrite_dparams=True)
+
+
+# ---- many rows: several groups to a CTA that walk different numbers of rows, joined at the end -----------------
+@pytest.mark.parametrize("rows,dim", [(1500, 96), (3001, 1027), (5000, 216), (2500, 5003), (9500, 2048), (40001, 33)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layernorm_forward_of_many_rows(rows, dim, dtype):
+    test_layernorm_forward(rows, dim, dtype)
+
+
+@pytest.mark.parametrize("rows,dim", [(2500, 1027), (5000, 216), (9500, 2048), (3000, 5003), (1777, 9000), (40001, 33)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layernorm_backward_of_many_rows(rows, dim, dtype):
+    test_layernorm_backward(rows, dim, dtype)
