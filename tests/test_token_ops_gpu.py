@@ -842,3 +842,28 @@ def test_layernorm_forward_of_many_rows(rows, dim, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_layernorm_backward_of_many_rows(rows, dim, dtype):
     test_layernorm_backward(rows, dim, dtype)
+
+
+# ---- tables above 2^23 elements and more than 2048 tokens: rows cleared beside the sort, by the marks ----------
+@pytest.mark.parametrize("tokens,vocab,dim", [(2049, 70001, 131), (5000, 70001, 131), (16384, 40000, 256), (40000, 60000, 200)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_backward_of_large_tables(tokens, vocab, dim, dtype):
+    test_embedding_backward(tokens, vocab, dim, dtype)
+
+
+def test_embedding_backward_of_large_tables_strides():
+    tokens, vocab, dim = 20000, 70001, 131
+    g = torch.Generator("cuda").manual_seed(125)
+    idx = torch.randint(0, vocab, (tokens,), device="cuda", generator=g)
+    idx[::3] = 70000  # a third of the text is the table's last row
+    dy = rnd((tokens, dim), 126, BF16)
+    plain = torch.full((vocab, dim), math.nan, device="cuda")
+    nz.embedding_backward(dy, idx, plain, overwrite=True)
+    want, mags, count = _embedding_grad(dy, idx, vocab, 1.0, None)
+    within(plain, want, mags * (count + 6) * U + 1e-30)
+    for extra, offset in ((1, 0), (5, 3), (13, 1)):
+        out = padded(torch.full((vocab, dim), math.nan, device="cuda"), extra, offset)
+        nz.embedding_backward(dy, idx, out, overwrite=True)
+        assert torch.equal(out, plain)
+        out.fill_(77.0)
+        assert (out._base == 77.0).all()  # nothing between the rows was written
