@@ -867,3 +867,45 @@ def test_embedding_backward_of_large_tables_strides():
         assert torch.equal(out, plain)
         out.fill_(77.0)
         assert (out._base == 77.0).all()  # nothing between the rows was written
+
+
+# ---- large sides: 256 x 256 tiles by pairs of CTAs in all three products, with remainders ----------------------
+def _tiles_launched(run):
+    """Which tiles (pair of CTAs?, columns, product) a call launches, by the kernels' names; None where no profiler runs."""
+    import re
+    from torch.profiler import ProfilerActivity, profile
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        run()
+        torch.cuda.synchronize()
+    if not any(e.device_type == torch.autograd.DeviceType.CUDA for e in p.events()):
+        return None
+    names = {e.name for e in p.events() if "ns_product_kernel" in e.name}
+    found = {re.search(r"NsCfg<\(?(?:bool\))?(\w+), ?(?:\(int\))?(\d+)>, ?(?:\(int\))?(\d+)", n) for n in names}
+    assert None not in found, names
+    return {(m[1] in ("true", "1"), int(m[2]), int(m[3])) for m in found}
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 2103, 2331), (1, 2331, 2103), (3, 2049, 2600), (2, 2600, 2049), (1, 4103, 4500), (1, 4500, 4103)])
+def test_orthogonalize_by_pairs(batch, rows, cols):
+    g = torch.stack([_gradient_like(rows, cols, 130 + i) for i in range(batch)])
+    got = nz.orthogonalize(g)
+    for i in range(batch):
+        assert _rel(got[i], _ortho_ref(g[i])) <= ORTHO_TOL
+    assert torch.equal(got, nz.orthogonalize(g))
+    half = nz.orthogonalize(g.to(BF16), out_dtype=F16)
+    assert _rel(half[0], _ortho_ref(g[0].to(BF16))) <= ORTHO_TOL + half_step(F16)
+    assert _tiles_launched(lambda: nz.orthogonalize(g)) in (None, {(True, 256, mode) for mode in range(3)})
+    assert nz.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(2103, 2331), (2331, 2103)])
+def test_muon_step_by_pairs(shape):
+    w, m, g = rnd(shape, 140), rnd(shape, 141), rnd(shape, 142)
+    got_w, got_m = w.clone(), m.clone()
+    nz.muon_step(got_w, got_m, g, 0.02, mu=0.9, weight_decay=0.1)
+    m2 = 0.9 * m.double() + g.double()
+    o = _ortho_ref(g.double() + 0.9 * m2)
+    step = 0.02 * max(1.0, shape[0] / shape[1]) ** 0.5
+    err = torch.linalg.norm(got_w.double() - ((1 - 0.02 * 0.1) * w.double() - step * o))
+    assert err <= step * ORTHO_TOL * torch.linalg.norm(o) + 4 * U * torch.linalg.norm(w)
+    within(got_m, m2, 2 * U * (m.abs() + g.abs()))
