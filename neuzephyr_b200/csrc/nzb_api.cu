@@ -37,7 +37,12 @@ int get_device_state(DeviceState** out) {
         NZB_CUDA_TRY(cudaGetDeviceProperties(&prop, dev));
         if (prop.major != 10) return fail(NZB_ERR_NO_DEVICE, "device %d is sm_%d%d; this library holds sm_100a code only", dev, prop.major, prop.minor);
         int* h = nullptr;
-        NZB_CUDA_TRY(cudaHostAlloc(&h, sizeof(int) * 16, cudaHostAllocMapped));
+        // an allocation would invalidate a stream capture that runs meanwhile; this one has nothing to do with it
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        NZB_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t allocated = cudaHostAlloc(&h, sizeof(int) * 16, cudaHostAllocMapped);
+        NZB_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+        NZB_CUDA_TRY(allocated);
         for (int i = 0; i < 16; i++) h[i] = 0;
         int* d = nullptr;
         NZB_CUDA_TRY(cudaHostGetDevicePointer(&d, h, 0));

@@ -909,3 +909,31 @@ def test_muon_step_by_pairs(shape):
     err = torch.linalg.norm(got_w.double() - ((1 - 0.02 * 0.1) * w.double() - step * o))
     assert err <= step * ORTHO_TOL * torch.linalg.norm(o) + 4 * U * torch.linalg.norm(w)
     within(got_m, m2, 2 * U * (m.abs() + g.abs()))
+
+
+FIRST_CALL = """
+import torch
+import neuzephyr_b200 as nz
+x, t = torch.randn(70, 300, device="cuda"), torch.randint(0, 300, (70,), device="cuda")
+table, dy, idx = torch.empty(70001, 131, device="cuda"), torch.randn(5000, 131, device="cuda"), torch.randint(0, 70001, (5000,), device="cuda")
+run = {"embedding": lambda: nz.embedding(x, t % 70), "embedding_backward": lambda: nz.embedding_backward(dy, idx, table, overwrite=True),
+       "layernorm": lambda: nz.layernorm_forward(x)[0], "token_logprobs": lambda: nz.token_logprobs(x, t, top_k=3).logprob,
+       "orthogonalize": lambda: nz.orthogonalize(x)}["CALL"]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = run()
+graph.replay()
+torch.cuda.synchronize()
+replayed = y.clone()
+assert torch.equal(replayed, run())
+"""
+
+
+@pytest.mark.parametrize("call", ["embedding", "embedding_backward", "layernorm", "token_logprobs", "orthogonalize"])
+def test_first_call_of_a_process_within_a_capture(call):
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("CALL", call)], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr[-2000:]
