@@ -476,7 +476,8 @@ NZB_API int nzb_scale(float* data, float factor, int64_t n, void* stream);
 /* Token models --------------------------------------------------------------------------------
  * Rows of a table, layer norm, log probabilities of tokens and the orthogonalised update: what a model of
  * tokens needs next to Linear, the softmax head and Adam. NeuZephyr has no counterpart of these four. All of
- * them compute in fp32 whatever the stored type, round once at the end, use no floating-point atomics (the
+ * them compute in fp32 whatever the stored type and round to it once at the end (the products of the orthogonalised
+ * update take operands of 22 bits, see there), use no floating-point atomics (the
  * same call gives the same bits) and only work on the arguments they are given, so calls on different streams
  * and captured graphs share nothing. Strides ("ld") are in elements between the starts of two rows; the
  * elements of a row are contiguous. Vectors of 16 bytes are used where a row's address allows; any address
@@ -572,8 +573,10 @@ NZB_API int nzb_token_logprob_backward(const nzb_token_logprob_desc* desc, const
  * Orthogonalised update: brings the singular values of each of `batch` matrices G {rows, cols} near 1 by
  * `steps` Newton-Schulz products, X = G / (|G|_F + eps), then steps times
  *   A = X X^T, B = coef[1] A + coef[2] A A, X = coef[0] X + B X      (rows <= cols; else with X^T X and X B).
- * X is held in fp32; the tensor cores read fp16 copies of X, A and B (scaled by 2^12, fp32 sums), the diagonal
- * of B is kept in fp32. Relative error of the result against 64 bits: about 1e-3 (2-norm), whatever out_dtype.
+ * X is held in fp32; the tensor cores multiply pairs of fp16 numbers that hold 22 bits of X, A and B (fp32 sums),
+ * the diagonal of B is kept in fp32. Error against 64 bits, relative in the Frobenius norm and before the one rounding to
+ * out_dtype: 1e-5 at sides of a few hundred, 6e-5 at 4096. What a matrix of low rank leaves empty fills with rounding
+ * noise that grows by coef[0] a step, as it does with fp32 products: 1e-4 and 1e-3 for matrices of rank one.
  * Coefficients have to keep the singular values of X below 2.8, as (3.4445, -4.775, 2.0315) do. A matrix of
  * zeros gives zeros. out may be g.
  */

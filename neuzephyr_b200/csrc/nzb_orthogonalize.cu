@@ -7,12 +7,15 @@
 // of which the symmetric A and B need one half each.
 //
 // Precision. The recurrence multiplies small singular values by c0 (3.4) a step, and with them whatever noise the
-// roundings put there, so X itself is held in fp32: X = (c0 + B_ii) X32 + (B - diag B) X16. Only the products'
-// operands are fp16 (rounding 2^-12 relative); X and A are stored times 2^12, so that entries down to 2^-26 keep all
-// bits, B as it is (entries below 2^-14 lose relative precision there, where c0 X outweighs them by far), and B's
-// diagonal, which carries most of B once X is near orthogonal, multiplies the fp32 X. Simulated against 64 bits
-// on full-rank, decaying and nearly low-rank matrices: 3e-4 .. 1e-3 for sides of 128 and more; with X rounded
-// to bf16 in every step 1e-2 .. 3e-1.
+// roundings put there: 140 times what the first step rounds off, in the directions that a matrix of low rank leaves empty. So
+// X is held in fp32, X = (c0 + B_ii) X32 + (B - diag B) X, and the products' operands as pairs of fp16 numbers, high =
+// fp16(v) and low = fp16(v - high), 22 bits together, of which a product takes high high + high low + low high. X and A
+// are stored times 2^12, so that entries down to 2^-26 keep 11 bits in each part, B as it is (its pairs leave out less than
+// 2^-25, where c0 X outweighs it by far); B's diagonal, which carries most of B once X is near orthogonal, multiplies the
+// fp32 X. Against 64 bits (Frobenius norm): 1e-5 at 256 x 512, 2e-5 at 1000 x 1400, 6e-5 at 4096 x 4096 (the tensor cores'
+// sums are what is left), and for matrices of rank one, where fp32 products do no better, 1e-4, 3e-4 and 9e-4. The
+// high parts alone take 0.4 of the time at large sides and are 1e-3 off, but 4e-2 for a rank-one matrix of uneven entries, at
+// any size.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -25,7 +28,7 @@
 
 namespace nzb {
 
-constexpr float kNsScale = 4096.f;            // 2^12: what X (both copies) and A are multiplied by
+constexpr float kNsScale = 4096.f;            // 2^12: what X (all copies) and A are multiplied by
 constexpr float kNsUnscale = 1.f / 4096.f;
 
 enum { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2 };
@@ -44,8 +47,8 @@ struct NsParams {
     float* partial;            // [split][matrix][rows and columns of the short side in blocks of 32 x 32]
     int64_t stride_part, batch;
     float c0, c1, c2;
-    __half* out16;             // 2^12 A, B or the next 2^12 X
-    int64_t ld16, stride16;
+    __half* out16;             // 2^12 A, B or the next 2^12 X: first all matrices' high parts, then their low parts
+    int64_t ld16, stride16, low16;  // low16: from a high part to its low part
     const __half* gram;        // NS_POLY: A times 2^12, same layout as out16
     float* diag;               // c0 + B_ii, `short_side` per matrix
     int64_t short_side;
@@ -62,15 +65,17 @@ template <bool PAIR_, int BN_>
 struct NsCfg {
     static constexpr bool PAIR = PAIR_;
     static constexpr int BM = PAIR ? 256 : 128, BN = BN_;
-    static constexpr int STAGES = 6;
+    static constexpr int STAGES = BN >= 128 ? 3 : 4;
     // two or four per quarter of the tensor-memory lanes. The epilogue is a long chain per warp (tensor memory, shared
-    // memory, memory): on a 256-wide tile eight warps took 15000 cycles, whatever they left out, sixteen 7500
+    // memory, memory): on a 256-wide tile, with one part to write, eight warps took 15000 cycles, whatever they left out,
+    // sixteen 7500
     static constexpr int EPI_WARPS = BN >= 128 ? 16 : 8;
     static constexpr int COLS = BN * 4 / EPI_WARPS;   // columns of a warp
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN; // rows of B that a CTA loads
-    static constexpr int A_BYTES = 128 * 64 * 2;      // per k block of 64
-    static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * 64 * 2;
+    static constexpr int A_BYTES = 128 * 64 * 2;      // per k block of 64 and part
+    static constexpr int B_BYTES = B_ROWS * 64 * 2;
+    static constexpr int STAGE_BYTES = 2 * (A_BYTES + B_BYTES);  // A high, A low, B high, B low
     static constexpr int EPI_BYTES = EPI_WARPS * 2048;  // 32 x 32 fp16 entries per warp
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
     static constexpr int TMEM_COLS = 2 * BN;
@@ -113,7 +118,7 @@ __device__ __forceinline__ void ns_decode(const NsParams& p, int64_t tile, int32
 // row and four lanes per row both go without bank conflicts.
 __device__ __forceinline__ uint4* ns_piece(float* stage, int r, int j) { return reinterpret_cast<uint4*>(stage) + r * 4 + (j ^ (r >> 1 & 3)); }
 
-// Writes 32 x 32 entries, a row per lane in h, at (row0, col0) of an A or B and, with `mirror`, their mirror image. Rows
+// Writes 32 x 32 entries of one part, a row per lane in h, at (row0, col0) of an A or B and, with `mirror`, their mirror image. Rows
 // go to memory four lanes to 64 bytes, by way of shared memory (a lane per row touches 32 lines an instruction: 19000
 // cycles for a 256 x 256 tile of B).
 __device__ __forceinline__ void ns_store_block(const NsParams& p, __half* out, float* stage, int lane, int32_t row0, int32_t col0,
@@ -146,6 +151,12 @@ __device__ __forceinline__ void ns_store_block(const NsParams& p, __half* out, f
     put(col0, p.N, row0);
 }
 
+// A pair of numbers as fp16 high parts and what they leave, in fp16 too.
+__device__ __forceinline__ __half2 ns_low(float x, float y, __half2 high) {
+    const float2 f = __half22float2(high);
+    return __floats2half2_rn(x - f.x, y - f.y);
+}
+
 // X32 (2^12 X) in the order the epilogue holds it: blocks of 32 x 32, in each the rows' first four columns, then the rows' next
 // four, so that a lane per row reads and writes 512 contiguous bytes an instruction. Offset of row r's columns c .. c + 3.
 __host__ __device__ __forceinline__ int64_t ns_state_at(int64_t r, int64_t c, int64_t ldx) {
@@ -153,8 +164,7 @@ __host__ __device__ __forceinline__ int64_t ns_state_at(int64_t r, int64_t c, in
 }
 
 // Drains 32 rows x a warp's columns of a finished A or B tile: every lane holds one row, 32 columns at a time. `ready` waits for
-// the accumulator; what else a group of columns needs is loaded before that, and for the next group before this one is
-// written.
+// the accumulator; what else a group of columns needs is loaded before that.
 template <class Cfg, int MODE, class Ready>
 __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t tmem, float* stage, int lane, int32_t b, int32_t row0,
                                                    int32_t col_first, bool mirror, int32_t split, int64_t batch, Ready ready) {
@@ -163,12 +173,15 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
     const int32_t row = row0 + lane;
     const int pr = lane >> 2, pj = lane & 3;
     const __half* gram = p.gram + b * p.stride16;
-    uint4 g[4];
+    uint4 g[2][4];  // A's high and low parts
     const auto fetch = [&](int32_t col0) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int32_t r = row0 + 8 * i + pr;
-            g[i] = r < p.M && col0 < p.N ? *reinterpret_cast<const uint4*>(gram + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj) : make_uint4(0, 0, 0, 0);
+            const __half* from = gram + static_cast<int64_t>(r) * p.ld16 + col0 + 8 * pj;
+            const bool in = r < p.M && col0 < p.N;
+            g[0][i] = in ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+            g[1][i] = in ? *reinterpret_cast<const uint4*>(from + p.low16) : make_uint4(0, 0, 0, 0);
         }
     };
     const float k1 = p.c1 * kNsUnscale, k2 = p.c2 * kNsUnscale * kNsUnscale;
@@ -181,7 +194,6 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
         uint32_t v[32];
         tmem_ld_32x32(tmem + c0, v);
         tmem_ld_wait();
-        __half2 h[16];
         if (MODE == NS_GRAM && p.splits > 1) {
             // a part of the sum, as the accumulator has it
             if (row0 < p.M) {
@@ -192,30 +204,45 @@ __device__ __forceinline__ bool ns_drain_symmetric(const NsParams& p, uint32_t t
             }
             continue;
         }
+        float x[32];
         if (MODE == NS_GRAM) {
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                h[j] = __floats2half2_rn(__uint_as_float(v[2 * j]) * kNsUnscale, __uint_as_float(v[2 * j + 1]) * kNsUnscale);
+            for (int j = 0; j < 32; j++) x[j] = __uint_as_float(v[j]) * kNsUnscale;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) *ns_piece(stage, 8 * i + pr, pj) = g[i];
-            __syncwarp();
-            uint4 mine[4];
+            for (int j = 0; j < 32; j++) x[j] = k2 * __uint_as_float(v[j]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) mine[j] = *ns_piece(stage, lane, j);
-            __syncwarp();
-            if (c0 + 32 < Cfg::COLS) fetch(col0 + 32);
-            const __half2* gh = reinterpret_cast<const __half2*>(mine);
+            for (int part = 0; part < 2; part++) {
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float2 a = __half22float2(gh[j]);
-                const float x = fmaf(k1, a.x, k2 * __uint_as_float(v[2 * j])), y = fmaf(k1, a.y, k2 * __uint_as_float(v[2 * j + 1]));
-                const int32_t c = col0 + 2 * j;
-                if (row < p.M && (row == c || row == c + 1)) p.diag[b * p.short_side + row] = p.c0 + (row == c ? x : y);
-                h[j] = __floats2half2_rn(row == c ? 0.f : x, row == c + 1 ? 0.f : y);
+                for (int i = 0; i < 4; i++) *ns_piece(stage, 8 * i + pr, pj) = g[part][i];
+                __syncwarp();
+                uint4 mine[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) mine[j] = *ns_piece(stage, lane, j);
+                __syncwarp();
+                const __half2* gh = reinterpret_cast<const __half2*>(mine);
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const float2 a = __half22float2(gh[j]);
+                    x[2 * j] = fmaf(k1, a.x, x[2 * j]);
+                    x[2 * j + 1] = fmaf(k1, a.y, x[2 * j + 1]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                if (row != col0 + j) continue;
+                if (row < p.M) p.diag[b * p.short_side + row] = p.c0 + x[j];
+                x[j] = 0.f;
             }
         }
+        __half2 h[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
         ns_store_block(p, out, stage, lane, row0, col0, h, mirror);
+#pragma unroll
+        for (int j = 0; j < 16; j++) h[j] = ns_low(x[2 * j], x[2 * j + 1], h[j]);
+        ns_store_block(p, out + p.low16, stage, lane, row0, col0, h, mirror);
+        if (MODE == NS_POLY && c0 + 32 < Cfg::COLS) fetch(col0 + 32);
     }
     return true;
 }
@@ -303,41 +330,52 @@ __device__ __forceinline__ bool ns_drain_apply(const NsParams& p, uint32_t tmem,
             }
             continue;
         }
-        uint32_t h[16];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (p.out_kind == NS_OUT_BF16) {
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[j].x, x[j].y), hi = __floats2bfloat162_rn(x[j].z, x[j].w);
-                h[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
-                h[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-            } else {
-                const __half2 lo = __floats2half2_rn(x[j].x, x[j].y), hi = __floats2half2_rn(x[j].z, x[j].w);
-                h[2 * j] = *reinterpret_cast<const uint32_t*>(&lo);
-                h[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
-        __syncwarp();
         const bool state = p.out_kind == NS_OUT_STATE;
         const int64_t ld = state ? p.ld16 : p.ld_out;
         uint16_t* out = (state ? reinterpret_cast<uint16_t*>(p.out16) + b * p.stride16 : static_cast<uint16_t*>(p.out) + b * p.stride_out) +
                         static_cast<int64_t>(row0 + pr) * ld + col0 + 8 * pj;
         const bool vec = state || (p.out_vec && col0 + 8 * pj + 8 <= p.N);  // the state's padded rows hold whole groups
+        __half2 h[16];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
-            if (row0 + 8 * i + pr >= p.M) continue;
-            if (vec) {
-                *reinterpret_cast<uint4*>(out + 8 * i * ld) = u;
+        for (int j = 0; j < 8; j++) {
+            if (p.out_kind == NS_OUT_BF16) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(x[j].x, x[j].y), hi = __floats2bfloat162_rn(x[j].z, x[j].w);
+                h[2 * j] = *reinterpret_cast<const __half2*>(&lo);
+                h[2 * j + 1] = *reinterpret_cast<const __half2*>(&hi);
             } else {
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (col0 + 8 * pj + k < p.N) out[8 * i * ld + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+                h[2 * j] = __floats2half2_rn(x[j].x, x[j].y);
+                h[2 * j + 1] = __floats2half2_rn(x[j].z, x[j].w);
             }
         }
-        __syncwarp();
+        // a result's rows, or the state's high parts and then its low parts
+#pragma unroll 1
+        for (int part = 0; part < (state ? 2 : 1); part++, out += p.low16) {
+            if (part) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    h[2 * j] = ns_low(x[j].x, x[j].y, h[2 * j]);
+                    h[2 * j + 1] = ns_low(x[j].z, x[j].w, h[2 * j + 1]);
+                }
+            }
+            const uint4* own = reinterpret_cast<const uint4*>(h);
+#pragma unroll
+            for (int j = 0; j < 4; j++) *ns_piece(stage, lane, j) = own[j];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint4 u = *ns_piece(stage, 8 * i + pr, pj);
+                if (row0 + 8 * i + pr >= p.M) continue;
+                if (vec) {
+                    *reinterpret_cast<uint4*>(out + 8 * i * ld) = u;
+                } else {
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (col0 + 8 * pj + k < p.N) out[8 * i * ld + k] = static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)));
+                }
+            }
+            __syncwarp();
+        }
     }
     return true;
 }
@@ -415,15 +453,21 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 }
                 if (elect_one()) {
                     uint8_t* sa = smem + s * Cfg::STAGE_BYTES;
+                    uint8_t* sb = sa + 2 * Cfg::A_BYTES;
+                    const int32_t low = b + static_cast<int32_t>(p.batch);  // the low parts follow all high parts
                     if constexpr (PAIR) {
                         const uint32_t leader_full = map_to_cta(smem_u32(&full[s]), 0);
                         if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
                         load_operand_pair<128>(sa, &tmA, p.a_mn, kb * 64, row_a, b, leader_full);
-                        load_operand_pair<Cfg::B_ROWS>(sa + Cfg::A_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, leader_full);
+                        load_operand_pair<Cfg::B_ROWS>(sb, &tmB, p.b_mn, kb * 64, row_b, b, leader_full);
+                        load_operand_pair<128>(sa + Cfg::A_BYTES, &tmA, p.a_mn, kb * 64, row_a, low, leader_full);
+                        load_operand_pair<Cfg::B_ROWS>(sb + Cfg::B_BYTES, &tmB, p.b_mn, kb * 64, row_b, low, leader_full);
                     } else {
                         mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
                         load_operand<128>(sa, &tmA, p.a_mn, kb * 64, row_a, b, &full[s]);
-                        load_operand<Cfg::B_ROWS>(sa + Cfg::A_BYTES, &tmB, p.b_mn, kb * 64, row_b, b, &full[s]);
+                        load_operand<Cfg::B_ROWS>(sb, &tmB, p.b_mn, kb * 64, row_b, b, &full[s]);
+                        load_operand<128>(sa + Cfg::A_BYTES, &tmA, p.a_mn, kb * 64, row_a, low, &full[s]);
+                        load_operand<Cfg::B_ROWS>(sb + Cfg::B_BYTES, &tmB, p.b_mn, kb * 64, row_b, low, &full[s]);
                     }
                 }
                 __syncwarp();
@@ -462,22 +506,28 @@ ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     tc_fence_after();
                     const uint32_t sa = smem_u32(smem + s * Cfg::STAGE_BYTES);
                     const uint64_t da = hi_a | ((sa & 0x3ffff) >> 4);
-                    const uint64_t db = hi_b | (((sa + Cfg::A_BYTES) & 0x3ffff) >> 4);
+                    const uint64_t db = hi_b | (((sa + 2 * Cfg::A_BYTES) & 0x3ffff) >> 4);
                     const int32_t ksteps = kb == p.k_blocks - 1 ? p.last_ksteps : 4;
                     if (elect_one()) {
-                        if constexpr (PAIR) {
-                            mma_f16_ss_pair(d_tmem, da, db, idesc, kb > k0 ? 1u : 0u);
-                            if (ksteps > 1) mma_f16_ss_pair(d_tmem, da + ka, db + kb_step, idesc, 1u);
-                            if (ksteps > 2) mma_f16_ss_pair(d_tmem, da + 2 * ka, db + 2 * kb_step, idesc, 1u);
-                            if (ksteps > 3) mma_f16_ss_pair(d_tmem, da + 3 * ka, db + 3 * kb_step, idesc, 1u);
-                            mma_commit_pair(&empty[s]);
-                        } else {
-                            mma_f16_ss(d_tmem, da, db, idesc, kb > k0 ? 1u : 0u);
-                            if (ksteps > 1) mma_f16_ss(d_tmem, da + ka, db + kb_step, idesc, 1u);
-                            if (ksteps > 2) mma_f16_ss(d_tmem, da + 2 * ka, db + 2 * kb_step, idesc, 1u);
-                            if (ksteps > 3) mma_f16_ss(d_tmem, da + 3 * ka, db + 3 * kb_step, idesc, 1u);
-                            mma_commit(&empty[s]);
+                        // high x high, high x low, low x high; low x low is below fp32's last bit
+#pragma unroll
+                        for (int term = 0; term < 3; term++) {
+                            const uint64_t ta = da + (term == 2 ? Cfg::A_BYTES >> 4 : 0), tb = db + (term == 1 ? Cfg::B_BYTES >> 4 : 0);
+                            const uint32_t onto = term || kb > k0 ? 1u : 0u;
+                            if constexpr (PAIR) {
+                                mma_f16_ss_pair(d_tmem, ta, tb, idesc, onto);
+                                if (ksteps > 1) mma_f16_ss_pair(d_tmem, ta + ka, tb + kb_step, idesc, 1u);
+                                if (ksteps > 2) mma_f16_ss_pair(d_tmem, ta + 2 * ka, tb + 2 * kb_step, idesc, 1u);
+                                if (ksteps > 3) mma_f16_ss_pair(d_tmem, ta + 3 * ka, tb + 3 * kb_step, idesc, 1u);
+                            } else {
+                                mma_f16_ss(d_tmem, ta, tb, idesc, onto);
+                                if (ksteps > 1) mma_f16_ss(d_tmem, ta + ka, tb + kb_step, idesc, 1u);
+                                if (ksteps > 2) mma_f16_ss(d_tmem, ta + 2 * ka, tb + 2 * kb_step, idesc, 1u);
+                                if (ksteps > 3) mma_f16_ss(d_tmem, ta + 3 * ka, tb + 3 * kb_step, idesc, 1u);
+                            }
                         }
+                        if constexpr (PAIR) mma_commit_pair(&empty[s]);
+                        else mma_commit(&empty[s]);
                     }
                     __syncwarp();
                 }
@@ -561,13 +611,21 @@ ns_gram_sum_kernel(const NsParams p) {
             sum[j].x += v.x; sum[j].y += v.y; sum[j].z += v.z; sum[j].w += v.w;
         }
     }
+    __half* out = p.out16 + b * p.stride16;
     __half2 h[16];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        h[2 * j] = __floats2half2_rn(sum[j].x * kNsUnscale, sum[j].y * kNsUnscale);
-        h[2 * j + 1] = __floats2half2_rn(sum[j].z * kNsUnscale, sum[j].w * kNsUnscale);
+        sum[j].x *= kNsUnscale; sum[j].y *= kNsUnscale; sum[j].z *= kNsUnscale; sum[j].w *= kNsUnscale;
+        h[2 * j] = __floats2half2_rn(sum[j].x, sum[j].y);
+        h[2 * j + 1] = __floats2half2_rn(sum[j].z, sum[j].w);
     }
-    ns_store_block(p, p.out16 + b * p.stride16, stage[warp], lane, row0, col0, h, row0 != col0);
+    ns_store_block(p, out, stage[warp], lane, row0, col0, h, row0 != col0);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        h[2 * j] = ns_low(sum[j].x, sum[j].y, h[2 * j]);
+        h[2 * j + 1] = ns_low(sum[j].z, sum[j].w, h[2 * j + 1]);
+    }
+    ns_store_block(p, out + p.low16, stage[warp], lane, row0, col0, h, row0 != col0);
 }
 
 // ---- Frobenius norm and first state ---------------------------------------------------------------------------
@@ -717,18 +775,21 @@ ns_start_kernel(const T* g, float* X32, __half* X16, const double* partial, int 
         load(following, next_v);
         int64_t r, c;
         if (inside(it, r, c)) {
-            uint32_t h[4];
+            uint32_t h[4], l[4];
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = v[i] * pre / div * kNsScale;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const __half2 two = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                const __half2 two = __floats2half2_rn(v[2 * i], v[2 * i + 1]), rest = ns_low(v[2 * i], v[2 * i + 1], two);
                 h[i] = *reinterpret_cast<const uint32_t*>(&two);
+                l[i] = *reinterpret_cast<const uint32_t*>(&rest);
             }
             float4* xp = reinterpret_cast<float4*>(X32 + b * stridex + ns_state_at(r, c, ldx));
             xp[0] = make_float4(v[0], v[1], v[2], v[3]);
             xp[32] = make_float4(v[4], v[5], v[6], v[7]);
-            *reinterpret_cast<uint4*>(X16 + (b * rows + r) * ldx + c) = make_uint4(h[0], h[1], h[2], h[3]);  // padded rows: whole groups
+            // padded rows: whole groups; the low parts behind all matrices' high parts
+            *reinterpret_cast<uint4*>(X16 + (b * rows + r) * ldx + c) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(X16 + ((gridDim.y + b) * rows + r) * ldx + c) = make_uint4(l[0], l[1], l[2], l[3]);
         }
         it = following;
 #pragma unroll
@@ -737,13 +798,14 @@ ns_start_kernel(const T* g, float* X32, __half* X16, const double* partial, int 
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------
-// Three tile sizes. A k block of 64 takes a pair of CTAs 565 cycles on its 256 x 256 tile, a CTA 455 on 128 x 128 (bound
-// by shared memory, which holds both operands) and 390 on 128 x 64. Between two tiles of a CTA the epilogue of the
-// first slows the second down (by about half its own length when it is X's, which moves ten bytes an entry); the last
+// Three tile sizes, and what a k block of 64 and an epilogue cost relative to each other (cycles where the high parts
+// are multiplied alone; with all three terms a block takes 1.0 us, 0.6 and 0.5, the first bound by the tensor pipe and
+// shared memory, the others by their loads at 64 bytes a cycle and SM). Between two tiles of a CTA the epilogue of the
+// first slows the second down (by about half its own length when it is X's, which moves twelve bytes an entry); the last
 // epilogue stands alone. Large products are fastest by pairs, products of few tiles by the size that gives every SM one, the
-// smallest by the tile with the shortest way (8192 x 4096: 2.4 ms by pairs, 3.4 by 128 x 128; 256 x 512: 71 us by 128 x 64,
-// 125 by 128 x 128). A = X X^T of a long X has few tiles and a long contraction: then several CTAs share a tile, at the price of
-// another kernel that adds their parts (about 6000 cycles).
+// smallest by the tile with the shortest way (by pairs, 128 x 128 and 128 x 64: 8192 x 4096 5.8, 7.1 and 12.5 ms; 2048 x 2048
+// 706, 501 and 978 us, chosen product by product 510; 256 x 512 251, 155 and 104). A = X X^T of a long X has few tiles and a
+// long contraction: then several CTAs share a tile, at the price of another kernel that adds their parts (about 6000 cycles).
 constexpr int kNsSms = 148;  // the workspace does not depend on the device
 enum { NS_PAIR = 0, NS_SINGLE = 1, NS_SMALL = 2 };
 struct NsChoice {
@@ -799,8 +861,8 @@ static int plan_ns(const nzb_orthogonalize_desc* d, NsPlan* pl) {
     pl->lda = round_up(pl->S > 0 ? pl->S : 1, kOperandKAlign);
     pl->stridex = round_up(d->rows, 32) * pl->ldx;
     pl->x32 = (size_t)round_up(d->batch * pl->stridex * 4, 256);
-    pl->x16 = (size_t)round_up(d->batch * d->rows * pl->ldx * 2, 256);
-    pl->gram = (size_t)round_up(d->batch * pl->S * pl->lda * 2, 256);
+    pl->x16 = (size_t)round_up(2 * d->batch * d->rows * pl->ldx * 2, 256);  // high and low parts
+    pl->gram = (size_t)round_up(2 * d->batch * pl->S * pl->lda * 2, 256);
     pl->diag = (size_t)round_up(d->batch * pl->S * 4, 256);
     pl->norm = (size_t)(d->batch * kNormParts * 8);
     pl->splits = d->batch > 0 && pl->S > 0 ? ns_choose(NS_GRAM, pl->S, pl->S, pl->L, d->batch).splits : 1;
@@ -854,8 +916,8 @@ struct NsOperand {
 template <class Cfg, int MODE>
 static int launch_product_of(const NsOperand& a, const NsOperand& b, NsParams& p, int64_t batch, const DeviceState& ds, cudaStream_t s) {
     CUtensorMap tmA, tmB;
-    int rc = operand(&tmA, a.base, a.mn, a.rows, a.cols, a.ld, batch, 128);
-    if (rc == NZB_OK) rc = operand(&tmB, b.base, b.mn, b.rows, b.cols, b.ld, batch, Cfg::B_ROWS);
+    int rc = operand(&tmA, a.base, a.mn, a.rows, a.cols, a.ld, 2 * batch, 128);
+    if (rc == NZB_OK) rc = operand(&tmB, b.base, b.mn, b.rows, b.cols, b.ld, 2 * batch, Cfg::B_ROWS);
     p.a_mn = a.mn;
     p.b_mn = b.mn;
     return rc == NZB_OK ? launch_product<Cfg, MODE>(tmA, tmB, p, batch, ds, s) : rc;
@@ -901,6 +963,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         p.out16 = A16;
         p.ld16 = pl.lda;
         p.stride16 = pl.S * pl.lda;
+        p.low16 = d->batch * p.stride16;
         p.partial = partial;
         p.stride_part = round_up(pl.S, 32) * pl.lda;
         const NsOperand x_k{X16[cur], false, d->rows, d->cols, pl.ldx}, x_mn{X16[cur], true, d->rows, d->cols, pl.ldx};
@@ -922,6 +985,7 @@ static int run_ns(const nzb_orthogonalize_desc* d, const NsPlan& pl, uint8_t* ws
         p.out16 = X16[cur ^ 1];
         p.ld16 = p.ldx = pl.ldx;
         p.stride16 = d->rows * pl.ldx;
+        p.low16 = d->batch * p.stride16;
         p.stridex = pl.stridex;
         p.X32 = X32;
         if (step == d->steps - 1) {

@@ -502,7 +502,8 @@ def _batch_strides(t, what):
 
 def orthogonalize(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, out=None, out_dtype=None):
     """The matrix (or batch of matrices) g with its singular values brought near 1 by Newton-Schulz products, as the
-    Muon optimizer applies them to an update. About 1e-3 off the 64-bit result whatever out_dtype (default: g's)."""
+    Muon optimizer applies them to an update; out_dtype: g's when not given. Before the rounding to out_dtype it is 1e-5 to 6e-5 off
+    the 64-bit result (Frobenius norm), up to 1e-3 for matrices of rank one, as a chain of fp32 products is."""
     device = _same_device(g, out)
     ld_g, stride_g = _batch_strides(g, "g")
     if out is None:

@@ -937,3 +937,39 @@ def test_first_call_of_a_process_within_a_capture(call):
     r = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("CALL", call)], capture_output=True, text=True, timeout=300,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---- products of 22-bit operands ------------------------------------------------------------------------------
+def _uneven_outer(rows, cols, seed):
+    """Rank one, entries whose sizes differ by orders of magnitude: a gradient of one token with outlying features."""
+    u, v = (rnd((rows,), seed) * 2).exp(), (rnd((cols,), seed + 1) * 2).exp()
+    return torch.outer(u, v * rnd((cols,), seed + 2).sign())
+
+
+def _ortho_noise(rows, cols, low_rank):
+    """Relative error: every sum of a product goes through at most 3 K / 16 + 8 additions that cut off up to 2 u (three terms,
+    sixteen elements an addition, the epilogue), three products in each of five steps. In what a matrix of low rank leaves empty the
+    noise of a step grows by 3.4445 in each later one, while the result stays near 1: 1 + 3.4445 + ... + 3.4445^4 = 198."""
+    return (198 if low_rank else 5) * 3 * (3 * max(rows, cols) / 16 + 8) * 2 * U
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 144), (144, 5), (16, 64), (64, 96), (100, 300), (300, 100), (256, 512), (512, 256), (1000, 1400),
+                                       (2331, 2103)])
+@pytest.mark.parametrize("low_rank", [False, True])
+def test_orthogonalize_keeps_what_fp32_holds(rows, cols, low_rank):
+    tol = _ortho_noise(rows, cols, low_rank)
+    if low_rank:
+        cases = [torch.outer(rnd((rows,), 150), rnd((cols,), 151)), _uneven_outer(rows, cols, 152),
+                 rnd((rows, 3), 155) @ rnd((3, cols), 156)]
+    else:
+        cases = [rnd((rows, cols), 157), _gradient_like(rows, cols, 158)]
+    for g in cases:
+        want = _ortho_ref(g)
+        assert _rel(nz.orthogonalize(g), want) <= tol
+        for out_dtype in (F16, BF16):
+            assert _rel(nz.orthogonalize(g, out_dtype=out_dtype), want) <= tol + half_step(out_dtype)
+        w, m = rnd((rows, cols), 160), torch.zeros(rows, cols, device="cuda")
+        start = w.double()
+        nz.muon_step(w, m, g, 0.5, scale=1.0, mu=0.0)
+        err = torch.linalg.norm(w.double() - (start - 0.5 * want))
+        assert err <= 0.5 * tol * torch.linalg.norm(want) + 4 * U * torch.linalg.norm(start)
