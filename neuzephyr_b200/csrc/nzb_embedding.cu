@@ -9,9 +9,10 @@
 //      rows of the tokens that do not occur: most of the bytes, and nothing they need from the sort;
 //   3. the sorted tokens are cut into chunks of 32 (8 or 16 when they are few), whatever runs of equal tokens they
 //      hold: one warp per chunk and 32 vectors of columns. A run inside a chunk goes straight to the table, what
-//      crosses a chunk's border to the workspace, so a token that makes up a tenth of the text costs no more than
-//      any other;
-//   4. the parts of the runs that cross are added in order.
+//      crosses a chunk's border to the workspace, so the rows of a token that makes up a tenth of the text are read by as
+//      many warps as any others;
+//   4. the parts of the runs that cross are added in order, a run's by one warp for each 128 columns (40000 tokens into
+//      60000 x 1024: 162 us, 288 when half of them are one token).
 // Tiles after the first add to the rows the earlier ones wrote, in launch order: the same bits every time.
 #include "nzb_internal.h"
 #include "nzb_elem.cuh"
