@@ -4,7 +4,7 @@
 // With z = scale x over a row: lse = ln sum exp z, logprob = z_t - lse, H = lse - sum p z. Everything is in powers of
 // two, k = scale log2(e). One walk over the row: every thread keeps its largest logit m, s = sum e and w = sum e u with
 // u = (x - m) k and e = 2^u; when m grows by d / k, u falls by d: w = f (w - d s), s = f s with f = 2^-d. Two such
-// triples join the same way, so log2 s and H = (log2 s - w / s) ln 2 need no second walk and cancel nothing (w <= 0).
+// triples join the same way, so ln s and H = ln s - (w / s) ln 2 need no second walk and cancel nothing (w <= 0).
 // Logits are read as no less than -2^27, so that a masked one (-inf, -1e9, the type's lowest) has e = 0 and e u = 0.
 #include <cooperative_groups.h>
 
@@ -430,20 +430,20 @@ token_logprob_kernel(const T* __restrict__ logits, const Index* __restrict__ tar
     __syncthreads();
     const RowSums all = cta_sums;
     const bool empty = all.top <= kEmpty && all.s == all.s;
-    const float log_s = log2f(all.s);
+    const float ln_s = logf(all.s);  // not log2f times ln 2: two more roundings, the first in a coarser place
     if (t == 0) {
-        if (lse_out) lse_out[r] = empty ? -INFINITY : fmaf(all.top, scale, log_s * kLn2);
+        if (lse_out) lse_out[r] = empty ? -INFINITY : fmaf(all.top, scale, ln_s);
         // a sum w of NaN beside a finite s: a logit so large (above 2^126) that u left fp32's range. Then every e is 0 or 1
-        if (entropy) entropy[r] = empty ? 0.f : (log_s - (all.w == all.w || all.s != all.s ? all.w / all.s : 0.f)) * kLn2;
+        if (entropy) entropy[r] = empty ? 0.f : fmaf(all.w == all.w || all.s != all.s ? all.w / all.s : 0.f, -kLn2, ln_s);
         if (logprob) {
             const int64_t tgt = static_cast<int64_t>(targets[r]);
             float lp = 0.f;
-            if (tgt >= 0 && tgt < vocab) lp = empty ? -INFINITY : fmaf(Elem<T>::to(row[tgt]) - all.top, scale, -log_s * kLn2);
+            if (tgt >= 0 && tgt < vocab) lp = empty ? -INFINITY : fmaf(Elem<T>::to(row[tgt]) - all.top, scale, -ln_s);
             logprob[r] = lp;
         }
     }
     if (t < top_k) {
-        if (top_logprob) top_logprob[r * top_k + t] = empty ? -INFINITY : fmaf(top.value[t] - all.top, scale, -log_s * kLn2);
+        if (top_logprob) top_logprob[r * top_k + t] = empty ? -INFINITY : fmaf(top.value[t] - all.top, scale, -ln_s);
         if (top_index) top_index[r * top_k + t] = static_cast<Index>(top.column[t]);
     }
 }

@@ -973,3 +973,15 @@ def test_orthogonalize_keeps_what_fp32_holds(rows, cols, low_rank):
         nz.muon_step(w, m, g, 0.5, scale=1.0, mu=0.0)
         err = torch.linalg.norm(w.double() - (start - 0.5 * want))
         assert err <= 0.5 * tol * torch.linalg.norm(want) + 4 * U * torch.linalg.norm(start)
+
+
+def test_token_logprobs_are_rounded_as_few_times_as_they_need():
+    """lse = top + ln sum: the logarithm's rounding and the addition's, each spread over half a step to either side (rms a step /
+    sqrt(12)); a quarter more is allowed for the sum's own roundings and a logarithm that is off by up to a step."""
+    rows, vocab = 4096, 2999
+    x = rnd((rows, vocab), 170) * 0.3 - 2.0  # lse near 6 and ln sum near 7: steps of 2^-21
+    f = nz.token_logprobs(x, torch.zeros(rows, dtype=torch.int64, device="cuda"))
+    want = torch.logsumexp(x.double(), 1)
+    assert want.min() > 4 and want.max() < 8
+    rms = (f.lse.double() - want).square().mean().sqrt()
+    assert rms <= 1.25 * math.sqrt(2 / 12) * 2.0 ** -21
