@@ -62,10 +62,9 @@ static std::vector<double> orthogonal(const float* g, size_t r, size_t c) {
     return x;
 }
 
-// |got - (before - step * orthogonal(grad))| against the size of the update. The operands' roundings in fp16 are noise in
-// directions that a gradient of low rank leaves empty, where five steps multiply it by 3.4 each: at most 6.5e-2 of the update in a
-// simulation in 64 bits of sides from 2 to 10 and ranks from 1 on. Twice that is allowed, and two roundings of w; a scale that
-// is off by 1.6 or more is off by far more.
+// |got - (before - step * orthogonal(grad))| against the size of the update. Sums of at most 288 products go through 3 * 288 / 16 + 8
+// additions that cut off up to 2^-23, three products in each of five steps, and what a matrix of low rank leaves empty has that
+// noise multiplied by 3.4445 a step, 198 in all: 4.4e-3. Two roundings of w beside it.
 static bool updated(const std::vector<float>& got, const std::vector<float>& before, const std::vector<float>& grad, size_t batch, size_t r,
                     size_t c, double step) {
     double err = 0, size = 0, w = 0;
@@ -78,7 +77,7 @@ static bool updated(const std::vector<float>& got, const std::vector<float>& bef
             w += want * want;
         }
     }
-    return std::sqrt(err) <= 0.13 * std::sqrt(size) + 8 * U * std::sqrt(w);
+    return std::sqrt(err) <= 4.4e-3 * std::sqrt(size) + 8 * U * std::sqrt(w);
 }
 static bool descended(const std::vector<float>& got, const std::vector<float>& before, const std::vector<float>& grad, double lr) {
     for (size_t i = 0; i < got.size(); i++) {
